@@ -83,6 +83,44 @@ class AmcuEmbeddingArgs(C.Structure):
                 ("dtype", C.c_int32), ("status", C.c_void_p)]
 
 
+class AmcuSampleArgs(C.Structure):
+    _fields_ = [("logits", C.c_void_p), ("row_stride", C.c_int64), ("rows", C.c_int64), ("vocab", C.c_int64),
+                ("dtype", C.c_int32), ("uniform", C.c_void_p), ("temperature", C.c_void_p), ("top_k", C.c_void_p),
+                ("top_p", C.c_void_p), ("min_p", C.c_void_p), ("out_index", C.c_void_p), ("out_prob", C.c_void_p)]
+
+
+class AmcuKv4Cache(C.Structure):
+    _fields_ = [("k_codes", C.c_void_p), ("k_params", C.c_void_p), ("v_codes", C.c_void_p),
+                ("v_params", C.c_void_p), ("codes_page_stride", C.c_int64), ("params_page_stride", C.c_int64),
+                ("num_pages", C.c_int64), ("page_size", C.c_int64), ("n_kv_heads", C.c_int64),
+                ("head_dim", C.c_int64)]
+
+
+class AmcuKv4Batch(C.Structure):
+    _fields_ = [("page_table", C.c_void_p), ("table_stride", C.c_int64), ("max_pages", C.c_int64),
+                ("row_start", C.c_void_p), ("ctx_len", C.c_void_p), ("n_seq", C.c_int64), ("rows", C.c_int64),
+                ("status", C.c_void_p)]
+
+
+class AmcuKv4AppendArgs(C.Structure):
+    _fields_ = [("cache", AmcuKv4Cache), ("batch", AmcuKv4Batch), ("q", C.c_void_p), ("k", C.c_void_p),
+                ("v", C.c_void_p), ("q_out", C.c_void_p), ("q_stride", C.c_int64), ("k_stride", C.c_int64),
+                ("v_stride", C.c_int64), ("q_out_stride", C.c_int64), ("q_norm", C.c_void_p),
+                ("k_norm", C.c_void_p), ("eps", C.c_float), ("dtype", C.c_int32), ("cos_sin", C.c_void_p),
+                ("max_pos", C.c_int64), ("n_q_heads", C.c_int64)]
+
+
+class AmcuKv4GatherArgs(C.Structure):
+    _fields_ = [("cache", AmcuKv4Cache), ("batch", AmcuKv4Batch), ("k_out", C.c_void_p), ("v_out", C.c_void_p),
+                ("k_out_stride", C.c_int64), ("v_out_stride", C.c_int64), ("dtype", C.c_int32)]
+
+
+class AmcuKv4AttentionArgs(C.Structure):
+    _fields_ = [("cache", AmcuKv4Cache), ("batch", AmcuKv4Batch), ("q", C.c_void_p), ("q_stride", C.c_int64),
+                ("out", C.c_void_p), ("out_stride", C.c_int64), ("n_q_heads", C.c_int64), ("scale", C.c_float),
+                ("dtype", C.c_int32), ("workspace", C.c_void_p), ("workspace_size", C.c_size_t)]
+
+
 class AmConfig(C.Structure):
     _fields_ = [("device_id", C.c_int32), ("tp_rank", C.c_int32), ("tp_size", C.c_int32),
                 ("nccl_unique_id", C.c_void_p)]
@@ -151,6 +189,11 @@ _SIGS = {
     "amcu_argmax": (C.c_int, [P, C.c_int64, C.c_int64, C.c_int64, C.c_int32, P, P, P]),
     "amcu_argmax_workspace_bytes": (C.c_size_t, [C.c_int64]),
     "amcu_argmax_ws": (C.c_int, [P, C.c_int64, C.c_int64, C.c_int64, C.c_int32, P, P, P, C.c_size_t, P]),
+    "amcu_sample": (C.c_int, [C.POINTER(AmcuSampleArgs), P]),
+    "amcu_kv4_append": (C.c_int, [C.POINTER(AmcuKv4AppendArgs), P]),
+    "amcu_kv4_gather": (C.c_int, [C.POINTER(AmcuKv4GatherArgs), P]),
+    "amcu_attn_kv4_workspace_bytes": (C.c_size_t, [C.POINTER(AmcuKv4AttentionArgs)]),
+    "amcu_attn_kv4": (C.c_int, [C.POINTER(AmcuKv4AttentionArgs), P]),
     "amcu_embedding": (C.c_int, [C.POINTER(AmcuEmbeddingArgs), P]),
     "amcu_allreduce_area_bytes": (C.c_size_t, []),
     "amcu_allreduce_oneshot_add": (C.c_int, [C.POINTER(AmcuAllReduceArgs), P]),

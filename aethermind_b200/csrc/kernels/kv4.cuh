@@ -1,0 +1,85 @@
+// The 4-bit paged KV cache: addressing and argument checks shared by the
+// append, gather and attention kernels. The format is described at
+// AmcuKv4Cache in aethermind_b200.h.
+#pragma once
+#include "../amcu_internal.h"
+#include "common.cuh"
+
+namespace amcu {
+
+constexpr int kKv4Group = 64;            // elements that share a scale and a minimum
+constexpr float kKv4StepMax = 4366.f;    // largest scale: 15 steps of it stay inside fp16
+constexpr float kHalfMax = 65504.f;
+
+// What the kernels need of AmcuKv4Cache / AmcuKv4Batch, by value.
+struct Kv4View {
+    uint8_t* kc;
+    uint8_t* kp;
+    uint8_t* vc;
+    uint8_t* vp;
+    int64_t cps, pps;          // bytes between pages
+    const int32_t* table;
+    int64_t table_stride;
+    const int32_t* row_start;
+    const int32_t* ctx_len;
+    int32_t* status;
+    int32_t num_pages, max_pages;
+    int32_t n_seq, rows;
+    int32_t page_shift;        // log2 of the page size
+    int32_t nkv;
+};
+
+// First (row0) and count of sequence b's rows, kept inside [0, rows).
+__device__ __forceinline__ void kv4_rows(const Kv4View& v, int b, int& row0, int& n) {
+    int r0 = v.row_start[b], r1 = v.row_start[b + 1];
+    r0 = min(max(r0, 0), v.rows);
+    r1 = min(max(r1, r0), v.rows);
+    row0 = r0;
+    n = r1 - r0;
+}
+
+// Sequence of a row: the last b with row_start[b] <= row, found by the whole
+// warp, 32 probes at a time (one load latency for up to 32 sequences, two for
+// up to 1024). -1 where row_start does not cover the row.
+__device__ __forceinline__ int kv4_find_seq(const Kv4View& v, int row) {
+    const int lane = threadIdx.x & 31;
+    int lo = 0, n = v.n_seq;   // the answer is in [lo, lo + n) or there is none
+    while (n > 1) {
+        const int step = (n + 31) / 32;
+        const int i = lane * step;
+        const bool le = i < n && v.row_start[lo + i] <= row;
+        const unsigned m = __ballot_sync(0xffffffffu, le);
+        if (m == 0) return -1;
+        const int at = (31 - __clz(m)) * step;
+        lo += at;
+        n = min(step, n - at);
+    }
+    return v.row_start[lo] <= row && row < v.row_start[lo + 1] ? lo : -1;
+}
+
+// Page of position pos of sequence b, or -1 (and the status word) where there is none.
+__device__ __forceinline__ int kv4_page(const Kv4View& v, int b, int pos) {
+    const int i = pos >> v.page_shift;
+    int page = -1;
+    if (pos >= 0 && i < v.max_pages) page = v.table[b * v.table_stride + i];
+    if (page < 0 || page >= v.num_pages) {
+        if (v.status) *v.status = (int32_t)AM_STATUS_OUT_OF_RANGE;
+        return -1;
+    }
+    return page;
+}
+
+// Byte offsets of a head's row in the code and parameter planes.
+template <int D>
+__device__ __forceinline__ int64_t kv4_code_off(const Kv4View& v, int page, int head, int slot) {
+    return (int64_t)page * v.cps + (((int64_t)head << v.page_shift) + slot) * (D / 2);
+}
+template <int D>
+__device__ __forceinline__ int64_t kv4_param_off(const Kv4View& v, int page, int head, int slot) {
+    return (int64_t)page * v.pps + (((int64_t)head << v.page_shift) + slot) * (D / 16);
+}
+
+// Checks the cache and batch of a call and fills the view.
+am_status_code kv4_check(const char* what, const AmcuKv4Cache& c, const AmcuKv4Batch& b, Kv4View* out);
+
+}  // namespace amcu

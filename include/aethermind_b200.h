@@ -394,6 +394,134 @@ am_status_code amcu_argmax_ws(const void* logits, int64_t rows, int64_t vocab, i
                               size_t workspace_size, void* stream);
 
 /* ------------------------------------------------------------------------ */
+/* Token sampling (no counterpart in the reference, which decodes greedily). */
+/* One token per row from given uniform numbers. Per row, in this order:      */
+/*   max = largest logit (NaN counts as -inf);                                */
+/*   z_i = 0 where x_i == max, else (x_i - max) / temperature   (fp32)        */
+/*   w_i = floor(expf(z_i) * 2^40)             (whole numbers: their sums do  */
+/*         not depend on an order, so neither does the token)                 */
+/*   min-p: keep w_i >= min_p * 2^40                                          */
+/*   top-k: keep the k largest z_i                                            */
+/*   top-p: keep the shortest run of largest z_i whose mass reaches top_p of  */
+/*          what is kept so far (at least one token)                          */
+/*   token: the first i, in index order, whose running mass of kept tokens is */
+/*          above floor(uniform * kept mass).                                 */
+/* Equal z_i are taken lowest index first. temperature <= 0 is greedy;        */
+/* top_k <= 0, top_p >= 1 and min_p <= 0 are off, and so is a NULL array      */
+/* (temperature NULL: 1). A row of -inf / NaN only: token -1, probability 0.  */
+/* Any rows, strides and vocabularies up to 2^22. No workspace.               */
+/* ------------------------------------------------------------------------ */
+typedef struct AmcuSampleArgs {
+    const void* logits;         /* [rows, vocab] */
+    int64_t row_stride;         /* elements; 0 = vocab */
+    int64_t rows, vocab;
+    int32_t dtype;              /* AMCU_F32 / AMCU_BF16 */
+    const float* uniform;       /* device [rows], in [0, 1) */
+    const float* temperature;   /* device [rows] or NULL */
+    const int32_t* top_k;       /* device [rows] or NULL */
+    const float* top_p;         /* device [rows] or NULL */
+    const float* min_p;         /* device [rows] or NULL */
+    int64_t* out_index;         /* device [rows] */
+    float* out_prob;            /* device [rows] or NULL: kept-set probability of the token */
+} AmcuSampleArgs;
+am_status_code amcu_sample(const AmcuSampleArgs* args, void* stream);
+
+/* ------------------------------------------------------------------------ */
+/* Paged KV cache in 4 bits ("kv4"; no counterpart in the reference, whose    */
+/* cache is static and in the activation type). One layer's cache:            */
+/*   codes  uint8 [num_pages][n_kv][page_size][head_dim / 2]                  */
+/*   params fp16  [num_pages][n_kv][page_size][head_dim / 64][2] = (s, m)     */
+/* for K and for V; an element is m + s * code, code in [0, 15], with one     */
+/* (scale, minimum) pair per 64 elements. A row's bytes are little-endian     */
+/* 32-bit words: word j holds group j % (head_dim / 64), elements             */
+/* 8 * (j / (head_dim / 64)) + i in nibble i (bits 4i..4i+3).                 */
+/* Quantising x (fp32, per group): m = fp16(min x), s = fp16(min((max x -     */
+/* min x) / 15, 4366)), code = clamp(rint((x - m) / s), 0, 15); s = 0: code   */
+/* 0. m saturates at +-65504; NaN elements are left out of min and max and    */
+/* stored as code 0.                                                          */
+/* ------------------------------------------------------------------------ */
+typedef struct AmcuKv4Cache {
+    void* k_codes;
+    void* k_params;
+    void* v_codes;
+    void* v_params;
+    int64_t codes_page_stride;   /* bytes between pages, multiple of 16; 0 = n_kv * page_size * head_dim / 2 */
+    int64_t params_page_stride;  /* bytes between pages, multiple of 16; 0 = n_kv * page_size * head_dim / 16 */
+    int64_t num_pages;
+    int64_t page_size;           /* tokens per page: 16, 32, 64, 128 or 256 */
+    int64_t n_kv_heads;
+    int64_t head_dim;            /* 64 or 128 */
+} AmcuKv4Cache;
+/* The sequences of a call. Sequence b's new rows are rows row_start[b] ..
+ * row_start[b + 1] - 1 of the call (any number, also none); ctx_len[b] counts
+ * its tokens WITH them, so row r of n is at position ctx_len[b] - n + r.
+ * page_table[b][p / page_size] names position p's page. row_start is
+ * non-decreasing from 0 to `rows`. A position below 0 or past the page table,
+ * or a page outside [0, num_pages), is never read or written; where a row or
+ * key needed it, *status (device, optional) becomes AM_STATUS_OUT_OF_RANGE. */
+typedef struct AmcuKv4Batch {
+    const int32_t* page_table;   /* device [n_seq][max_pages] */
+    int64_t table_stride;        /* elements; 0 = max_pages */
+    int64_t max_pages;
+    const int32_t* row_start;    /* device [n_seq + 1] */
+    const int32_t* ctx_len;      /* device [n_seq] */
+    int64_t n_seq;
+    int64_t rows;                /* rows of the call */
+    int32_t* status;
+} AmcuKv4Batch;
+/* New rows into the cache: per head, q and k are RMS-normalised over head_dim
+ * (where a weight is given), rotated (split halves, fp32 products rounded one
+ * by one as in amcu_rope_kv_write), q is rounded once to q_out, and k and v
+ * are quantised from fp32 into their pages. */
+typedef struct AmcuKv4AppendArgs {
+    AmcuKv4Cache cache;
+    AmcuKv4Batch batch;
+    const void* q;               /* [rows, n_q_heads * head_dim] */
+    const void* k;               /* [rows, n_kv_heads * head_dim] */
+    const void* v;
+    void* q_out;                 /* [rows, n_q_heads * head_dim]; may be q */
+    int64_t q_stride, k_stride, v_stride, q_out_stride;   /* elements, even */
+    const void* q_norm;          /* [head_dim] or NULL */
+    const void* k_norm;          /* [head_dim] or NULL */
+    float eps;
+    int32_t dtype;               /* AMCU_F32 / AMCU_BF16: q, k, v, q_out and the norm weights */
+    const float* cos_sin;        /* amcu_rope_table's [max_pos][head_dim / 2] (cos, sin) */
+    int64_t max_pos;             /* positions in cos_sin; a row at or past it is out of range */
+    int64_t n_q_heads;
+} AmcuKv4AppendArgs;
+am_status_code amcu_kv4_append(const AmcuKv4AppendArgs* args, void* stream);
+/* Reads the call's rows back from the cache as the values they stand for
+ * (row_start over whole sequences exports them). Rows out of range are zero. */
+typedef struct AmcuKv4GatherArgs {
+    AmcuKv4Cache cache;
+    AmcuKv4Batch batch;
+    void* k_out;                 /* [rows, n_kv_heads * head_dim] */
+    void* v_out;
+    int64_t k_out_stride, v_out_stride;   /* elements, multiples of 8 */
+    int32_t dtype;               /* AMCU_F32 / AMCU_BF16 */
+} AmcuKv4GatherArgs;
+am_status_code amcu_kv4_gather(const AmcuKv4GatherArgs* args, void* stream);
+/* Causal GQA attention of the call's rows over the cache, which already holds
+ * them: out = sum_j softmax_j(scale * q . k_j) v_j over positions j up to the
+ * row's own. Rows that see no key are zero. Any mixture of single tokens and
+ * prompts; n_q_heads a multiple of n_kv_heads. */
+typedef struct AmcuKv4AttentionArgs {
+    AmcuKv4Cache cache;
+    AmcuKv4Batch batch;
+    const void* q;               /* [rows, n_q_heads * head_dim], rotated */
+    int64_t q_stride;            /* elements */
+    void* out;                   /* [rows, n_q_heads * head_dim] */
+    int64_t out_stride;          /* elements */
+    int64_t n_q_heads;
+    float scale;                 /* 0: 1 / sqrt(head_dim) */
+    int32_t dtype;               /* AMCU_F32 / AMCU_BF16: q and out */
+    void* workspace;             /* device, amcu_attn_kv4_workspace_bytes, 16-byte aligned */
+    size_t workspace_size;
+} AmcuKv4AttentionArgs;
+size_t amcu_attn_kv4_workspace_bytes(const AmcuKv4AttentionArgs* args);
+am_status_code amcu_attn_kv4(const AmcuKv4AttentionArgs* args, void* stream);
+
+/* ------------------------------------------------------------------------ */
 /* Embedding gather (src/backend/cpu/kernels/embedding/embedding_entry.cpp:  */
 /* 32-126). ids: int32/int64/uint32 [count]. table: act-dtype [vocab, hidden] */
 /* or INT8 rows + fp32 row scales (tied int8 lm_head), dequantized to bf16.  */
