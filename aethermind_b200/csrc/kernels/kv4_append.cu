@@ -3,9 +3,9 @@
 // Append, per row and head: q and k are scaled by w / sqrt(mean(x^2) + eps)
 // where a weight is given, rotated (out[i] = a_i c - b_i s, out[i + d/2] =
 // b_i c + a_i s; a, b the halves), q is rounded once to its type, k and v are
-// quantised per 64 elements from fp32: m = fp16(min), s = fp16((max - min) /
-// 15), code = rint((x - m) / s). Products and sums of the rotation are rounded
-// one by one (no fused multiply-add) and the divisions are IEEE ones, so the
+// quantised per 64 elements from fp32: m = fp16(min), s = fp16((max - min) *
+// (1/15)), code = rint((x - m) / s). Products and sums of the rotation are rounded
+// one by one (no fused multiply-add) and (x - m) / s is an IEEE division, so the
 // codes are those of the written expressions.
 #include "kv4.cuh"
 
@@ -83,12 +83,6 @@ __device__ __forceinline__ void kv4_st2(__nv_bfloat16* p, float a, float b) {
 
 // Reduction over the LPH lanes that hold one head.
 template <int LPH>
-__device__ __forceinline__ float head_sum(float v) {
-#pragma unroll
-    for (int o = LPH / 2; o > 0; o >>= 1) v += __shfl_xor_sync(0xffffffffu, v, o);
-    return v;
-}
-template <int LPH>
 __device__ __forceinline__ float head_min(float v) {
 #pragma unroll
     for (int o = LPH / 2; o > 0; o >>= 1) v = fminf(v, __shfl_xor_sync(0xffffffffu, v, o));
@@ -138,9 +132,30 @@ __global__ void __launch_bounds__(128) kv4_append_kernel(Kv4AppendParams p) {
         y = kv4_ld2<T>(src + half + 2 * l);
     }
     const T* nw = static_cast<const T*>(is_q ? p.qw : is_k ? p.kw : nullptr);
-    const float ss = head_sum<LPH>(x.x * x.x + x.y * x.y + y.x * y.x + y.y * y.y);
+    // Sum of squares in a fixed order, each addition rounded by itself: halves
+    // onto each other down to one element (d = 64), or to runs of four
+    // neighbours that are added first (d = 128).
+    float2 q0 = make_float2(__fmul_rn(x.x, x.x), __fmul_rn(x.y, x.y)), q1 = make_float2(__fmul_rn(y.x, y.x), __fmul_rn(y.y, y.y));
+    float ss;
+    if (D == 128) {
+        const float2 o0 = make_float2(__shfl_xor_sync(0xffffffffu, q0.x, 1), __shfl_xor_sync(0xffffffffu, q0.y, 1));
+        const float2 o1 = make_float2(__shfl_xor_sync(0xffffffffu, q1.x, 1), __shfl_xor_sync(0xffffffffu, q1.y, 1));
+        const bool odd = l & 1;
+        const float a = __fadd_rn(__fadd_rn(odd ? __fadd_rn(o0.x, o0.y) : __fadd_rn(q0.x, q0.y), odd ? q0.x : o0.x), odd ? q0.y : o0.y);
+        const float c = __fadd_rn(__fadd_rn(odd ? __fadd_rn(o1.x, o1.y) : __fadd_rn(q1.x, q1.y), odd ? q1.x : o1.x), odd ? q1.y : o1.y);
+        ss = __fadd_rn(a, c);
+#pragma unroll
+        for (int o = 16; o > 1; o >>= 1) ss = __fadd_rn(ss, __shfl_xor_sync(0xffffffffu, ss, o));
+    } else {
+        q0 = make_float2(__fadd_rn(q0.x, q1.x), __fadd_rn(q0.y, q1.y));
+#pragma unroll
+        for (int o = 8; o > 0; o >>= 1)
+            q0 = make_float2(__fadd_rn(q0.x, __shfl_xor_sync(0xffffffffu, q0.x, o)),
+                             __fadd_rn(q0.y, __shfl_xor_sync(0xffffffffu, q0.y, o)));
+        ss = __fadd_rn(q0.x, q0.y);
+    }
     if (nw) {
-        const float r = __frsqrt_rn(ss / (float)D + p.eps);
+        const float r = rsqrtf(__fadd_rn(ss / (float)D, p.eps));
         const float2 wa = kv4_ld2<T>(nw + 2 * l), wb = kv4_ld2<T>(nw + half + 2 * l);
         x = make_float2(x.x * r * wa.x, x.y * r * wa.y);
         y = make_float2(y.x * r * wb.x, y.y * r * wb.y);
@@ -181,8 +196,8 @@ __global__ void __launch_bounds__(128) kv4_append_kernel(Kv4AppendParams p) {
     uint8_t* params = (is_k ? p.v.kp : p.v.vp) + kv4_param_off<D>(p.v, page, kvh, slot);
     const __half m0 = __float2half_rn(fminf(fmaxf(lo0, -kHalfMax), kHalfMax));
     const __half m1 = __float2half_rn(fminf(fmaxf(lo1, -kHalfMax), kHalfMax));
-    const __half s0 = __float2half_rn(fminf(__fdiv_rn(__fsub_rn(hi0, lo0), 15.f), kKv4StepMax));
-    const __half s1 = __float2half_rn(fminf(__fdiv_rn(__fsub_rn(hi1, lo1), 15.f), kKv4StepMax));
+    const __half s0 = __float2half_rn(fminf(__fmul_rn(__fsub_rn(hi0, lo0), 1.f / 15.f), kKv4StepMax));
+    const __half s1 = __float2half_rn(fminf(__fmul_rn(__fsub_rn(hi1, lo1), 1.f / 15.f), kKv4StepMax));
     const float fm0 = __half2float(m0), fm1 = __half2float(m1), fs0 = __half2float(s0), fs1 = __half2float(s1);
     const uint8_t b0 = (uint8_t)(kv4_code(x.x, fs0, fm0) | (kv4_code(x.y, fs0, fm0) << 4));
     const uint8_t b1 = (uint8_t)(kv4_code(y.x, fs1, fm1) | (kv4_code(y.y, fs1, fm1) << 4));

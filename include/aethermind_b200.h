@@ -436,8 +436,8 @@ am_status_code amcu_sample(const AmcuSampleArgs* args, void* stream);
 /* 32-bit words: word j holds group j % (head_dim / 64), elements             */
 /* 8 * (j / (head_dim / 64)) + i in nibble i (bits 4i..4i+3).                 */
 /* Quantising x (fp32, per group): m = fp16(min x), s = fp16(min((max x -     */
-/* min x) / 15, 4366)), code = clamp(rint((x - m) / s), 0, 15); s = 0: code   */
-/* 0. m saturates at +-65504; NaN elements are left out of min and max and    */
+/* min x) * fp32(1/15), 4366)), code = clamp(rint((x - m) / s), 0, 15); s = 0 */
+/* gives code 0. m saturates at +-65504; NaN elements are left out of min and max and    */
 /* stored as code 0.                                                          */
 /* ------------------------------------------------------------------------ */
 typedef struct AmcuKv4Cache {

@@ -39,7 +39,7 @@ def quantise(x):
     g = x.reshape(x.shape[:-1] + (-1, GROUP))
     lo, hi = g.min(-1), g.max(-1)
     m = np.clip(lo, -HALF_MAX, HALF_MAX).astype(np.float16)
-    s = np.minimum((hi - lo) / x.dtype.type(15), x.dtype.type(STEP_MAX)).astype(np.float16)
+    s = np.minimum((hi - lo) * x.dtype.type(np.float32(1) / np.float32(15)), x.dtype.type(STEP_MAX)).astype(np.float16)
     sf, mf = s.astype(x.dtype)[..., None], m.astype(x.dtype)[..., None]
     with np.errstate(divide="ignore", invalid="ignore"):
         c = np.where(sf > 0, np.clip(np.rint((g - mf) / sf), 0, 15), 0)
