@@ -19,7 +19,8 @@ am_status_code kv4_check(const char* what, const AmcuKv4Cache& c, const AmcuKv4B
     AMCU_REQUIRE(c.num_pages > 0 && c.num_pages <= INT32_MAX, "%s: num_pages must be positive", what);
     AMCU_REQUIRE(b.rows >= 0 && b.rows <= (1 << 24) && b.n_seq >= 0 && b.n_seq <= (1 << 24),
                  "%s: rows and n_seq must be in [0, 2^24]", what);
-    AMCU_REQUIRE(b.max_pages >= 0 && b.max_pages <= (INT32_MAX >> 8), "%s: bad max_pages", what);
+    AMCU_REQUIRE(b.max_pages >= 0 && b.max_pages <= (1 << 30) / c.page_size,
+                 "%s: max_pages must be in [0, 2^30 / page_size]", what);
     const int64_t codes = c.n_kv_heads * c.page_size * c.head_dim / 2, params = codes / 8;
     AMCU_REQUIRE(c.codes_page_stride == 0 || (c.codes_page_stride >= codes && c.codes_page_stride % 16 == 0),
                  "%s: codes_page_stride must be a multiple of 16 and hold a page", what);

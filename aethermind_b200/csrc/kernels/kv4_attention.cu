@@ -3,6 +3,7 @@
 // out[row, h] = sum_j p_j v_j / sum_j p_j, p_j = exp(scale q . k_j - max), over
 // the positions j <= pos of the row's sequence; k_j = m + s * code.
 #include "kv4.cuh"
+#include "mma_int4.cuh"
 
 namespace amcu {
 
@@ -15,72 +16,642 @@ struct Kv4AttnParams {
     float scale;
 };
 
-// One warp per (row, q head): 32 keys at a time, one per lane, then the
-// output's elements are shared out over the lanes.
+// ---------------------------------------------------------------------------
+// Single tokens and short runs of rows.
+//
+// The columns of a product are (row, q head) pairs of one kv head, 8 to a tile
+// (fp32: 4, each as a high and a low fp16 half in neighbouring columns), the
+// rows are keys: S^T = K Q^T and O^T = V^T P^T with mma.sync m16n8k16, so the
+// big operand needs no padding whatever the group size. The work is cut in
+// units of 16 keys of one (sequence, kv head, column tile); the units of the
+// whole call lie in one row, and every CTA takes an equal, contiguous share
+// of them (found from row_start and ctx_len on the device), so ragged batches
+// and single long sequences fill the GPU alike. A CTA's 8 warps take its units
+// in turn, each through a cp.async ring of its own. An item cut between CTAs
+// leaves partial sums that kv4_combine_kernel adds in the order of the CTAs.
+//
+// Codes enter the MMA without any conversion: a nibble in bits 0-3 of a half
+// is the fp16 subnormal c * 2^-24, one in bits 4-7 is c * 2^-20. q is scaled
+// by a power of two to [1, 2) and its elements at the low nibbles by 16 more,
+// which makes the integer dot product exact up to fp32 sums; scale and minimum
+// of a key's group are applied to the 64-element sums (m through sum(q)).
+// For V the contraction runs over keys, so c * s is formed before the product:
+// (1024 + c) s - 1024 s in one fp16x2 FMA, rounded once to 11 bits (fp32: the
+// rounding's remainder in a second product). The minima and the softmax
+// denominator are three more rows of the same product.
+constexpr int kDecWarps = 8;
+constexpr int kDecThreads = kDecWarps * 32;
+constexpr int kDecStages = 5;
+constexpr int kDecUnit = 16;       // keys per unit
+constexpr int kDecMinUnits = 8;    // units of a CTA at least: one for each warp
+constexpr float kLog2e = 1.4426950408889634f;
+constexpr float kDecLift = 3.f;    // p stays below 2^3 before its reference moves
+
+template <typename T> constexpr int dec_cols() { return sizeof(T) == 2 ? 8 : 4; }  // (row, head) pairs per tile
+template <int D> constexpr int dec_stage_bytes() { return 2 * kDecUnit * (D / 2 + D / 16) + 16; }
+template <int D> constexpr int dec_merge_stride() { return D + 4; }
+template <int D> constexpr int dec_merge_bytes() { return kDecWarps * 8 * (dec_merge_stride<D>() + 4) * 4; }
+template <int D> constexpr int dec_smem_bytes() {
+    const int ring = kDecWarps * kDecStages * dec_stage_bytes<D>();
+    return ring > dec_merge_bytes<D>() ? ring : dec_merge_bytes<D>();
+}
+
+struct DecMeta {   // for the CTA that holds an item's last unit but not its first
+    int32_t first;   // CTA of the first unit; -1: nothing to combine
+    int32_t b, kvh, ct;
+};
+struct DecWork {
+    float2* ml;    // [CTA][2][8] (reference, denominator)
+    float* o;      // [CTA][2][8][D]
+    DecMeta* meta; // [CTA]
+};
+
+__device__ __forceinline__ void cp16(uint32_t dst, const void* src, uint32_t bytes) {
+    asm volatile("cp.async.cg.shared.global [%0], [%1], 16, %2;" ::"r"(dst), "l"(src), "r"(bytes) : "memory");
+}
+__device__ __forceinline__ uint32_t movm_trans(uint32_t v) {
+    uint32_t r;
+    asm volatile("movmatrix.sync.aligned.m8n8.trans.b16 %0, %1;" : "=r"(r) : "r"(v));
+    return r;
+}
+__device__ __forceinline__ float ex2(float x) {
+    float r;
+    asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(r) : "f"(x));
+    return r;
+}
+__device__ __forceinline__ uint32_t h2u(__half2 h) { return *reinterpret_cast<uint32_t*>(&h); }
+__device__ __forceinline__ __half2 u2h(uint32_t u) { return *reinterpret_cast<__half2*>(&u); }
+
+// 16-byte chunk of a stage that holds chunk c of token tk: the rows of a
+// 128-byte line are XOR-swizzled so that a K read (8 bytes or 16 of 4 or 2
+// neighbouring tokens) and a V read (every second token) both touch every
+// bank once.
+template <int D>
+__device__ __forceinline__ int dec_chunk(int tk, int c) {
+    return D == 128 ? (tk >> 1) * 8 + ((((tk & 1) << 2) + c) ^ (((tk >> 1) & 3) << 1))
+                    : (tk >> 2) * 8 + ((((tk & 3) << 1) + c) ^ (((tk >> 2) & 1) << 1));
+}
+
+// Cost of sequence b in units, and what a segment needs of it.
+struct DecSeq {
+    int row0, n, ctx, units, tiles;
+};
+template <typename T>
+__device__ __forceinline__ DecSeq dec_seq(const Kv4View& v, int grp, int b) {
+    DecSeq s;
+    kv4_rows(v, b, s.row0, s.n);
+    s.ctx = v.ctx_len[b];
+    const int64_t cap = (int64_t)v.max_pages << v.page_shift;
+    const int vis = (int)min((int64_t)max(s.ctx, 0), cap);
+    s.units = max((vis + kDecUnit - 1) / kDecUnit, 1);
+    s.tiles = (int)(((int64_t)s.n * grp + dec_cols<T>() - 1) / dec_cols<T>());
+    return s;
+}
+
 template <typename T, int D>
-__global__ void __launch_bounds__(128) kv4_attn_simple_kernel(Kv4AttnParams p) {
-    constexpr int G = D / kKv4Group, EPL = D / 32;
-    __shared__ float qs[4][D];
+__global__ void __launch_bounds__(kDecThreads, 2) kv4_decode_kernel(Kv4AttnParams p, DecWork ws) {
+    constexpr int G = D / kKv4Group, CT = dec_cols<T>();
+    constexpr bool kWide = sizeof(T) == 4;  // fp32: two halves per value
+    constexpr int kCodes = kDecUnit * D / 2, kParams = kDecUnit * D / 16;
+    constexpr int kStage = dec_stage_bytes<D>(), S = kDecStages;
+    constexpr int kMS = dec_merge_stride<D>();
+    extern __shared__ __align__(128) uint8_t smem[];
+    __shared__ int64_t scan_part[kDecWarps];
+    __shared__ int64_t s_off;
+    __shared__ int s_b;
+
+    const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31, r = lane >> 2, t = lane & 3;
     pdl_wait();
     pdl_trigger();
-    const int lane = threadIdx.x & 31, wi = threadIdx.x >> 5;
-    const int64_t w = (int64_t)blockIdx.x * 4 + wi;
-    if (w >= (int64_t)p.v.rows * p.nq) return;
-    const int row = (int)(w / p.nq), h = (int)(w % p.nq), kvh = h / p.grp;
-    const int b = kv4_find_seq(p.v, row);
-    if (b < 0) return;
-    const int pos = p.v.ctx_len[b] - p.v.row_start[b + 1] + row;
-    const T* q = static_cast<const T*>(p.q) + row * p.qs + (int64_t)h * D;
-    for (int e = lane; e < D; e += 32) qs[wi][e] = Act<T>::load(q[e]) * p.scale;
-    __syncwarp();
-    float mx = -INFINITY, sum = 0.f, acc[EPL] = {};
-    for (int k0 = 0; k0 <= pos; k0 += 32) {
-        const int key = k0 + lane;
-        int page = -1;
-        int64_t co = 0, po = 0;
-        float s = -INFINITY;
-        if (key <= pos) page = kv4_page(p.v, b, key);
-        if (page >= 0) {
-            const int slot = key & ((1 << p.v.page_shift) - 1);
-            co = kv4_code_off<D>(p.v, page, kvh, slot);
-            po = kv4_param_off<D>(p.v, page, kvh, slot);
-            s = 0.f;
-            for (int word = 0; word < D / 8; ++word) {
-                const uint32_t c = *reinterpret_cast<const uint32_t*>(p.v.kc + co + 4 * word);
-                const float2 sm = __half22float2(*reinterpret_cast<const __half2*>(p.v.kp + po + 4 * (word % G)));
-                const float* qe = &qs[wi][(word % G) * kKv4Group + (word / G) * 8];
-                for (int i = 0; i < 8; ++i) s += qe[i] * ((float)((c >> (4 * i)) & 15u) * sm.x + sm.y);
+
+    // ---- this CTA's share [x, x_end) of all units
+    const Kv4View& v = p.v;
+    const int chunk = (v.n_seq + kDecThreads - 1) / kDecThreads;
+    const int b_lo = threadIdx.x * chunk, b_hi = min(b_lo + chunk, v.n_seq);
+    int64_t mine = 0;
+    for (int b = b_lo; b < b_hi; ++b) {
+        const DecSeq s = dec_seq<T>(v, p.grp, b);
+        mine += (int64_t)s.units * s.tiles * v.nkv;
+    }
+    int64_t incl = mine;
+#pragma unroll
+    for (int o = 1; o < 32; o <<= 1) {
+        const int64_t y = __shfl_up_sync(0xffffffffu, incl, o);
+        if (lane >= o) incl += y;
+    }
+    if (lane == 31) scan_part[warp] = incl;
+    __syncthreads();
+    int64_t base = 0, total = 0;
+#pragma unroll
+    for (int w = 0; w < kDecWarps; ++w) {
+        if (w < warp) base += scan_part[w];
+        total += scan_part[w];
+    }
+    int64_t share = (total + gridDim.x - 1) / gridDim.x;
+    if (share < kDecMinUnits) share = kDecMinUnits;
+    int64_t x = blockIdx.x * share;
+    const int64_t x_end = min(x + share, total);
+    if (threadIdx.x == 0) ws.meta[blockIdx.x].first = -1;
+    if (x >= x_end) return;
+    {
+        const int64_t ex = base + incl - mine;
+        if (x >= ex && x < ex + mine) {  // exactly one thread
+            int64_t off = x - ex;
+            int b = b_lo;
+            for (;; ++b) {
+                const DecSeq s = dec_seq<T>(v, p.grp, b);
+                const int64_t cost = (int64_t)s.units * s.tiles * v.nkv;
+                if (off < cost) break;
+                off -= cost;
             }
-        }
-        const float nm = fmaxf(mx, warp_max(s));
-        const float corr = nm == -INFINITY ? 1.f : expf(mx - nm);
-        const float pr = page >= 0 ? expf(s - nm) : 0.f;
-        sum = sum * corr + warp_sum(pr);
-        mx = nm;
-        for (int i = 0; i < EPL; ++i) acc[i] *= corr;
-        for (int j = 0; j < 32; ++j) {
-            const float pj = __shfl_sync(0xffffffffu, pr, j);
-            const int64_t cj = __shfl_sync(0xffffffffu, co, j), pj_off = __shfl_sync(0xffffffffu, po, j);
-            if (!__shfl_sync(0xffffffffu, (int)(page >= 0), j)) continue;
-            for (int i = 0; i < EPL; ++i) {
-                const int e = i * 32 + lane, g = e / kKv4Group, r = e % kKv4Group;
-                const uint8_t c = p.v.vc[cj + 4 * ((r / 8) * G + g) + (r % 8) / 2];
-                const float2 sm = __half22float2(*reinterpret_cast<const __half2*>(p.v.vp + pj_off + 4 * g));
-                acc[i] += pj * ((float)((c >> (4 * (r & 1))) & 15) * sm.x + sm.y);
-            }
+            s_b = b;
+            s_off = off;
         }
     }
-    T* o = static_cast<T*>(p.out) + row * p.os + (int64_t)h * D;
-    for (int i = 0; i < EPL; ++i) o[i * 32 + lane] = Act<T>::store(sum > 0.f ? acc[i] / sum : 0.f);
+    __syncthreads();
+    int b = s_b;
+    int64_t off = s_off;
+    const uint32_t ring = smem_u32(smem) + warp * (S * kStage);
+    const uint8_t* ring_p = smem + warp * (S * kStage);
+    const int page_units_shift = v.page_shift - 4;
+
+    while (x < x_end) {
+        const DecSeq sq = dec_seq<T>(v, p.grp, b);
+        const int64_t cost = (int64_t)sq.units * sq.tiles * v.nkv;
+        if (off >= cost) {
+            off -= cost;
+            ++b;
+            continue;
+        }
+        const int item = (int)(off / sq.units), u0 = (int)(off - (int64_t)item * sq.units);
+        const int kvh = item / sq.tiles, ct = item - kvh * sq.tiles;
+        const int u1 = (int)min((int64_t)sq.units, u0 + (x_end - x));
+        const int cap = (int)min((int64_t)max(sq.ctx, 0), (int64_t)v.max_pages << v.page_shift);  // keys that can exist
+        const int cols = min(CT, sq.n * p.grp - ct * CT);
+        if (sq.ctx > cap && v.status && threadIdx.x == 0) *v.status = (int32_t)AM_STATUS_OUT_OF_RANGE;
+
+        // ---- the tile's columns: this lane's is r (MMA operand), its results are of columns 2t, 2t + 1
+        const int c_op = kWide ? r >> 1 : r;
+        const bool c_live = c_op < cols;
+        const int fc = ct * CT + (c_live ? c_op : 0);
+        const int c_row = fc / p.grp, c_head = kvh * p.grp + fc - c_row * p.grp;
+        const T* qp = static_cast<const T*>(p.q) + (int64_t)(sq.row0 + c_row) * p.qs + (int64_t)c_head * D + 16 * t;
+        float qv[G][16];
+#pragma unroll
+        for (int g = 0; g < G; ++g)
+#pragma unroll
+            for (int i = 0; i < 16; ++i) qv[g][i] = c_live ? Act<T>::load(qp[g * kKv4Group + i]) : 0.f;
+        float amax = 0.f, qsum[G];
+#pragma unroll
+        for (int g = 0; g < G; ++g) {
+            qsum[g] = 0.f;
+#pragma unroll
+            for (int i = 0; i < 16; ++i) {
+                amax = fmaxf(amax, fabsf(qv[g][i]));
+                qsum[g] += qv[g][i];
+            }
+            qsum[g] += __shfl_xor_sync(0xffffffffu, qsum[g], 1);
+            qsum[g] += __shfl_xor_sync(0xffffffffu, qsum[g], 2);
+        }
+        amax = fmaxf(amax, __shfl_xor_sync(0xffffffffu, amax, 1));
+        amax = fmaxf(amax, __shfl_xor_sync(0xffffffffu, amax, 2));
+        const uint32_t eb = min(max(__float_as_uint(amax) >> 23, 1u), 253u);
+        const float inv = __uint_as_float((254u - eb) << 23);
+        uint32_t qf[2 * G][2][2];  // [word][half of the word][b0, b1]
+#pragma unroll
+        for (int j = 0; j < 2 * G; ++j)
+#pragma unroll
+            for (int hh = 0; hh < 2; ++hh)
+#pragma unroll
+                for (int e = 0; e < 2; ++e) {  // nibbles 2 hh + e and 2 hh + e + 4
+                    const int i = 8 * (j / G) + 2 * hh + e;
+                    float a = qv[j % G][i] * inv, c = qv[j % G][i + 4] * inv;
+                    if (kWide) {
+                        const float ah = __half2float(__float2half_rn(a)), ch = __half2float(__float2half_rn(c));
+                        a = (r & 1) ? a - ah : ah;
+                        c = (r & 1) ? c - ch : ch;
+                    }
+                    const float lift = e == 0 ? 16.f : 1.f;
+                    qf[j][hh][e] = h2u(__floats2half2_rn(a * lift, c * lift));
+                }
+        // results: factor of the integer sums, sum(q) per group, last visible position
+        const float sl = p.scale * kLog2e;
+        const float f_op = __uint_as_float(eb << 23) * sl * 1048576.f;
+        const int lim_op = c_live ? min(sq.ctx - sq.n + c_row, cap - 1) : -1;
+        float f[2], qg[G][2];
+        int lim[2];
+#pragma unroll
+        for (int j = 0; j < 2; ++j) {
+            const int src = kWide ? 8 * t : 8 * t + 4 * j;
+            f[j] = __shfl_sync(0xffffffffu, f_op, src);
+            lim[j] = __shfl_sync(0xffffffffu, lim_op, src);
+#pragma unroll
+            for (int g = 0; g < G; ++g) qg[g][j] = __shfl_sync(0xffffffffu, qsum[g] * sl, src);
+        }
+        // keys past the last column's limit need no unit; before the first one's, no mask
+        const int lim_last = __shfl_sync(0xffffffffu, lim_op, kWide ? 8 * (cols - 1) : 4 * (cols - 1));
+        const int lim_first = __shfl_sync(0xffffffffu, lim_op, 0);
+        const int u_end = min(u1, (lim_last + kDecUnit) / kDecUnit);  // lim_last = -1: none
+        const int full = (lim_first + 1) / kDecUnit;  // units before it need no mask
+
+        // ---- ring: unit k of this warp is u0 + warp + 8 k
+        const int nk = u_end > u0 + warp ? (u_end - u0 - warp + kDecWarps - 1) / kDecWarps : 0;
+        int pages = -1;
+        auto fetch = [&](int k) {
+            if (k < nk) {
+                if ((k & 31) == 0) {  // page ids of the next 32 units, one per lane
+                    const int u = u0 + warp + kDecWarps * (k + lane);
+                    pages = u < u_end ? kv4_page(v, b, u * kDecUnit) : -1;
+                }
+                const int u = u0 + warp + kDecWarps * k;
+                const int page = __shfl_sync(0xffffffffu, pages, k & 31);
+                const uint32_t st = ring + (k % S) * kStage;
+                const uint32_t ok = page >= 0 ? 16u : 0u;
+                const int slot = (u & ((1 << page_units_shift) - 1)) * kDecUnit;
+                const int64_t co = page >= 0 ? kv4_code_off<D>(v, page, kvh, slot) : 0;
+                const int64_t po = page >= 0 ? kv4_param_off<D>(v, page, kvh, slot) : 0;
+                constexpr int CPT = D / 32;  // 16-byte chunks per token
+#pragma unroll
+                for (int i = 0; i < kCodes / 512; ++i) {
+                    const int c = i * 32 + lane;
+                    const uint32_t d = (uint32_t)dec_chunk<D>(c / CPT, c % CPT) * 16;
+                    cp16(st + d, v.kc + co + c * 16, ok);
+                    cp16(st + kCodes + d, v.vc + co + c * 16, ok);
+                }
+                constexpr int PC = kParams / 16;
+                if (lane < 2 * PC) {
+                    const bool is_v = lane >= PC;
+                    cp16(st + 2 * kCodes + lane * 16, (is_v ? v.vp + po + (lane - PC) * 16 : v.kp + po + lane * 16), ok);
+                }
+                if (lane == 0) *reinterpret_cast<int*>(const_cast<uint8_t*>(ring_p) + (k % S) * kStage + 2 * (kCodes + kParams)) = page;
+            }
+            asm volatile("cp.async.commit_group;" ::: "memory");
+        };
+
+        float ref[2] = {-1e30f, -1e30f};
+        float o[G][4][4], xa[4] = {};
+#pragma unroll
+        for (int g = 0; g < G; ++g)
+#pragma unroll
+            for (int i = 0; i < 4; ++i)
+#pragma unroll
+                for (int c = 0; c < 4; ++c) o[g][i][c] = 0.f;
+#pragma unroll
+        for (int k = 0; k < S - 1; ++k) fetch(k);
+
+        for (int k = 0; k < nk; ++k) {
+            asm volatile("cp.async.wait_group %0;" ::"n"(S - 2) : "memory");
+            __syncwarp();
+            fetch(k + S - 1);
+            const uint8_t* st = ring_p + (k % S) * kStage;
+            const int u = u0 + warp + kDecWarps * k;
+            const uint8_t* kpar = st + 2 * kCodes;
+            const uint8_t* vpar = kpar + kParams;
+
+            // ---- S^T: keys r and r + 8
+            float a[G][4];
+#pragma unroll
+            for (int g = 0; g < G; ++g)
+#pragma unroll
+                for (int c = 0; c < 4; ++c) a[g][c] = 0.f;
+            uint32_t k0[2 * G], k1[2 * G];
+            if (D == 128) {
+                const uint4 w0 = lds_u4(st + dec_chunk<D>(r, t) * 16), w1 = lds_u4(st + dec_chunk<D>(r + 8, t) * 16);
+                k0[0] = w0.x; k0[1] = w0.y; k0[2 * G - 2] = w0.z; k0[2 * G - 1] = w0.w;
+                k1[0] = w1.x; k1[1] = w1.y; k1[2 * G - 2] = w1.z; k1[2 * G - 1] = w1.w;
+            } else {
+                const uint2 w0 = *reinterpret_cast<const uint2*>(st + dec_chunk<D>(r, t >> 1) * 16 + (t & 1) * 8);
+                const uint2 w1 = *reinterpret_cast<const uint2*>(st + dec_chunk<D>(r + 8, t >> 1) * 16 + (t & 1) * 8);
+                k0[0] = w0.x; k0[1] = w0.y;
+                k1[0] = w1.x; k1[1] = w1.y;
+            }
+#pragma unroll
+            for (int j = 0; j < 2 * G; ++j) {
+                const uint32_t lo[4] = {k0[j] & 0x000F000Fu, k1[j] & 0x000F000Fu, k0[j] & 0x00F000F0u, k1[j] & 0x00F000F0u};
+                mma_f16_16816(a[j % G], lo, qf[j][0][0], qf[j][0][1]);
+                const uint32_t s0 = k0[j] >> 8, s1 = k1[j] >> 8;
+                const uint32_t hi[4] = {s0 & 0x000F000Fu, s1 & 0x000F000Fu, s0 & 0x00F000F0u, s1 & 0x00F000F0u};
+                mma_f16_16816(a[j % G], hi, qf[j][1][0], qf[j][1][1]);
+            }
+            float sc[4];  // (key r: columns 2t, 2t + 1), (key r + 8: ...); fp32: one head, in [0] and [2]
+#pragma unroll
+            for (int hh = 0; hh < 2; ++hh) {
+                float2 sm[G];
+                const uint8_t* kr = kpar + (r + 8 * hh) * (4 * G);
+#pragma unroll
+                for (int g = 0; g < G; ++g) sm[g] = __half22float2(*reinterpret_cast<const __half2*>(kr + 4 * g));
+#pragma unroll
+                for (int j = 0; j < (kWide ? 1 : 2); ++j) {
+                    float dot = 0.f, add = 0.f;
+#pragma unroll
+                    for (int g = 0; g < G; ++g) {
+                        const float ag = kWide ? a[g][2 * hh] + a[g][2 * hh + 1] : a[g][2 * hh + j];
+                        dot = fmaf(sm[g].x, ag, dot);
+                        add = fmaf(sm[g].y, qg[g][j], add);
+                    }
+                    sc[2 * hh + j] = fmaf(dot, f[j], add);
+                }
+                if (kWide) sc[2 * hh + 1] = sc[2 * hh];
+            }
+            // V's parameters of tokens 2t, 2t + 1 and 2t + 8, 2t + 9
+            uint32_t vs[2][G], vm[2][G];  // (token, token + 1) pairs: scales, minima
+#pragma unroll
+            for (int hh = 0; hh < 2; ++hh) {
+                uint32_t w[2 * G];
+                const uint8_t* vr = vpar + (2 * t + 8 * hh) * (4 * G);
+                if (G == 2) {
+                    const uint4 y = lds_u4(vr);
+                    w[0] = y.x; w[1] = y.y; w[2 * G - 2] = y.z; w[2 * G - 1] = y.w;
+                } else {
+                    const uint2 y = *reinterpret_cast<const uint2*>(vr);
+                    w[0] = y.x; w[1] = y.y;
+                }
+#pragma unroll
+                for (int g = 0; g < G; ++g) {
+                    vs[hh][g] = __byte_perm(w[g], w[G + g], 0x5410);
+                    vm[hh][g] = __byte_perm(w[g], w[G + g], 0x7632);
+                }
+            }
+            const int page = *reinterpret_cast<const int*>(st + 2 * (kCodes + kParams));
+            if (u >= full || page < 0) {  // masks; nothing of an unseen key may reach a product
+                const int key = u * kDecUnit + r;
+#pragma unroll
+                for (int hh = 0; hh < 2; ++hh) {
+#pragma unroll
+                    for (int j = 0; j < 2; ++j)
+                        if (page < 0 || key + 8 * hh > lim[j]) sc[2 * hh + j] = -INFINITY;
+                    const int vk = u * kDecUnit + 2 * t + 8 * hh;
+                    const uint32_t keep = (vk <= lim_last ? 0x0000FFFFu : 0u) | (vk + 1 <= lim_last ? 0xFFFF0000u : 0u);
+#pragma unroll
+                    for (int g = 0; g < G; ++g) {
+                        vs[hh][g] &= keep;
+                        vm[hh][g] &= keep;
+                    }
+                }
+            }
+            // ---- softmax: the reference moves only when a score passes it by kDecLift
+            const bool over = fmaxf(sc[0], sc[2]) > ref[0] + kDecLift || fmaxf(sc[1], sc[3]) > ref[1] + kDecLift;
+            if (__any_sync(0xffffffffu, over)) {
+#pragma unroll
+                for (int j = 0; j < 2; ++j) {
+                    float m = fmaxf(sc[j], sc[2 + j]);
+                    m = fmaxf(m, __shfl_xor_sync(0xffffffffu, m, 4));
+                    m = fmaxf(m, __shfl_xor_sync(0xffffffffu, m, 8));
+                    m = fmaxf(m, __shfl_xor_sync(0xffffffffu, m, 16));
+                    m = fmaxf(m, ref[j]);
+                    const float corr = ex2(ref[j] - m);
+                    ref[j] = m;
+                    xa[j] *= corr;
+                    xa[2 + j] *= corr;
+#pragma unroll
+                    for (int g = 0; g < G; ++g)
+#pragma unroll
+                        for (int i = 0; i < 4; ++i) {
+                            o[g][i][j] *= corr;
+                            o[g][i][2 + j] *= corr;
+                        }
+                }
+            }
+            float pr[4];
+#pragma unroll
+            for (int c = 0; c < 4; ++c) pr[c] = ex2(sc[c] - ref[c & 1]);
+            // scales of 64 and more: 1024 s would leave fp16
+            uint32_t one = 0x3C003C00u;
+            {
+                bool big = false;
+#pragma unroll
+                for (int hh = 0; hh < 2; ++hh)
+#pragma unroll
+                    for (int g = 0; g < G; ++g)
+                        big |= (vs[hh][g] & 0x7FFFu) >= 0x5380u || (vs[hh][g] & 0x7FFF0000u) >= 0x53800000u;
+                if (__any_sync(0xffffffffu, big)) {
+                    const __half2 down = __float2half2_rn(0.0078125f);
+                    one = h2u(down);
+#pragma unroll
+                    for (int hh = 0; hh < 2; ++hh)
+#pragma unroll
+                        for (int g = 0; g < G; ++g) {
+                            vs[hh][g] = h2u(__hmul2(u2h(vs[hh][g]), down));
+                            vm[hh][g] = h2u(__hmul2(u2h(vm[hh][g]), down));
+                        }
+#pragma unroll
+                    for (int c = 0; c < 4; ++c) pr[c] *= 128.f;
+                }
+            }
+            uint32_t pb[2];
+#pragma unroll
+            for (int hh = 0; hh < 2; ++hh) {
+                __half2 h;
+                if (kWide) {
+                    const __half ph = __float2half_rn(pr[2 * hh]);
+                    h = __halves2half2(ph, __float2half_rn(pr[2 * hh] - __half2float(ph)));
+                } else {
+                    h = __floats2half2_rn(pr[2 * hh], pr[2 * hh + 1]);
+                }
+                pb[hh] = movm_trans(h2u(h));
+            }
+            // ---- rows: minima of the groups, ones
+            {
+                uint32_t e[4] = {0, 0, 0, 0};
+#pragma unroll
+                for (int hh = 0; hh < 2; ++hh) {
+                    uint32_t w = r == G ? one : 0u;
+#pragma unroll
+                    for (int g = 0; g < G; ++g) w = r == g ? vm[hh][g] : w;
+                    e[2 * hh] = w;
+                }
+                mma_f16_16816(xa, e, pb[0], pb[1]);
+            }
+            // ---- O^T: this lane's rows are elements 8 r .. 8 r + 7 of each group
+            uint32_t vw[2][2][G];  // [half][token of the pair][group]
+#pragma unroll
+            for (int hh = 0; hh < 2; ++hh)
+#pragma unroll
+                for (int y = 0; y < 2; ++y) {
+                    const int tk = 2 * t + 8 * hh + y;
+                    if (G == 2) {
+                        const uint2 w = *reinterpret_cast<const uint2*>(st + kCodes + dec_chunk<D>(tk, r >> 1) * 16 + (r & 1) * 8);
+                        vw[hh][y][0] = w.x;
+                        vw[hh][y][G - 1] = w.y;
+                    } else {
+                        vw[hh][y][0] = *reinterpret_cast<const uint32_t*>(st + kCodes + dec_chunk<D>(tk, r >> 2) * 16 + (r & 3) * 4);
+                    }
+                }
+            const __half2 k1024 = __float2half2_rn(-1024.f), k64 = __float2half2_rn(-64.f);
+#pragma unroll
+            for (int g = 0; g < G; ++g) {
+                const __half2 s2[2] = {u2h(vs[0][g]), u2h(vs[1][g])};
+                const __half2 n1[2] = {__hmul2(s2[0], k1024), __hmul2(s2[1], k1024)};
+                const __half2 n2[2] = {__hmul2(s2[0], k64), __hmul2(s2[1], k64)};
+#pragma unroll
+                for (int part = 0; part < 2; ++part) {  // elements 4 part .. 4 part + 3
+                    uint32_t w[2];
+#pragma unroll
+                    for (int hh = 0; hh < 2; ++hh)
+                        w[hh] = __byte_perm(vw[hh][0][g], vw[hh][1][g], part ? 0x7632 : 0x5410);
+#pragma unroll
+                    for (int q2 = 0; q2 < 2; ++q2) {
+                        uint32_t hi[4], lo[4];
+#pragma unroll
+                        for (int hh = 0; hh < 2; ++hh) {
+                            const uint32_t ww = q2 ? w[hh] >> 8 : w[hh];
+                            const __half2 x0 = u2h((ww & 0x000F000Fu) | 0x64006400u);
+                            const __half2 x1 = u2h((ww & 0x00F000F0u) | 0x54005400u);
+                            const __half2 y0 = __hfma2(x0, s2[hh], n1[hh]), y1 = __hfma2(x1, s2[hh], n2[hh]);
+                            hi[2 * hh] = h2u(y0);
+                            hi[2 * hh + 1] = h2u(y1);
+                            if (kWide) {
+                                lo[2 * hh] = h2u(__hfma2(__hadd2(x0, k1024), s2[hh], __hneg2(y0)));
+                                lo[2 * hh + 1] = h2u(__hfma2(__hadd2(x1, k64), s2[hh], __hneg2(y1)));
+                            }
+                        }
+                        mma_f16_16816(o[g][2 * part + q2], hi, pb[0], pb[1]);
+                        if (kWide) mma_f16_16816(o[g][2 * part + q2], lo, pb[0], pb[1]);
+                    }
+                }
+            }
+        }
+        asm volatile("cp.async.wait_group 0;" ::: "memory");
+
+        // ---- the warps' sums together: [warp][column][D] and (reference, denominator, minima)
+        __syncthreads();  // the rings are read out
+        float* mo = reinterpret_cast<float*>(smem);
+        float* mx = mo + kDecWarps * 8 * kMS;  // [warp][column][4]
+        if (kWide) {  // high and low columns of one head
+#pragma unroll
+            for (int c = 0; c < 4; c += 2) {
+                xa[c] += xa[c + 1];
+#pragma unroll
+                for (int g = 0; g < G; ++g)
+#pragma unroll
+                    for (int i = 0; i < 4; ++i) o[g][i][c] += o[g][i][c + 1];
+            }
+        }
+#pragma unroll
+        for (int j = 0; j < (kWide ? 1 : 2); ++j) {
+            const int col = kWide ? t : 2 * t + j;
+            float* dst = mo + (warp * 8 + col) * kMS;
+#pragma unroll
+            for (int g = 0; g < G; ++g)
+#pragma unroll
+                for (int i = 0; i < 4; ++i)
+                    *reinterpret_cast<float2*>(dst + g * kKv4Group + 8 * r + 2 * i) = make_float2(o[g][i][j], o[g][i][2 + j]);
+            if (r <= G) mx[(warp * 8 + col) * 4 + (r == G ? 1 : 2 + r)] = xa[j];
+            if (r == 0) mx[(warp * 8 + col) * 4] = ref[j];
+        }
+        __syncthreads();
+        const bool whole = u0 == 0 && u1 == sq.units;
+        const int slot = blockIdx.x * 2 + (u0 == 0 ? 1 : 0);
+        if (!whole && threadIdx.x == 0 && u0 > 0 && u1 == sq.units)
+            ws.meta[blockIdx.x] = {(int)((x - u0) / share), b, kvh, ct};
+        for (int e = threadIdx.x; e < cols * D; e += kDecThreads) {
+            const int col = e / D, d = e % D;
+            float m = -1e30f;
+#pragma unroll
+            for (int w = 0; w < kDecWarps; ++w) m = fmaxf(m, mx[(w * 8 + col) * 4]);
+            float l = 0.f, val = 0.f;
+#pragma unroll
+            for (int w = 0; w < kDecWarps; ++w) {
+                const float4 y = *reinterpret_cast<const float4*>(mx + (w * 8 + col) * 4);
+                const float fw = ex2(y.x - m);
+                l = fmaf(fw, y.y, l);
+                val = fmaf(fw, mo[(w * 8 + col) * kMS + d] + (d < kKv4Group ? y.z : y.w), val);
+            }
+            if (whole) {
+                const int fcol = ct * CT + col, rw = fcol / p.grp, hd = kvh * p.grp + fcol - rw * p.grp;
+                static_cast<T*>(p.out)[(int64_t)(sq.row0 + rw) * p.os + (int64_t)hd * D + d] =
+                        Act<T>::store(l > 0.f ? val / l : 0.f);
+            } else {
+                ws.o[((int64_t)slot * 8 + col) * D + d] = val;
+                if (d == 0) ws.ml[slot * 8 + col] = make_float2(m, l);
+            }
+        }
+        __syncthreads();  // before the next segment's copies overwrite the sums
+        x += u1 - u0;
+        off += u1 - u0;
+    }
+}
+
+// Partial sums of an item that was cut between CTAs, one column per CTA row.
+template <typename T, int D>
+__global__ void __launch_bounds__(128) kv4_combine_kernel(Kv4AttnParams p, DecWork ws) {
+    constexpr int CT = dec_cols<T>(), E = D / 32;
+    __shared__ float so[4][D];
+    __shared__ float2 sm[4];
+    pdl_wait();
+    pdl_trigger();
+    const DecMeta me = ws.meta[blockIdx.x];
+    if (me.first < 0) return;
+    int row0, n;
+    kv4_rows(p.v, me.b, row0, n);
+    const int col = blockIdx.y, fcol = me.ct * CT + col;
+    if (fcol >= n * p.grp) return;
+    const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+    float m = -1e30f, l = 0.f, acc[E] = {};
+    for (int c = me.first + warp; c <= (int)blockIdx.x; c += 4) {
+        const int slot = 2 * c + (c == me.first ? 1 : 0);
+        const float2 y = ws.ml[slot * 8 + col];
+        float val[E];
+#pragma unroll
+        for (int i = 0; i < E; ++i) val[i] = ws.o[((int64_t)slot * 8 + col) * D + lane * E + i];
+        const float nm = fmaxf(m, y.x), fa = ex2(m - nm), fb = ex2(y.x - nm);
+        l = l * fa + y.y * fb;
+#pragma unroll
+        for (int i = 0; i < E; ++i) acc[i] = acc[i] * fa + val[i] * fb;
+        m = nm;
+    }
+    if (lane == 0) sm[warp] = make_float2(m, l);
+#pragma unroll
+    for (int i = 0; i < E; ++i) so[warp][lane * E + i] = acc[i];
+    __syncthreads();
+    for (int d = threadIdx.x; d < D; d += 128) {
+        const float mm = fmaxf(fmaxf(sm[0].x, sm[1].x), fmaxf(sm[2].x, sm[3].x));
+        float ls = 0.f, vs = 0.f;
+#pragma unroll
+        for (int w = 0; w < 4; ++w) {
+            const float fw = ex2(sm[w].x - mm);
+            ls = fmaf(fw, sm[w].y, ls);
+            vs = fmaf(fw, so[w][d], vs);
+        }
+        const int rw = fcol / p.grp, hd = me.kvh * p.grp + fcol - rw * p.grp;
+        static_cast<T*>(p.out)[(int64_t)(row0 + rw) * p.os + (int64_t)hd * D + d] = Act<T>::store(ls > 0.f ? vs / ls : 0.f);
+    }
 }
 
 }  // namespace amcu
 
 using namespace amcu;
 
+namespace {
+
+int dec_ctas() { return 2 * num_sms(); }
+
+// The decode workspace: partial sums and their bookkeeping, 16-byte aligned parts.
+size_t dec_layout(int64_t ctas, int64_t d, uint8_t* base, DecWork* w) {
+    const size_t o = (size_t)ctas * 16 * d * sizeof(float), ml = (size_t)ctas * 16 * sizeof(float2);
+    if (w) {
+        w->o = reinterpret_cast<float*>(base);
+        w->ml = reinterpret_cast<float2*>(base + o);
+        w->meta = reinterpret_cast<DecMeta*>(base + o + ml);
+    }
+    return o + ml + (size_t)ctas * sizeof(DecMeta);
+}
+
+template <typename T, int D>
+void launch_decode(const Kv4AttnParams& p, const DecWork& w, cudaStream_t s) {
+    constexpr int smem = dec_smem_bytes<D>();
+    set_func_attr_once(reinterpret_cast<const void*>(&kv4_decode_kernel<T, D>),
+                       cudaFuncAttributeMaxDynamicSharedMemorySize, smem);
+    const unsigned ctas = (unsigned)dec_ctas();
+    launch_pdl(kv4_decode_kernel<T, D>, dim3(ctas), dim3(kDecThreads), smem, s, p, w);
+    launch_pdl(kv4_combine_kernel<T, D>, dim3(ctas, dec_cols<T>()), dim3(128), 0, s, p, w);
+}
+
+}  // namespace
+
 extern "C" size_t amcu_attn_kv4_workspace_bytes(const AmcuKv4AttentionArgs* a) {
-    (void)a;
-    return 0;
+    if (!a || a->batch.rows <= 0 || a->batch.n_seq <= 0) return 0;
+    return dec_layout(dec_ctas(), a->cache.head_dim, nullptr, nullptr);
 }
 
 extern "C" am_status_code amcu_attn_kv4(const AmcuKv4AttentionArgs* a, void* stream) {
@@ -102,15 +673,16 @@ extern "C" am_status_code amcu_attn_kv4(const AmcuKv4AttentionArgs* a, void* str
     p.nq = (int)a->n_q_heads;
     p.grp = (int)(a->n_q_heads / a->cache.n_kv_heads);
     p.scale = a->scale > 0.f ? a->scale : 1.f / sqrtf((float)a->cache.head_dim);
-    const int64_t blocks = ceil_div(a->batch.rows * a->n_q_heads, 4);
-    AMCU_REQUIRE(blocks <= INT32_MAX, "amcu_attn_kv4: too many rows");
-    const dim3 grid((unsigned)blocks), block(128);
+    const size_t need = amcu_attn_kv4_workspace_bytes(a);
+    AMCU_REQUIRE(a->workspace && a->workspace_size >= need && aligned(a->workspace, 16),
+                 "amcu_attn_kv4: needs a 16-byte aligned workspace of %zu bytes", need);
+    DecWork w;
+    dec_layout(dec_ctas(), a->cache.head_dim, static_cast<uint8_t*>(a->workspace), &w);
     const bool f32 = a->dtype == AMCU_F32;
+    cudaStream_t s = as_stream(stream);
     if (a->cache.head_dim == 64)
-        f32 ? launch_pdl(kv4_attn_simple_kernel<float, 64>, grid, block, 0, as_stream(stream), p)
-            : launch_pdl(kv4_attn_simple_kernel<__nv_bfloat16, 64>, grid, block, 0, as_stream(stream), p);
+        f32 ? launch_decode<float, 64>(p, w, s) : launch_decode<__nv_bfloat16, 64>(p, w, s);
     else
-        f32 ? launch_pdl(kv4_attn_simple_kernel<float, 128>, grid, block, 0, as_stream(stream), p)
-            : launch_pdl(kv4_attn_simple_kernel<__nv_bfloat16, 128>, grid, block, 0, as_stream(stream), p);
+        f32 ? launch_decode<float, 128>(p, w, s) : launch_decode<__nv_bfloat16, 128>(p, w, s);
     return check_launch("amcu_attn_kv4");
 }
