@@ -79,6 +79,58 @@ __device__ __forceinline__ int64_t kv4_param_off(const Kv4View& v, int page, int
     return (int64_t)page * v.pps + (((int64_t)head << v.page_shift) + slot) * (D / 16);
 }
 
+// Positions in a call's flat list of work: sequence b has cost(b) items (the
+// same in every thread), and the CTA wants item pick(all items). Every thread of the block
+// (THREADS of them) calls this; it returns true in the one thread that found
+// the sequence, with off = the item's place in sequence b. `total` is
+// the same in all threads. Each thread adds up a run of sequences.
+template <int THREADS, typename P, typename F>
+__device__ __forceinline__ bool kv4_share(int n_seq, P pick, F cost, int64_t& total, int& b, int64_t& off) {
+    __shared__ int64_t part[THREADS / 32];
+    const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
+    const int chunk = (n_seq + THREADS - 1) / THREADS;
+    const int lo = threadIdx.x * chunk, hi = min(lo + chunk, n_seq);
+    int64_t mine = 0;
+    for (int i = lo; i < hi; ++i) mine += cost(i);
+    int64_t incl = mine;
+#pragma unroll
+    for (int o = 1; o < 32; o <<= 1) {
+        const int64_t y = __shfl_up_sync(0xffffffffu, incl, o);
+        if (lane >= o) incl += y;
+    }
+    if (lane == 31) part[warp] = incl;
+    __syncthreads();
+    int64_t base = 0;
+    total = 0;
+#pragma unroll
+    for (int w = 0; w < THREADS / 32; ++w) {
+        if (w < warp) base += part[w];
+        total += part[w];
+    }
+    off = pick(total) - (base + incl - mine);
+    b = lo;
+    if (off < 0 || off >= mine) return false;
+    for (;; ++b) {
+        const int64_t c = cost(b);
+        if (off < c) return true;
+        off -= c;
+    }
+}
+
+struct Kv4AttnParams {
+    Kv4View v;
+    const void* q;
+    void* out;
+    int64_t qs, os;
+    int nq, grp;
+    float scale;
+    int vec;   // q and out rows start on 16-byte boundaries
+};
+
+// Prompts (bf16): whether their kernel is the faster one for this call, and its launch.
+bool kv4_prefill_wanted(const Kv4View& v, int64_t grp);
+am_status_code kv4_prefill_launch(const Kv4AttnParams& p, int64_t d, cudaStream_t s);
+
 // Checks the cache and batch of a call and fills the view.
 am_status_code kv4_check(const char* what, const AmcuKv4Cache& c, const AmcuKv4Batch& b, Kv4View* out);
 

@@ -7,15 +7,6 @@
 
 namespace amcu {
 
-struct Kv4AttnParams {
-    Kv4View v;
-    const void* q;
-    void* out;
-    int64_t qs, os;
-    int nq, grp;
-    float scale;
-};
-
 // ---------------------------------------------------------------------------
 // Single tokens and short runs of rows.
 //
@@ -116,7 +107,6 @@ __global__ void __launch_bounds__(kDecThreads, 2) kv4_decode_kernel(Kv4AttnParam
     constexpr int kStage = dec_stage_bytes<D>(), S = kDecStages;
     constexpr int kMS = dec_merge_stride<D>();
     extern __shared__ __align__(128) uint8_t smem[];
-    __shared__ int64_t scan_part[kDecWarps];
     __shared__ int64_t s_off;
     __shared__ int s_b;
 
@@ -126,48 +116,29 @@ __global__ void __launch_bounds__(kDecThreads, 2) kv4_decode_kernel(Kv4AttnParam
 
     // ---- this CTA's share [x, x_end) of all units
     const Kv4View& v = p.v;
-    const int chunk = (v.n_seq + kDecThreads - 1) / kDecThreads;
-    const int b_lo = threadIdx.x * chunk, b_hi = min(b_lo + chunk, v.n_seq);
-    int64_t mine = 0;
-    for (int b = b_lo; b < b_hi; ++b) {
-        const DecSeq s = dec_seq<T>(v, p.grp, b);
-        mine += (int64_t)s.units * s.tiles * v.nkv;
-    }
-    int64_t incl = mine;
-#pragma unroll
-    for (int o = 1; o < 32; o <<= 1) {
-        const int64_t y = __shfl_up_sync(0xffffffffu, incl, o);
-        if (lane >= o) incl += y;
-    }
-    if (lane == 31) scan_part[warp] = incl;
-    __syncthreads();
-    int64_t base = 0, total = 0;
-#pragma unroll
-    for (int w = 0; w < kDecWarps; ++w) {
-        if (w < warp) base += scan_part[w];
-        total += scan_part[w];
-    }
-    int64_t share = (total + gridDim.x - 1) / gridDim.x;
-    if (share < kDecMinUnits) share = kDecMinUnits;
-    int64_t x = blockIdx.x * share;
-    const int64_t x_end = min(x + share, total);
-    if (threadIdx.x == 0) ws.meta[blockIdx.x].first = -1;
-    if (x >= x_end) return;
+    auto cost_of = [&](int i) {
+        const DecSeq q = dec_seq<T>(v, p.grp, i);
+        return (int64_t)q.units * q.tiles * v.nkv;
+    };
+    int64_t total, share, x;
     {
-        const int64_t ex = base + incl - mine;
-        if (x >= ex && x < ex + mine) {  // exactly one thread
-            int64_t off = x - ex;
-            int b = b_lo;
-            for (;; ++b) {
-                const DecSeq s = dec_seq<T>(v, p.grp, b);
-                const int64_t cost = (int64_t)s.units * s.tiles * v.nkv;
-                if (off < cost) break;
-                off -= cost;
-            }
+        int b;
+        int64_t off;
+        const bool have = kv4_share<kDecThreads>(
+                v.n_seq,
+                [&](int64_t all) {
+                    share = max((all + gridDim.x - 1) / gridDim.x, (int64_t)kDecMinUnits);
+                    return x = blockIdx.x * share;
+                },
+                cost_of, total, b, off);
+        if (have) {
             s_b = b;
             s_off = off;
         }
     }
+    const int64_t x_end = min(x + share, total);
+    if (threadIdx.x == 0) ws.meta[blockIdx.x].first = -1;
+    if (x >= x_end) return;
     __syncthreads();
     int b = s_b;
     int64_t off = s_off;
@@ -673,6 +644,8 @@ extern "C" am_status_code amcu_attn_kv4(const AmcuKv4AttentionArgs* a, void* str
     p.nq = (int)a->n_q_heads;
     p.grp = (int)(a->n_q_heads / a->cache.n_kv_heads);
     p.scale = a->scale > 0.f ? a->scale : 1.f / sqrtf((float)a->cache.head_dim);
+    p.vec = aligned(a->q, 16) && aligned(a->out, 16) && a->q_stride % 8 == 0 && a->out_stride % 8 == 0;
+    const bool prompts = a->dtype == AMCU_BF16 && kv4_prefill_wanted(p.v, p.grp);
     const size_t need = amcu_attn_kv4_workspace_bytes(a);
     AMCU_REQUIRE(a->workspace && a->workspace_size >= need && aligned(a->workspace, 16),
                  "amcu_attn_kv4: needs a 16-byte aligned workspace of %zu bytes", need);
@@ -680,6 +653,7 @@ extern "C" am_status_code amcu_attn_kv4(const AmcuKv4AttentionArgs* a, void* str
     dec_layout(dec_ctas(), a->cache.head_dim, static_cast<uint8_t*>(a->workspace), &w);
     const bool f32 = a->dtype == AMCU_F32;
     cudaStream_t s = as_stream(stream);
+    if (prompts) return kv4_prefill_launch(p, a->cache.head_dim, s);
     if (a->cache.head_dim == 64)
         f32 ? launch_decode<float, 64>(p, w, s) : launch_decode<__nv_bfloat16, 64>(p, w, s);
     else

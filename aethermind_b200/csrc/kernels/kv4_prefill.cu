@@ -1,0 +1,580 @@
+// Causal attention of prompts over the 4-bit paged KV cache on the
+// 5th-generation tensor cores (tcgen05 + TMEM), bf16.
+//
+// The rows of a product are (token, q head) pairs of one kv head, 256 to a CTA
+// (two tiles of 128), so a key tile is dequantised once for all of the group's
+// heads. Per key tile of 128:
+//   S = Q K^T   A = Q (shared memory, fp16, scaled by a power of two per row),
+//               B = K, S in tensor memory (one lane per row)
+//   P = 2^(S f - ref) by one thread per row, in fp16 over S's own columns
+//   O += P V    A = P (tensor memory), B = V^T, O in tensor memory
+// Warps 0-3 and 4-7 are the softmax of the two row tiles, warps 8-11 turn codes
+// into fp16 tiles, warp 12 issues the MMAs and owns the tensor memory. While
+// one row tile's softmax runs, the other's products do.
+//
+// K tile and V^T tile have the 128-byte-swizzled K-major layout. A word of 8
+// codes is one 16-byte chunk of a K row; its nibbles come out in the order
+// 0 4 1 5 2 6 3 7, and Q's elements are stored in that order too. V is read
+// across 8 tokens, so a chunk of V^T is 8 keys of one element. Values are
+// m + s c in fp16: (1024 + c) - 1024 exactly, then one fused multiply-add
+// rounded once to 11 bits (an element beyond fp16 becomes 65504).
+//
+// The softmax reference of a row moves (and O and the sum are rescaled) only
+// when the tile's maximum passes it by 2^8: p stays inside fp16, whose relative
+// precision does not depend on the reference.
+//
+// Waits are bounded: one that runs out records an error code, and the CTA goes
+// through its control flow without waiting again.
+#include "kv4.cuh"
+#include "tcgen05.cuh"
+
+namespace amcu {
+
+constexpr int kPfRows = 256, kPfKeys = 128;
+constexpr int kPfThreads = 13 * 32;
+constexpr int kPfDqThreads = 128;
+constexpr int32_t kErrKv4Wait = 0x501;
+constexpr float kPfLog2e = 1.4426950408889634f;
+constexpr float kPfLift = 8.f;
+
+template <int D>
+struct PfLayout {  // shared memory, bytes
+    static constexpr int kQ = 128 * D * 2;            // one row tile of Q
+    static constexpr int kK = kPfKeys * D * 2;        // a K or V^T stage
+    static constexpr int kRawK = kPfKeys * D / 2;
+    static constexpr int kVPitch = 8 * D / 2 + 16;    // 8 tokens of V codes
+    static constexpr int kRawV = kPfKeys / 8 * kVPitch;
+    static constexpr int kParK = kPfKeys * D / 16;
+    static constexpr int kVParPitch = 8 * D / 16 + 16;
+    static constexpr int kParV = kPfKeys / 8 * kVParPitch;
+    static constexpr int oQ = 0, oK = oQ + 2 * kQ, oV = oK + 2 * kK, oRawK = oV + 2 * kK, oRawV = oRawK + kRawK,
+                         oParK = oRawV + kRawV, oParV = oParK + kParK, oBar = oParV + kParV;
+    static constexpr int kTotal = oBar + 256 + 1024;  // + alignment slack
+};
+
+// Offset of 16-byte chunk c of row r in a K-major tile of ROWS rows: halves of
+// 64 elements (128 bytes a row), 16-byte chunks XOR-swizzled by row % 8.
+template <int ROWS>
+__device__ __forceinline__ uint32_t pf_sw(int r, int c) {
+    return (uint32_t)((c >> 3) * (ROWS * 128) + (r >> 3) * 1024 + (r & 7) * 128 + (((c & 7) ^ (r & 7)) << 4));
+}
+
+__device__ __forceinline__ void tc_ld32_issue(uint32_t taddr, uint32_t (&r)[32]) {
+    asm volatile(
+            "tcgen05.ld.sync.aligned.32x32b.x32.b32 {%0,%1,%2,%3,%4,%5,%6,%7,%8,%9,%10,%11,%12,%13,%14,%15,"
+            "%16,%17,%18,%19,%20,%21,%22,%23,%24,%25,%26,%27,%28,%29,%30,%31}, [%32];"
+            : "=r"(r[0]), "=r"(r[1]), "=r"(r[2]), "=r"(r[3]), "=r"(r[4]), "=r"(r[5]), "=r"(r[6]), "=r"(r[7]),
+              "=r"(r[8]), "=r"(r[9]), "=r"(r[10]), "=r"(r[11]), "=r"(r[12]), "=r"(r[13]), "=r"(r[14]), "=r"(r[15]),
+              "=r"(r[16]), "=r"(r[17]), "=r"(r[18]), "=r"(r[19]), "=r"(r[20]), "=r"(r[21]), "=r"(r[22]),
+              "=r"(r[23]), "=r"(r[24]), "=r"(r[25]), "=r"(r[26]), "=r"(r[27]), "=r"(r[28]), "=r"(r[29]),
+              "=r"(r[30]), "=r"(r[31])
+            : "r"(taddr));
+}
+// Waits for this thread's tcgen05.ld; the registers are tied so that nothing reads them earlier.
+__device__ __forceinline__ void tc_ld32_wait(uint32_t (&r)[32]) {
+    asm volatile("tcgen05.wait::ld.sync.aligned;"
+                 : "+r"(r[0]), "+r"(r[1]), "+r"(r[2]), "+r"(r[3]), "+r"(r[4]), "+r"(r[5]), "+r"(r[6]), "+r"(r[7]),
+                   "+r"(r[8]), "+r"(r[9]), "+r"(r[10]), "+r"(r[11]), "+r"(r[12]), "+r"(r[13]), "+r"(r[14]),
+                   "+r"(r[15]), "+r"(r[16]), "+r"(r[17]), "+r"(r[18]), "+r"(r[19]), "+r"(r[20]), "+r"(r[21]),
+                   "+r"(r[22]), "+r"(r[23]), "+r"(r[24]), "+r"(r[25]), "+r"(r[26]), "+r"(r[27]), "+r"(r[28]),
+                   "+r"(r[29]), "+r"(r[30]), "+r"(r[31])::"memory");
+}
+__device__ __forceinline__ void tc_st32(uint32_t taddr, const uint32_t (&r)[32]) {
+    tc_st_32x32b_x32(taddr, r);
+}
+__device__ __forceinline__ float pf_ex2(float x) {
+    float r;
+    asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(r) : "f"(x));
+    return r;
+}
+__device__ __forceinline__ uint32_t pf_h2u(__half2 h) { return *reinterpret_cast<uint32_t*>(&h); }
+__device__ __forceinline__ __half2 pf_u2h(uint32_t u) { return *reinterpret_cast<__half2*>(&u); }
+// Two fp32 operations in one instruction.
+__device__ __forceinline__ uint64_t f2_pack(float a, float b) {
+    uint64_t r;
+    asm("mov.b64 %0, {%1, %2};" : "=l"(r) : "f"(a), "f"(b));
+    return r;
+}
+__device__ __forceinline__ void f2_unpack(uint64_t v, float& a, float& b) { asm("mov.b64 {%0, %1}, %2;" : "=f"(a), "=f"(b) : "l"(v)); }
+__device__ __forceinline__ uint64_t f2_fma(uint64_t a, uint64_t b, uint64_t c) {
+    uint64_t r;
+    asm("fma.rn.f32x2 %0, %1, %2, %3;" : "=l"(r) : "l"(a), "l"(b), "l"(c));
+    return r;
+}
+__device__ __forceinline__ uint64_t f2_add(uint64_t a, uint64_t b) {
+    uint64_t r;
+    asm("add.rn.f32x2 %0, %1, %2;" : "=l"(r) : "l"(a), "l"(b));
+    return r;
+}
+__device__ __forceinline__ void pf_cp16(void* dst, const void* src, uint32_t bytes) {
+    asm volatile("cp.async.cg.shared.global [%0], [%1], 16, %2;" ::"r"(smem_u32(dst)), "l"(src), "r"(bytes) : "memory");
+}
+
+// m + s c of a register's two codes: low nibbles in bits 0-3 of the halves, or in bits 4-7.
+__device__ __forceinline__ __half2 pf_value(uint32_t w, bool high, __half2 s, __half2 m) {
+    const __half2 c = high ? __hadd2(pf_u2h((w & 0x00F000F0u) | 0x54005400u), __float2half2_rn(-64.f))
+                           : __hadd2(pf_u2h((w & 0x000F000Fu) | 0x64006400u), __float2half2_rn(-1024.f));
+    return __hfma2(c, s, m);
+}
+
+template <int D>
+__global__ void __launch_bounds__(kPfThreads, 1) kv4_prefill_kernel(Kv4AttnParams p, int32_t* err) {
+    using L = PfLayout<D>;
+    constexpr int G = D / kKv4Group, WPR = D / 8;  // groups, words per row
+    extern __shared__ uint8_t pf_raw[];
+    uint8_t* sm = reinterpret_cast<uint8_t*>((reinterpret_cast<uintptr_t>(pf_raw) + 1023) & ~(uintptr_t)1023);
+    uint64_t* bar = reinterpret_cast<uint64_t*>(sm + L::oBar);
+    uint64_t *k_full = bar, *k_empty = bar + 2, *v_full = bar + 4, *v_empty = bar + 6, *s_full = bar + 8,
+             *p_full = bar + 10, *o_full = bar + 12;
+    uint32_t* tmem_slot = reinterpret_cast<uint32_t*>(bar + 14);
+    int* s_item = reinterpret_cast<int*>(bar + 15);  // b, item of b
+
+    const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+    pdl_wait();
+    pdl_trigger();
+
+    // ---- this CTA's item: sequence, kv head and row tile
+    const Kv4View& v = p.v;
+    {
+        auto cost = [&](int b) {
+            int r0, n;
+            kv4_rows(v, b, r0, n);
+            return ((int64_t)n * p.grp + kPfRows - 1) / kPfRows * v.nkv;
+        };
+        int64_t total, off;
+        int b;
+        const bool have = kv4_share<kPfThreads>(v.n_seq, [&](int64_t) { return (int64_t)blockIdx.x; }, cost, total, b, off);
+        if ((int64_t)blockIdx.x >= total) return;
+        if (have) {
+            s_item[0] = b;
+            s_item[1] = (int)off;
+        }
+    }
+    if (warp == 12) {
+        if (lane == 0) {
+            for (int i = 0; i < 2; ++i) {
+                mbar_init(&k_full[i], 4);
+                mbar_init(&k_empty[i], 1);
+                mbar_init(&v_full[i], 4);
+                mbar_init(&v_empty[i], 1);
+                mbar_init(&s_full[i], 1);
+                mbar_init(&p_full[i], 4);
+                mbar_init(&o_full[i], 1);
+            }
+            fence_mbar_init();
+        }
+        __syncwarp();
+        asm volatile("tcgen05.alloc.cta_group::1.sync.aligned.shared::cta.b32 [%0], %1;" ::"r"(smem_u32(tmem_slot)),
+                     "r"(512)
+                     : "memory");
+        asm volatile("tcgen05.relinquish_alloc_permit.cta_group::1.sync.aligned;" ::: "memory");
+    }
+    __syncthreads();
+    const int b = s_item[0];
+    int row0, n;
+    kv4_rows(v, b, row0, n);
+    const int nt_rows = (int)(((int64_t)n * p.grp + kPfRows - 1) / kPfRows);
+    const int tile = nt_rows - 1 - s_item[1] / v.nkv, kvh = s_item[1] % v.nkv;  // the longest rows first
+    const int ctx = v.ctx_len[b];
+    const int cap = (int)min((int64_t)max(ctx, 0), (int64_t)v.max_pages << v.page_shift);
+    const int m0 = tile * kPfRows, m_end = min(m0 + kPfRows, n * p.grp);  // flat rows: token * grp + head
+    const int lim_last = min(ctx - n + (m_end - 1) / p.grp, cap - 1);     // last key that any row sees
+    const int nt = lim_last >= 0 ? lim_last / kPfKeys + 1 : 0;            // key tiles
+    const int ni = m_end - m0 > 128 ? 2 : 1;                              // row tiles
+    if (ctx > cap && v.status && threadIdx.x == 0) *v.status = (int32_t)AM_STATUS_OUT_OF_RANGE;
+
+    // ---- Q: one thread per row
+    float f = 0.f;           // 2^e scale log2(e) of this thread's row
+    int lim = -1;            // its last key
+    const int m = m0 + threadIdx.x;
+    const bool row_live = threadIdx.x < kPfRows && m < m_end;
+    const int tok = row_live ? m / p.grp : 0, head = kvh * p.grp + (row_live ? m - tok * p.grp : 0);
+    if (warp < 8) {
+        const __nv_bfloat16* qp = static_cast<const __nv_bfloat16*>(p.q) + (int64_t)(row0 + tok) * p.qs + (int64_t)head * D;
+        uint32_t q[D / 2];
+        if (row_live && p.vec) {
+#pragma unroll
+            for (int i = 0; i < D / 8; ++i) {
+                const uint4 y = *reinterpret_cast<const uint4*>(qp + 8 * i);
+                q[4 * i] = y.x; q[4 * i + 1] = y.y; q[4 * i + 2] = y.z; q[4 * i + 3] = y.w;
+            }
+        } else {
+            const uint16_t* qe = reinterpret_cast<const uint16_t*>(qp);
+#pragma unroll
+            for (int i = 0; i < D / 2; ++i) q[i] = row_live ? (uint32_t)qe[2 * i] | ((uint32_t)qe[2 * i + 1] << 16) : 0u;
+        }
+        float amax = 0.f;
+#pragma unroll
+        for (int i = 0; i < D / 2; ++i)
+            amax = fmaxf(amax, fmaxf(fabsf(__uint_as_float(q[i] << 16)), fabsf(__uint_as_float(q[i] & 0xffff0000u))));
+        const uint32_t eb = min(max(__float_as_uint(amax) >> 23, 1u), 253u);
+        const float inv = __uint_as_float((254u - eb) << 23);
+        f = __uint_as_float(eb << 23) * p.scale * kPfLog2e;
+        if (row_live) lim = min(ctx - n + tok, cap - 1);
+        uint8_t* Q = sm + L::oQ + (warp >> 2) * L::kQ;
+        const int r = threadIdx.x & 127;
+#pragma unroll
+        for (int c = 0; c < D / 8; ++c) {  // elements 0 4 1 5 2 6 3 7 of the chunk
+            float e[8];
+#pragma unroll
+            for (int i = 0; i < 4; ++i) {
+                e[2 * i] = __uint_as_float(q[4 * c + i] << 16) * inv;
+                e[2 * i + 1] = __uint_as_float(q[4 * c + i] & 0xffff0000u) * inv;
+            }
+            *reinterpret_cast<uint4*>(Q + pf_sw<128>(r, c)) =
+                    make_uint4(pf_h2u(__floats2half2_rn(e[0], e[4])), pf_h2u(__floats2half2_rn(e[1], e[5])),
+                               pf_h2u(__floats2half2_rn(e[2], e[6])), pf_h2u(__floats2half2_rn(e[3], e[7])));
+        }
+        asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
+    }
+    tc_fence_before();
+    __syncthreads();
+    tc_fence_after();
+    const uint32_t tmem = *tmem_slot;
+    bool ok = true;
+    auto wait = [&](uint64_t* w, uint32_t parity) {
+        if (ok && !mbar_wait(w, parity)) {
+            ok = false;
+            record_device_error(err, kErrKv4Wait);
+        }
+    };
+
+    if (warp == 12) {
+        // ---- MMA issuer
+        if (lane == 0 && nt > 0) {
+            constexpr uint32_t id_s = tc_idesc_f16(128, kPfKeys), id_o = tc_idesc_f16(128, D);
+            auto qk = [&](int i, int j) {
+                const uint32_t a = smem_u32(sm + L::oQ + i * L::kQ), bb = smem_u32(sm + L::oK + (j & 1) * L::kK);
+#pragma unroll
+                for (int s = 0; s < D / 16; ++s) {
+                    const uint32_t o = (uint32_t)((s >> 2) * 16384 + (s & 3) * 32);
+                    tc_mma(tmem + (uint32_t)(128 * i), tc_desc_sw128(a + o), tc_desc_sw128(bb + o), id_s, s != 0);
+                }
+            };
+            wait(&k_full[0], 0);
+            tc_fence_after();
+            for (int i = 0; i < ni; ++i) {
+                if (ok) qk(i, 0);
+                tc_commit(&s_full[i]);
+            }
+            tc_commit(&k_empty[0]);
+            for (int j = 0; j < nt; ++j) {
+                const bool more = j + 1 < nt;
+                wait(&v_full[j & 1], (j >> 1) & 1);
+                if (more) wait(&k_full[(j + 1) & 1], ((j + 1) >> 1) & 1);
+                for (int i = 0; i < ni; ++i) {
+                    wait(&p_full[i], j & 1);
+                    tc_fence_after();
+                    if (ok) {
+                        const uint32_t bb = smem_u32(sm + L::oV + (j & 1) * L::kK);
+#pragma unroll
+                        for (int s = 0; s < kPfKeys / 16; ++s) {
+                            const uint32_t o = (uint32_t)((s >> 2) * (D * 128) + (s & 3) * 32);
+                            tc_mma_ts(tmem + 256u + (uint32_t)(128 * i), tmem + (uint32_t)(128 * i + 8 * s),
+                                      tc_desc_sw128(bb + o), id_o, j != 0 || s != 0);
+                        }
+                        if (more) qk(i, j + 1);
+                    }
+                    tc_commit(more ? &s_full[i] : &o_full[i]);
+                }
+                tc_commit(&v_empty[j & 1]);
+                if (more) tc_commit(&k_empty[(j + 1) & 1]);
+            }
+        }
+        __syncwarp();
+    } else if (warp >= 8) {
+        // ---- codes to fp16 tiles
+        const int t = threadIdx.x - 256;  // 0..127: the token of a K row
+        const int w = t >> 5;
+        constexpr int CPT = D / 32;       // 16-byte chunks of codes per token
+        const int kmax = lim_last + 1;    // keys past it are zeros
+        auto load = [&](bool is_v, int j) {
+            const uint8_t* codes = is_v ? v.vc : v.kc;
+            const uint8_t* params = is_v ? v.vp : v.kp;
+#pragma unroll
+            for (int i = 0; i < CPT; ++i) {
+                const int e = i * kPfDqThreads + t, tk = e / CPT, c = e % CPT, key = j * kPfKeys + tk;
+                const int page = key < kmax ? kv4_page(v, b, key) : -1;
+                const int slot = key & ((1 << v.page_shift) - 1);
+                const uint8_t* src = codes + (page >= 0 ? kv4_code_off<D>(v, page, kvh, slot) + 16 * c : 0);
+                uint8_t* dst = is_v ? sm + L::oRawV + (tk >> 3) * L::kVPitch + (tk & 7) * (D / 2) + 16 * c
+                                    : sm + L::oRawK + tk * (D / 2) + 16 * (D == 128 ? c ^ ((tk >> 1) & 3) : c ^ ((tk >> 2) & 1));
+                pf_cp16(dst, src, page >= 0 ? 16u : 0u);
+            }
+            if (t < L::kParK / 16) {  // parameters: 16 bytes are 2 (D = 128) or 4 tokens
+                constexpr int TPC = 256 / D;
+                const int tk = t * TPC, key = j * kPfKeys + tk;
+                const int page = key < kmax ? kv4_page(v, b, key) : -1;
+                const int slot = key & ((1 << v.page_shift) - 1);
+                const uint8_t* src = params + (page >= 0 ? kv4_param_off<D>(v, page, kvh, slot) : 0);
+                // tokens past the last key may hold anything: leave them out
+                const int live = min(max(kmax - key, 0), TPC);
+                uint8_t* dst = is_v ? sm + L::oParV + (tk >> 3) * L::kVParPitch + (tk & 7) * (D / 16) : sm + L::oParK + tk * (D / 16);
+                pf_cp16(dst, src, page >= 0 ? (uint32_t)(live * (D / 16)) : 0u);
+            }
+            asm volatile("cp.async.commit_group;" ::: "memory");
+        };
+        if (nt > 0) {
+            load(false, 0);
+            load(true, 0);
+        }
+        for (int j = 0; j < nt; ++j) {
+            const int s = j & 1;
+            // K: row t
+            asm volatile("cp.async.wait_group 1;" ::: "memory");
+            named_bar_sync(1, kPfDqThreads);
+            if (j >= 2) wait(&k_empty[s], ((j >> 1) & 1) ^ 1);
+            {
+                uint32_t cw[WPR];
+#pragma unroll
+                for (int c = 0; c < CPT; ++c) {
+                    const uint4 y = lds_u4(sm + L::oRawK + t * (D / 2) + 16 * (D == 128 ? c ^ ((t >> 1) & 3) : c ^ ((t >> 2) & 1)));
+                    cw[4 * c] = y.x; cw[4 * c + 1] = y.y; cw[4 * c + 2] = y.z; cw[4 * c + 3] = y.w;
+                }
+                __half2 sc[G], mn[G];
+                bool big = false;
+#pragma unroll
+                for (int g = 0; g < G; ++g) {
+                    const __half2 y = *reinterpret_cast<const __half2*>(sm + L::oParK + t * (D / 16) + 4 * g);
+                    sc[g] = __low2half2(y);
+                    mn[g] = __high2half2(y);
+                    big |= __half2float(__high2half(y)) + 15.f * __half2float(__low2half(y)) >= 65504.f;
+                }
+                uint8_t* K = sm + L::oK + s * L::kK;
+#pragma unroll
+                for (int i = 0; i < WPR; ++i) {
+                    const int g = i % G;
+                    __half2 h[4] = {pf_value(cw[i], false, sc[g], mn[g]), pf_value(cw[i], true, sc[g], mn[g]),
+                                    pf_value(cw[i] >> 8, false, sc[g], mn[g]), pf_value(cw[i] >> 8, true, sc[g], mn[g])};
+                    if (big) {
+#pragma unroll
+                        for (int q = 0; q < 4; ++q) h[q] = __hmin2(h[q], __float2half2_rn(65504.f));
+                    }
+                    *reinterpret_cast<uint4*>(K + pf_sw<kPfKeys>(t, 8 * g + i / G)) =
+                            make_uint4(pf_h2u(h[0]), pf_h2u(h[1]), pf_h2u(h[2]), pf_h2u(h[3]));
+                }
+            }
+            asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
+            named_bar_sync(1, kPfDqThreads);  // raw K is read out
+            if (j + 1 < nt) load(false, j + 1);
+            else asm volatile("cp.async.commit_group;" ::: "memory");
+            __syncwarp();
+            if (lane == 0) mbar_arrive(&k_full[s]);
+
+            // V: tokens 8 tg .. + 7, words of 8 elements of one or both groups
+            asm volatile("cp.async.wait_group 1;" ::: "memory");
+            named_bar_sync(1, kPfDqThreads);
+            if (j >= 2) wait(&v_empty[s], ((j >> 1) & 1) ^ 1);
+            {
+                const int tg = (lane & 7) + 8 * (w & 1), q8 = (lane >> 3) + 4 * (w >> 1);  // token group, word (pair)
+                uint32_t cw[8][G];
+                const uint8_t* src = sm + L::oRawV + tg * L::kVPitch + q8 * (4 * G);
+#pragma unroll
+                for (int i = 0; i < 8; ++i) {
+                    if (G == 2) {
+                        const uint2 y = *reinterpret_cast<const uint2*>(src + i * (D / 2));
+                        cw[i][0] = y.x;
+                        cw[i][G - 1] = y.y;
+                    } else {
+                        cw[i][0] = *reinterpret_cast<const uint32_t*>(src + i * (D / 2));
+                    }
+                }
+                uint32_t par[8][G];
+#pragma unroll
+                for (int i = 0; i < 8 * G / 4; ++i) {
+                    const uint4 y = lds_u4(sm + L::oParV + tg * L::kVParPitch + 16 * i);
+                    const uint32_t yy[4] = {y.x, y.y, y.z, y.w};
+#pragma unroll
+                    for (int e = 0; e < 4; ++e) par[(4 * i + e) / G][(4 * i + e) % G] = yy[e];
+                }
+                bool big = false;
+#pragma unroll
+                for (int i = 0; i < 8; ++i)
+#pragma unroll
+                    for (int g = 0; g < G; ++g) {
+                        const float2 y = __half22float2(pf_u2h(par[i][g]));
+                        big |= y.y + 15.f * y.x >= 65504.f;
+                    }
+                uint8_t* V = sm + L::oV + s * L::kK;
+#pragma unroll
+                for (int g = 0; g < G; ++g) {
+                    __half2 sc[4], mn[4];
+#pragma unroll
+                    for (int y = 0; y < 4; ++y) {
+                        sc[y] = pf_u2h(__byte_perm(par[2 * y][g], par[2 * y + 1][g], 0x5410));
+                        mn[y] = pf_u2h(__byte_perm(par[2 * y][g], par[2 * y + 1][g], 0x7632));
+                    }
+#pragma unroll
+                    for (int part = 0; part < 2; ++part) {
+                        uint32_t ww[4];
+#pragma unroll
+                        for (int y = 0; y < 4; ++y) ww[y] = __byte_perm(cw[2 * y][g], cw[2 * y + 1][g], part ? 0x7632 : 0x5410);
+#pragma unroll
+                        for (int e = 0; e < 4; ++e) {  // element 4 part + e
+                            __half2 h[4];
+#pragma unroll
+                            for (int y = 0; y < 4; ++y) h[y] = pf_value(e < 2 ? ww[y] : ww[y] >> 8, e & 1, sc[y], mn[y]);
+                            if (big) {
+#pragma unroll
+                                for (int y = 0; y < 4; ++y) h[y] = __hmin2(h[y], __float2half2_rn(65504.f));
+                            }
+                            *reinterpret_cast<uint4*>(V + pf_sw<D>(64 * g + 8 * q8 + 4 * part + e, tg)) =
+                                    make_uint4(pf_h2u(h[0]), pf_h2u(h[1]), pf_h2u(h[2]), pf_h2u(h[3]));
+                        }
+                    }
+                }
+            }
+            asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
+            named_bar_sync(1, kPfDqThreads);  // raw V is read out
+            if (j + 1 < nt) load(true, j + 1);
+            else asm volatile("cp.async.commit_group;" ::: "memory");
+            __syncwarp();
+            if (lane == 0) mbar_arrive(&v_full[s]);
+        }
+        asm volatile("cp.async.wait_group 0;" ::: "memory");
+    } else if (warp / 4 < ni) {
+        // ---- softmax of row tile i: thread = row
+        const int i = warp >> 2;
+        const uint32_t lane_base = (uint32_t)((warp & 3) * 32) << 16;
+        const uint32_t ts = tmem + lane_base + (uint32_t)(128 * i), to = tmem + lane_base + 256u + (uint32_t)(128 * i);
+        // tiles below `full` need no mask in this warp
+        const int full = (__reduce_min_sync(0xffffffffu, row_live ? lim : 0x7fffffff) + 1) / kPfKeys;
+        float ref = -1e30f;  // log2 units
+        uint64_t l2 = f2_pack(0.f, 0.f);
+        for (int j = 0; j < nt; ++j) {
+            // pages that are none mask their 16 keys (looked up before the wait: one per lane)
+            const int pk = j * kPfKeys + lane * 16;
+            const unsigned bad = __ballot_sync(0xffffffffu, lane < 8 && pk <= lim_last && kv4_page(v, b, pk) < 0);
+            wait(&s_full[i], j & 1);
+            tc_fence_after();
+            const bool mask = j >= full || bad != 0;
+            uint32_t x[32];
+            float mx = -INFINITY;
+            auto masked = [&](int c) {  // key j * 128 + c
+                return j * kPfKeys + c > lim || ((bad >> (c >> 4)) & 1u);
+            };
+#pragma unroll
+            for (int q = 0; q < 4; ++q) {
+                tc_ld32_issue(ts + 32 * q, x);
+                tc_ld32_wait(x);
+                if (!mask) {
+#pragma unroll
+                    for (int c = 0; c < 32; ++c) mx = fmaxf(mx, __uint_as_float(x[c]));
+                } else {
+#pragma unroll
+                    for (int c = 0; c < 32; ++c) mx = masked(32 * q + c) ? mx : fmaxf(mx, __uint_as_float(x[c]));
+                }
+            }
+            mx *= f;  // f > 0: the order stays; -inf stays (f = 0 is a dead row's)
+            if (!(mx > -1e30f)) mx = -1e30f;
+            const bool over = j == 0 || mx > ref + kPfLift;
+            if (__any_sync(0xffffffffu, over)) {
+                const float nref = fmaxf(ref, mx), corr = pf_ex2(ref - nref);
+                ref = nref;
+                if (j > 0) {
+                    l2 = f2_fma(l2, f2_pack(corr, corr), f2_pack(0.f, 0.f));
+#pragma unroll 1
+                    for (int q = 0; q < D / 32; ++q) {
+                        tc_ld32_issue(to + 32 * q, x);
+                        tc_ld32_wait(x);
+#pragma unroll
+                        for (int c = 0; c < 32; ++c) x[c] = __float_as_uint(__uint_as_float(x[c]) * corr);
+                        tc_st32(to + 32 * q, x);
+                    }
+                }
+            }
+            const uint64_t f2 = f2_pack(f, f), r2 = f2_pack(-ref, -ref);
+#pragma unroll
+            for (int q = 0; q < 4; ++q) {
+                tc_ld32_issue(ts + 32 * q, x);
+                tc_ld32_wait(x);
+                uint32_t pk16[16];
+#pragma unroll
+                for (int c = 0; c < 16; ++c) {
+                    const uint64_t y = f2_fma(f2_pack(__uint_as_float(x[2 * c]), __uint_as_float(x[2 * c + 1])), f2, r2);
+                    float a, bb;
+                    f2_unpack(y, a, bb);
+                    a = pf_ex2(a);
+                    bb = pf_ex2(bb);
+                    if (mask) {
+                        a = masked(32 * q + 2 * c) ? 0.f : a;
+                        bb = masked(32 * q + 2 * c + 1) ? 0.f : bb;
+                    }
+                    l2 = f2_add(l2, f2_pack(a, bb));
+                    pk16[c] = pf_h2u(__floats2half2_rn(a, bb));
+                }
+                tc_st_32x32b_x16_nowait(ts + 16 * q, pk16);
+            }
+            asm volatile("tcgen05.wait::st.sync.aligned;" ::: "memory");
+            tc_fence_before();
+            __syncwarp();
+            if (lane == 0) mbar_arrive(&p_full[i]);
+        }
+        // ---- out = O / l
+        float la, lb;
+        f2_unpack(l2, la, lb);
+        const float l = la + lb, inv = l > 0.f ? 1.f / l : 0.f;
+        if (nt > 0) {
+            wait(&o_full[i], 0);
+            tc_fence_after();
+        }
+        __nv_bfloat16* op = static_cast<__nv_bfloat16*>(p.out) + (int64_t)(row0 + tok) * p.os + (int64_t)head * D;
+#pragma unroll
+        for (int q = 0; q < D / 32; ++q) {
+            uint32_t x[32];
+            if (nt > 0) {
+                tc_ld32_issue(to + 32 * q, x);
+                tc_ld32_wait(x);
+            }
+            uint32_t y[16];
+#pragma unroll
+            for (int c = 0; c < 16; ++c) {
+                const float a = nt > 0 && l > 0.f ? __uint_as_float(x[2 * c]) * inv : 0.f;
+                const float bb = nt > 0 && l > 0.f ? __uint_as_float(x[2 * c + 1]) * inv : 0.f;
+                __nv_bfloat162 h = __floats2bfloat162_rn(a, bb);
+                y[c] = *reinterpret_cast<uint32_t*>(&h);
+            }
+            if (!row_live || !ok) continue;
+            if (p.vec) {
+#pragma unroll
+                for (int c = 0; c < 4; ++c)
+                    *reinterpret_cast<uint4*>(op + 32 * q + 8 * c) = make_uint4(y[4 * c], y[4 * c + 1], y[4 * c + 2], y[4 * c + 3]);
+            } else {
+#pragma unroll
+                for (int c = 0; c < 32; ++c)
+                    reinterpret_cast<uint16_t*>(op)[32 * q + c] = (uint16_t)(y[c / 2] >> (16 * (c & 1)));
+            }
+        }
+    }
+    tc_fence_before();
+    __syncthreads();
+    if (warp == 12) {
+        tc_fence_after();
+        asm volatile("tcgen05.dealloc.cta_group::1.sync.aligned.b32 %0, %1;" ::"r"(tmem), "r"(512) : "memory");
+    }
+}
+
+template <int D>
+static void launch_prefill(const Kv4AttnParams& p, unsigned ctas, cudaStream_t s) {
+    set_func_attr_once(reinterpret_cast<const void*>(&kv4_prefill_kernel<D>), cudaFuncAttributeMaxDynamicSharedMemorySize,
+                       PfLayout<D>::kTotal);
+    launch_pdl(kv4_prefill_kernel<D>, dim3(ctas), dim3(kPfThreads), PfLayout<D>::kTotal, s, p, device_error_word());
+}
+
+bool kv4_prefill_wanted(const Kv4View& v, int64_t grp) {
+    const int64_t cols = v.rows * grp, tiles = (cols / kPfRows + v.n_seq) * v.nkv;
+    // One wave of row tiles takes about as long per key as 1.5 eight-column
+    // tiles of the other kernel on every SM (2500 cycles per 128 keys against
+    // 207 per 16): take it once there are more columns than that.
+    const int64_t sms = num_sms();
+    return ceil_div(cols, 8) * v.nkv * 2 > 3 * sms * ceil_div(tiles, sms);
+}
+
+am_status_code kv4_prefill_launch(const Kv4AttnParams& p, int64_t d, cudaStream_t s) {
+    const int64_t ctas = ((int64_t)p.v.rows * p.grp / kPfRows + p.v.n_seq) * p.v.nkv;  // at least as many as there are row tiles
+    AMCU_REQUIRE(ctas <= INT32_MAX, "amcu_attn_kv4: too many rows");
+    d == 64 ? launch_prefill<64>(p, (unsigned)ctas, s) : launch_prefill<128>(p, (unsigned)ctas, s);
+    return check_launch("amcu_attn_kv4");
+}
+
+}  // namespace amcu

@@ -121,6 +121,90 @@ def test_attention(ops, lens, nq, nkv, d, page, dtype):
     assert torch.equal(got, again)  # no atomics decide a result
 
 
+PROMPTS = [  # enough rows for the kernel of prompts
+    ([(60, 60)], 32, 8, 128, 16),
+    ([(128, 64)], 32, 8, 128, 64),
+    ([(129, 65), (300, 64), (3, 1), (0, 0), (257, 63)], 32, 8, 128, 32),
+    ([(200, 100), (383, 33)], 64, 8, 128, 16),
+    ([(385, 129), (90, 2)], 32, 8, 64, 256),
+    ([(77, 77), (400, 1), (400, 60)], 56, 8, 64, 16),
+    ([(513, 100)], 16, 16, 64, 128),
+    ([(130, 70)], 72, 8, 128, 16),
+]
+
+
+@pytest.mark.parametrize("lens,nq,nkv,d,page", PROMPTS)
+def test_attention_prompts(ops, lens, nq, nkv, d, page):
+    rng = np.random.default_rng(len(lens) * 100 + lens[0][0])
+    table, start, ctx, total = make_batch(lens, page, rng)
+    cache = random_cache(total, nkv, page, d, rng)
+    poison_unused(cache, table, ctx)
+    q = rng.normal(0, 1.5, (start[-1], nq * d)).astype(np.float32)
+    q[0, :d] = 0
+    q[-1, -d:] *= 30  # one head whose scores are far apart
+    q = bf16(q)
+    want = ref.attention(q.double().numpy(), cache, table, start, ctx, nq, nkv, d)
+    out = torch.full((start[-1], nq * d), float("nan"), dtype=torch.bfloat16, device="cuda")
+    got = ops.attention_kv4(q.cuda(), dev(cache), di(table), di(start), di(ctx), nq, nkv, d, out=out)
+    check_attention(got, want, torch.bfloat16, 4.0)
+    again = ops.attention_kv4(q.cuda(), dev(cache), di(table), di(start), di(ctx), nq, nkv, d)
+    assert torch.equal(got, again)
+
+
+def test_attention_prompts_rising_scores(ops):
+    """Scores that grow along the keys, so that the softmax reference moves many times."""
+    rng = np.random.default_rng(31)
+    nq, nkv, d, page = 32, 8, 128, 64
+    table, start, ctx, total = make_batch([(700, 64)], page, rng)
+    kc, kp, vc, vp = random_cache(total, nkv, page, d, rng)
+    for i in range(700):
+        kp[table[0, i // page], :, i % page, :, 1] += np.float16(0.01 * i)
+    q = bf16(np.abs(rng.normal(0, 1, (64, nq * d))))
+    want = ref.attention(q.double().numpy(), (kc, kp, vc, vp), table, start, ctx, nq, nkv, d)
+    got = ops.attention_kv4(q.cuda(), dev((kc, kp, vc, vp)), di(table), di(start), di(ctx), nq, nkv, d)
+    got = got.double().cpu().numpy()
+    # scores of hundreds from keys rounded to 11 bits: an absolute error of some 2^-5 in the exponent
+    assert np.linalg.norm(got - want) <= 2.0 ** -4 * np.linalg.norm(want)
+
+
+def test_attention_prompts_strides_and_missing_pages(ops):
+    """Unaligned rows, a page that is none and a context past the page table, with many rows."""
+    rng = np.random.default_rng(32)
+    nq, nkv, d, page = 32, 8, 64, 16
+    table, start, ctx, total = make_batch([(300, 70), (20, 40)], page, rng, pages=19)
+    cache = random_cache(total, nkv, page, d, rng)
+    table[0, 2], table[0, 9] = -3, total + 5
+    ctx[0] = 19 * 16 + 9
+    wide = bf16(rng.normal(0, 1, (110, nq * d + 7))).cuda()
+    q = wide[:, 3: 3 + nq * d]
+    want = ref.attention(q.double().cpu().numpy(), cache, table, start, ctx, nq, nkv, d)
+    out = torch.zeros(110, nq * d + 5, dtype=torch.bfloat16, device="cuda")
+    status = torch.zeros(1, dtype=torch.int32, device="cuda")
+    ops.attention_kv4(q, dev(cache), di(table), di(start), di(ctx), nq, nkv, d, out=out[:, 1: 1 + nq * d],
+                      status=status)
+    check_attention(out[:, 1: 1 + nq * d], want, torch.bfloat16, 4.0)
+    assert (out[:, 0] == 0).all() and (out[:, 1 + nq * d:] == 0).all()
+    assert (out[start[1]: start[1] + 20] == 0).all()
+    assert status.item() == 11
+
+
+def test_attention_prompts_largest_values(ops):
+    """Elements at and beyond fp16's largest value stay finite."""
+    rng = np.random.default_rng(33)
+    nq, nkv, d, page = 32, 8, 128, 16
+    table, start, ctx, total = make_batch([(100, 60)], page, rng)
+    kc, kp, vc, vp = random_cache(total, nkv, page, d, rng)
+    vp[..., 0], vp[..., 1] = np.float16(4366), np.float16(0)
+    kp[..., 0], kp[..., 1] = np.float16(4000), np.float16(-30000)
+    q = bf16(rng.normal(0, 1e-5, (60, nq * d)))
+    want = ref.attention(q.double().numpy(), (kc, kp, vc, vp), table, start, ctx, nq, nkv, d)
+    got = ops.attention_kv4(q.cuda(), dev((kc, kp, vc, vp)), di(table), di(start), di(ctx), nq, nkv, d)
+    assert np.linalg.norm(got.double().cpu().numpy() - want) <= 2.0 ** -7 * np.linalg.norm(want)
+    vp[..., 1] = np.float16(30000)  # 30000 + 15 * 4366 is beyond fp16: taken as 65504
+    got = ops.attention_kv4(q.cuda(), dev((kc, kp, vc, vp)), di(table), di(start), di(ctx), nq, nkv, d)
+    assert torch.isfinite(got).all()
+
+
 @pytest.mark.parametrize("dtype", [torch.bfloat16, torch.float32])
 @pytest.mark.parametrize("big", [1.0, 60.0])
 def test_attention_sharp_and_flat(ops, dtype, big):
