@@ -245,6 +245,29 @@ def lib() -> C.CDLL:
     return _lib
 
 
+_native = None
+
+
+def native():
+    """The extension module of the small calls (lib/_ops_native.so), bound to lib()."""
+    global _native
+    if _native is None:
+        import importlib.machinery
+        import importlib.util
+        path = Path(__file__).resolve().parent / "lib" / "_ops_native.so"
+        if not path.exists():
+            raise RuntimeError(f"aethermind_b200 native binding not built ({path}); "
+                               "run `python -m aethermind_b200.build`")
+        loader = importlib.machinery.ExtensionFileLoader("_ops_native", str(path))
+        m = importlib.util.module_from_spec(importlib.util.spec_from_loader("_ops_native", loader))
+        loader.exec_module(m)
+        l = lib()
+        m.bind(*(C.cast(f, C.c_void_p).value for f in (l.amcu_sample, l.amcu_kv4_append, l.amcu_kv4_gather,
+                                                       l.amcu_attn_kv4_workspace_bytes, l.amcu_attn_kv4)))
+        _native = m
+    return _native
+
+
 def exported_symbols() -> list[str]:
     return list(_SIGS)
 

@@ -23,6 +23,7 @@ INCLUDE = ROOT / "include"
 OBJ_DIR = PKG / "_build"
 LIB_DIR = PKG / "lib"
 LIB = LIB_DIR / "libaethermind_b200.so"
+NATIVE = LIB_DIR / "_ops_native.so"
 
 ARCH = ["-gencode", "arch=compute_100a,code=sm_100a"]
 
@@ -80,6 +81,7 @@ def _compile(src: Path, hdr: str, verbose: bool) -> Path:
 
 
 def build(verbose: bool = False) -> Path:
+    build_native()
     OBJ_DIR.mkdir(exist_ok=True)
     LIB_DIR.mkdir(exist_ok=True)
     hdr = _headers_digest()
@@ -102,6 +104,33 @@ def build(verbose: bool = False) -> Path:
         if o.name not in keep:
             o.unlink()
     return LIB
+
+
+def build_native() -> Path:
+    """The CPython extension lib/_ops_native.so (csrc_python/ops_native.cpp), against
+    the headers of the torch that is installed."""
+    import sysconfig
+
+    import torch
+    src = PKG / "csrc_python" / "ops_native.cpp"
+    base = Path(torch.__file__).resolve().parent
+    cmd = [_host_cxx(), "-std=c++20", "-O2", "-fPIC", "-shared", "-fvisibility=hidden",
+           f"-D_GLIBCXX_USE_CXX11_ABI={int(torch._C._GLIBCXX_USE_CXX11_ABI)}", f"-I{INCLUDE}",
+           "-isystem", str(base / "include"), "-isystem", str(base / "include" / "torch" / "csrc" / "api" / "include"),
+           "-isystem", sysconfig.get_paths()["include"], "-isystem", str(Path(_nvcc()).resolve().parent.parent / "include"),
+           str(src), "-o", str(NATIVE), f"-L{base / 'lib'}", "-ltorch_python", "-ltorch", "-ltorch_cpu", "-lc10_cuda",
+           "-lc10"]
+    stamp = hashlib.sha256((" ".join(cmd) + torch.__version__).encode() + src.read_bytes()
+                           + b"".join(p.read_bytes() for p in sorted(INCLUDE.glob("*.h")))).hexdigest()
+    stamp_file = LIB_DIR / ".native_stamp"
+    if NATIVE.exists() and stamp_file.exists() and stamp_file.read_text() == stamp:
+        return NATIVE
+    LIB_DIR.mkdir(exist_ok=True)
+    r = subprocess.run(cmd, capture_output=True, text=True)
+    if r.returncode != 0:
+        raise RuntimeError(f"compile failed: {src}\n{r.stdout}\n{r.stderr}")
+    stamp_file.write_text(stamp)
+    return NATIVE
 
 
 if __name__ == "__main__":

@@ -16,7 +16,7 @@ from typing import NamedTuple
 import torch
 
 from . import _lib as L
-from ._lib import check, lib
+from ._lib import check, lib, native
 
 _DT = {torch.float32: L.F32, torch.bfloat16: L.BF16, torch.int32: L.I32, torch.int64: L.I64}
 
@@ -331,6 +331,13 @@ def embedding(ids: torch.Tensor, table: torch.Tensor, row_scales: torch.Tensor |
 
 
 # ------------------------------------------------------------------ sampling
+def _done(r, what: str):
+    """The native binding's outputs; a status code of the C ABI raises AmError."""
+    if r.__class__ is int:
+        check(r, what)
+    return r
+
+
 def sample(logits: torch.Tensor, uniform: torch.Tensor, temperature: torch.Tensor | None = None,
            top_k: torch.Tensor | None = None, top_p: torch.Tensor | None = None, min_p: torch.Tensor | None = None,
            with_prob: bool = False, out: torch.Tensor | None = None):
@@ -339,21 +346,7 @@ def sample(logits: torch.Tensor, uniform: torch.Tensor, temperature: torch.Tenso
 
     The settings are float32 (top_k: int32) tensors [rows]; None is off. Returns
     int64 tokens [rows], or (tokens, float32 probabilities among the kept)."""
-    _require_here(logits, uniform, temperature, top_k, top_p, min_p, out)
-    if (logits.dim() != 2 or (logits.stride(1) != 1 and logits.shape[1] > 1)
-            or (logits.stride(0) < logits.shape[1] and logits.shape[0] > 1)):
-        raise ValueError("sample takes logits [rows, vocab] with contiguous rows that do not overlap")
-    rows, vocab = logits.shape
-    for t, dt in ((uniform, torch.float32), (temperature, torch.float32), (top_k, torch.int32),
-                  (top_p, torch.float32), (min_p, torch.float32), (out, torch.int64)):
-        if t is not None and (t.dtype != dt or t.shape != (rows,) or not t.is_contiguous()):
-            raise ValueError(f"sample takes one contiguous {dt} per row")
-    idx = out if out is not None else torch.empty(rows, dtype=torch.int64, device=logits.device)
-    prob = torch.empty(rows, dtype=torch.float32, device=logits.device) if with_prob else None
-    a = L.AmcuSampleArgs(_p(logits), logits.stride(0), rows, vocab, _dt(logits), _p(uniform), _p(temperature),
-                         _p(top_k), _p(top_p), _p(min_p), _p(idx), _p(prob))
-    check(lib().amcu_sample(C.byref(a), _stream()), "amcu_sample")
-    return (idx, prob) if with_prob else idx
+    return _done(native().sample(logits, uniform, temperature, top_k, top_p, min_p, bool(with_prob), out), "amcu_sample")
 
 
 # ------------------------------------------------------------------ 4-bit paged KV cache
@@ -375,53 +368,6 @@ def kv4_cache(num_pages: int, page_size: int, n_kv: int, head_dim: int, device="
     return Kv4Cache(*plane(), *plane())
 
 
-def _require_here(*ts: torch.Tensor | None) -> None:
-    """CUDA tensors of the current device: the launch goes to its current stream."""
-    here = torch.cuda.current_device() if torch.cuda.is_available() else None
-    for t in ts:
-        if t is not None and (not t.is_cuda or t.device.index != here):
-            raise ValueError("aethermind_b200 ops take CUDA tensors of the current device")
-
-
-def _kv4(cache, page_table, row_start, ctx_len, rows, n_kv, head_dim, status):
-    """The checked AmcuKv4Cache and AmcuKv4Batch of a call."""
-    kc, kp, vc, vp = cache
-    _require_here(kc, kp, vc, vp, page_table, row_start, ctx_len, status)
-    pages, page = kc.shape[0], kc.shape[2] if kc.dim() == 4 else 0
-    groups = head_dim // 64
-    for t, dt, shape in ((kc, torch.uint8, (pages, n_kv, page, head_dim // 2)),
-                         (vc, torch.uint8, (pages, n_kv, page, head_dim // 2)),
-                         (kp, torch.float16, (pages, n_kv, page, groups, 2)),
-                         (vp, torch.float16, (pages, n_kv, page, groups, 2))):
-        if t.dtype != dt or t.shape != shape:
-            raise ValueError(f"kv4 cache: expected {dt} {list(shape)}, got {t.dtype} {list(t.shape)}")
-    cs, ps = kc.stride(), kp.stride()
-    if pages > 1 and (cs[0] < n_kv * page * head_dim // 2 or ps[0] < n_kv * page * groups * 2):
-        raise ValueError("kv4 cache: pages overlap")
-    if (vc.stride() != cs or vp.stride() != ps or cs[1:] != (page * head_dim // 2, head_dim // 2, 1)
-            or ps[1:] != (page * groups * 2, groups * 2, 2, 1)):
-        raise ValueError("kv4 cache: pages are contiguous inside, and K's and V's strides are the same")
-    n_seq = ctx_len.shape[0] if ctx_len.dim() == 1 else -1
-    if (page_table.dtype != torch.int32 or row_start.dtype != torch.int32 or ctx_len.dtype != torch.int32
-            or page_table.dim() != 2 or page_table.shape[0] != n_seq or row_start.shape != (n_seq + 1,)
-            or (page_table.stride(1) != 1 and page_table.shape[1] > 1)
-            or (page_table.stride(0) < page_table.shape[1] and n_seq > 1)
-            or not row_start.is_contiguous() or not ctx_len.is_contiguous()):
-        raise ValueError("kv4: int32 page_table [n_seq, pages], row_start [n_seq + 1] and ctx_len [n_seq]")
-    if status is not None and status.dtype != torch.int32:
-        raise ValueError("kv4: status is one int32")
-    return (L.AmcuKv4Cache(_p(kc), _p(kp), _p(vc), _p(vp), cs[0], 2 * ps[0], pages, page, n_kv, head_dim),
-            L.AmcuKv4Batch(_p(page_table), page_table.stride(0), page_table.shape[1], _p(row_start), _p(ctx_len),
-                           n_seq, rows, _p(status)))
-
-
-def _rows_of(t: torch.Tensor, width: int, dtype: torch.dtype, what: str, written: bool = False) -> None:
-    if t.dim() != 2 or t.shape[1] != width or t.stride(1) != 1 or t.dtype != dtype:
-        raise ValueError(f"{what}: expected {dtype} rows of {width} contiguous elements")
-    if written and t.shape[0] > 1 and t.stride(0) < width:
-        raise ValueError(f"{what}: rows overlap")
-
-
 def kv4_append(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, cache: Kv4Cache, page_table: torch.Tensor,
                row_start: torch.Tensor, ctx_len: torch.Tensor, cos_sin: torch.Tensor, n_q: int, n_kv: int,
                head_dim: int, q_norm: torch.Tensor | None = None, k_norm: torch.Tensor | None = None,
@@ -432,28 +378,8 @@ def kv4_append(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, cache: Kv4Cach
     into their pages. Row r of sequence b's n rows (row_start) is at position
     ctx_len[b] - n + r; ctx_len counts them already. cos_sin: rope_table's
     [positions, head_dim/2, 2]. Returns the rotated q (q_out may be q)."""
-    _require_here(q, k, v, cos_sin, q_norm, k_norm, q_out)
-    rows = q.shape[0]
-    _rows_of(q, n_q * head_dim, q.dtype, "q")
-    _rows_of(k, n_kv * head_dim, q.dtype, "k")
-    _rows_of(v, n_kv * head_dim, q.dtype, "v")
-    if k.shape[0] != rows or v.shape[0] != rows:
-        raise ValueError("kv4_append: q, k and v have as many rows")
-    if cos_sin.dtype != torch.float32 or not cos_sin.is_contiguous() or cos_sin.shape[1:] != (head_dim // 2, 2):
-        raise ValueError("kv4_append: cos_sin is float32 [positions, head_dim/2, 2]")
-    for w in (q_norm, k_norm):
-        if w is not None and (w.dtype != q.dtype or w.shape != (head_dim,) or not w.is_contiguous()):
-            raise ValueError("kv4_append: norm weights are [head_dim] of q's type")
-    if q_out is None:
-        q_out = torch.empty(rows, n_q * head_dim, dtype=q.dtype, device=q.device)
-    _rows_of(q_out, n_q * head_dim, q.dtype, "q_out", written=True)
-    if q_out.shape[0] != rows:
-        raise ValueError("kv4_append: q_out has as many rows as q")
-    c, b = _kv4(cache, page_table, row_start, ctx_len, rows, n_kv, head_dim, status)
-    a = L.AmcuKv4AppendArgs(c, b, _p(q), _p(k), _p(v), _p(q_out), q.stride(0), k.stride(0), v.stride(0),
-                            q_out.stride(0), _p(q_norm), _p(k_norm), eps, _dt(q), _p(cos_sin), cos_sin.shape[0], n_q)
-    check(lib().amcu_kv4_append(C.byref(a), _stream()), "amcu_kv4_append")
-    return q_out
+    return _done(native().kv4_append(q, k, v, cache, page_table, row_start, ctx_len, cos_sin, n_q, n_kv, head_dim,
+                                     q_norm, k_norm, eps, q_out, status), "amcu_kv4_append")
 
 
 def kv4_gather(cache: Kv4Cache, page_table: torch.Tensor, row_start: torch.Tensor, ctx_len: torch.Tensor, rows: int,
@@ -461,12 +387,10 @@ def kv4_gather(cache: Kv4Cache, page_table: torch.Tensor, row_start: torch.Tenso
                status: torch.Tensor | None = None) -> tuple[torch.Tensor, torch.Tensor]:
     """The call's rows of a 4-bit paged cache as the keys and values they stand
     for, each [rows, n_kv * head_dim] (amcu_kv4_gather)."""
-    c, b = _kv4(cache, page_table, row_start, ctx_len, rows, n_kv, head_dim, status)
-    k = torch.empty(rows, n_kv * head_dim, dtype=dtype, device=ctx_len.device)
-    v = torch.empty_like(k)
-    a = L.AmcuKv4GatherArgs(c, b, _p(k), _p(v), k.stride(0), v.stride(0), _DT[dtype])
-    check(lib().amcu_kv4_gather(C.byref(a), _stream()), "amcu_kv4_gather")
-    return k, v
+    if dtype not in (torch.bfloat16, torch.float32):
+        raise ValueError("kv4_gather: float32 or bfloat16")
+    return _done(native().kv4_gather(cache, page_table, row_start, ctx_len, rows, n_kv, head_dim,
+                                     dtype == torch.float32, status), "amcu_kv4_gather")
 
 
 def attention_kv4(q: torch.Tensor, cache: Kv4Cache, page_table: torch.Tensor, row_start: torch.Tensor,
@@ -474,20 +398,5 @@ def attention_kv4(q: torch.Tensor, cache: Kv4Cache, page_table: torch.Tensor, ro
                   out: torch.Tensor | None = None, status: torch.Tensor | None = None) -> torch.Tensor:
     """Causal GQA attention of the call's rows over a 4-bit paged cache that holds
     them already (amcu_attn_kv4). scale 0: 1 / sqrt(head_dim)."""
-    _require_here(q, out)
-    _rows_of(q, n_q * head_dim, q.dtype, "q")
-    rows = q.shape[0]
-    o = out if out is not None else torch.empty(rows, n_q * head_dim, dtype=q.dtype, device=q.device)
-    _rows_of(o, n_q * head_dim, q.dtype, "out", written=True)
-    if o.shape[0] != rows:
-        raise ValueError("attention_kv4: out has as many rows as q")
-    c, b = _kv4(cache, page_table, row_start, ctx_len, rows, n_kv, head_dim, status)
-    a = L.AmcuKv4AttentionArgs(c, b, _p(q), q.stride(0), _p(o), o.stride(0), n_q, scale, _dt(q), None, 0)
-    nb = lib().amcu_attn_kv4_workspace_bytes(C.byref(a))
-    ws = None
-    if nb:
-        ws = torch.empty(nb, dtype=torch.uint8, device=q.device)
-        a.workspace, a.workspace_size = _p(ws), nb
-    check(lib().amcu_attn_kv4(C.byref(a), _stream()), "amcu_attn_kv4")
-    del ws
-    return o
+    return _done(native().attention_kv4(q, cache, page_table, row_start, ctx_len, n_q, n_kv, head_dim, scale, out,
+                                        status), "amcu_attn_kv4")

@@ -113,3 +113,19 @@ def test_reference_rows_round_trip():
     v = ref.values(ref.pack_rows(code), par)
     span = x.reshape(9, 2, 64).max(-1) - x.reshape(9, 2, 64).min(-1)
     assert (np.abs(v - x).reshape(9, 2, 64).max(-1) <= span / 30 * 1.01 + 2e-3).all()
+
+
+def test_front_end_wants_cuda_tensors(built_lib):
+    torch = pytest.importorskip("torch")
+    from aethermind_b200 import ops
+    x, i = torch.zeros(2, 64), torch.zeros(2, dtype=torch.int32)
+    with pytest.raises(ValueError):
+        ops.sample(x, x[0])
+    with pytest.raises(ValueError):
+        ops.attention_kv4(x, (i, i, i, i), i, i, i, 1, 1, 64)
+    with pytest.raises(ValueError):
+        ops.kv4_append(None, x, x, (i, i, i, i), i, i, i, x, 1, 1, 64)
+    with pytest.raises(ValueError):
+        ops.kv4_gather((i, i, i, i), i, i, i, 2, 1, 64)
+    with pytest.raises(ValueError):
+        ops.kv4_gather((i, i, i, i), i, i, i, 2, 1, 64, dtype=torch.float64)
