@@ -31,8 +31,11 @@ namespace cg = cooperative_groups;
 constexpr int kSampleThreads = 512;
 constexpr int kSampleWarps = kSampleThreads / 32;
 constexpr int kSampleBins = 256;
-constexpr int kSampleList = kSampleThreads;       // candidates of a cut that are ranked against one another
-constexpr int kSampleSlice = 16384;               // most keys that a CTA keeps in shared memory
+constexpr int kSampleList = kSampleThreads;       // most candidates that are sorted
+constexpr int kSampleWarpList = 64;               // of one warp's tokens
+constexpr int kSamplePlace = 9;                   // bits of a place among them
+constexpr int kSampleTop = 256;                   // largest top-k whose tokens are gathered
+constexpr int kSampleSlice = 16384;               // most logits that a CTA keeps in shared memory
 constexpr float kSampleOne = 1099511627776.f;     // 2^40
 constexpr float kSampleBinScale = kSampleBins / 28.f;  // weights end at z = -27.7
 constexpr uint32_t kSampleNever = 0x7f800000u;    // key of a masked token
@@ -43,35 +46,55 @@ __device__ __forceinline__ uint32_t sample_key(float x, float mx, float t) {
     const float z = __fdiv_rn(__fsub_rn(x, mx), t);
     return z <= 0.f ? __float_as_uint(-z) & 0x7fffffffu : kSampleNever;  // NaN: comparison is false
 }
+// floor(expf(-|z|) * 2^40), from the float's fields (a 64-bit conversion is slow).
 __device__ __forceinline__ u64 sample_weight(uint32_t key) {
-    return (u64)__fmul_rn(expf(-__uint_as_float(key)), kSampleOne);
+    const uint32_t f = __float_as_uint(expf(-__uint_as_float(key)));
+    const uint32_t m = (f & 0x007fffffu) | 0x00800000u;
+    const int sh = (int)(f >> 23) - 110;
+    return sh >= 0 ? (u64)m << sh : (u64)(sh > -24 ? m >> -sh : 0u);
 }
 // Position of a key on a scale of 256 bins; bin and sub-bin are monotone in the key.
 __device__ __forceinline__ float sample_place(uint32_t key) { return __fmul_rn(__uint_as_float(key), kSampleBinScale); }
-__device__ __forceinline__ int sample_bin(float place) { return min((int)place, kSampleBins - 1); }
+__device__ __forceinline__ int sample_bin(float place) { return (int)fminf(place, (float)(kSampleBins - 1)); }
 __device__ __forceinline__ int sample_sub(float place, int bin) {
     return min((int)__fmul_rn(__fsub_rn(place, (float)bin), 256.f), kSampleBins - 1);
 }
 
 struct SampleShared {
-    u64 mass[2][kSampleBins];
+    uint32_t mass[2][3][kSampleBins];  // a weight's bits 0-13, 14-27 and 28-40 (64-bit shared atomics are far slower)
     uint32_t count[2][kSampleBins];
-    u64 list[kSampleList];       // this CTA's candidates
+    float group[kSampleThreads];       // maxima of the threads, or of 2, 4 or 8 neighbours
+    u64 list[kSampleWarps][kSampleWarpList];  // each warp's candidates
+    uint32_t n_list[kSampleWarps];
     u64 all[kSampleList];        // every CTA's
+    u64 weight[kSampleList];     // by place: weights of the kept
+    u64 tmp[kSampleList];
     u64 part[kSampleWarps];
     u64 scan[kSampleBins / 32];
     u64 xchg[2];
-    float mx;
-    float red[kSampleWarps];
-    uint32_t n_list, kmin, kmax;
-    u64 cut, before;
+    uint32_t kmin, kmax;
+    u64 top, cut, before;
     uint32_t members;
-    int bin, where;
+    int bin;
 };
 
 __device__ __forceinline__ u64 warp_sum_u64(u64 v) {
 #pragma unroll
     for (int o = 16; o > 0; o >>= 1) v += __shfl_xor_sync(0xffffffffu, v, o);
+    return v;
+}
+__device__ __forceinline__ u64 warp_max_u64(u64 v) {
+#pragma unroll
+    for (int o = 16; o > 0; o >>= 1) v = max(v, __shfl_xor_sync(0xffffffffu, v, o));
+    return v;
+}
+__device__ __forceinline__ u64 warp_scan_u64(u64 v) {  // inclusive
+    const int lane = threadIdx.x & 31;
+#pragma unroll
+    for (int o = 1; o < 32; o <<= 1) {
+        const u64 z = __shfl_up_sync(0xffffffffu, v, o);
+        if (lane >= o) v += z;
+    }
     return v;
 }
 
@@ -81,7 +104,8 @@ struct SampleTeam {
     cg::cluster_group cl;
     int rank, C, turn;
 
-    __device__ __forceinline__ u64 at(int r, const u64* p) { return *cl.map_shared_rank(const_cast<u64*>(p), r); }
+    template <typename V>
+    __device__ __forceinline__ V at(int r, const V* p) { return *cl.map_shared_rank(const_cast<V*>(p), r); }
 
     // Sum over the cluster; `before`: of the ranks below this one. One cluster barrier.
     __device__ u64 sum(u64 v, u64* before = nullptr) {
@@ -93,19 +117,112 @@ struct SampleTeam {
             v = warp_sum_u64(lane < kSampleWarps ? s->part[lane] : 0);
             if (lane == 0) s->xchg[turn & 1] = v;
         }
+        return gather(before);
+    }
+    // The same once xchg[turn & 1] holds this CTA's value.
+    __device__ u64 gather(u64* before) {
+        const int lane = threadIdx.x & 31;
         cl.sync();
         const u64 x = lane < C ? at(lane, &s->xchg[turn & 1]) : 0;
         ++turn;
         if (before) *before = warp_sum_u64(lane < rank ? x : 0);
         return warp_sum_u64(x);
     }
+
+    // Every warp's list (in index order, as the warps and CTAs are) into all[],
+    // members as (key, index, place in all[]); returns their number, or -1 where
+    // they are too many.
+    __device__ int collect() {
+        cl.sync();
+        int n = 0;
+        for (int first = 0; first < C * kSampleWarps; first += kSampleThreads) {  // one list per thread (C <= 16: once)
+            const int q = first + threadIdx.x, r = q / kSampleWarps;
+            const int m = q < C * kSampleWarps ? (int)at(r, &s->n_list[q % kSampleWarps]) : 0;
+            u64 all;
+            const bool bad = __syncthreads_or(m > kSampleWarpList);
+            int o = n + (int)scan((u64)m, all) - m;
+            n += (int)all;
+            if (bad || n > kSampleList) return -1;
+            for (int i = 0; i < m; ++i, ++o) {
+                const u64 c = at(r, &s->list[q % kSampleWarps][i]);
+                s->all[o] = (c & 0xffffffff00000000ull) | ((c & 0x3fffffu) << kSamplePlace) | (u64)o;
+            }
+        }
+        __syncthreads();
+        return n;
+    }
+
+    // all[0 .. m) in ascending order, one per thread (~0 past the end): up to 128
+    // by counting the smaller ones (0.3 us for 64 against 1.0 for the sort), more
+    // by a bitonic sort of the next power of two, strides below a warp by shuffles.
+    __device__ u64 sorted(int m) {
+        const int tid = threadIdx.x;
+        if (m <= 128) {
+            if (tid < m) {
+                const u64 me = s->all[tid];
+                int less = 0;
+#pragma unroll 8
+                for (int j = 0; j < m; ++j) less += s->all[j] < me;
+                s->tmp[less] = me;
+            }
+            __syncthreads();
+            return tid < m ? s->tmp[tid] : ~0ull;
+        }
+        int P = 32;
+        while (P < m) P *= 2;
+        u64 v = tid < m ? s->all[tid] : ~0ull;
+        for (int size = 2; size <= P; size *= 2) {
+            for (int stride = size / 2; stride > 0; stride /= 2) {
+                u64 o;
+                if (stride < 32) {
+                    if (tid >= P) continue;
+                    o = __shfl_xor_sync(0xffffffffu, v, stride);
+                } else {
+                    if (tid < P) s->tmp[tid] = v;
+                    __syncthreads();
+                    o = tid < P ? s->tmp[tid ^ stride] : 0;
+                    __syncthreads();
+                }
+                const bool low = (tid & stride) == 0, up = (tid & size) == 0;
+                if ((v < o) != (low == up)) v = o;
+            }
+        }
+        return tid < P ? v : ~0ull;
+    }
+
+    // Running total of v over the block's threads, and the block's.
+    __device__ u64 scan(u64 v, u64& all) {
+        const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
+        const u64 inc = warp_scan_u64(v);
+        if (lane == 31) s->part[warp] = inc;
+        __syncthreads();
+        u64 b = 0;
+        all = 0;
+#pragma unroll
+        for (int w = 0; w < kSampleWarps; ++w) {
+            const u64 y = s->part[w];
+            if (w < warp) b += y;
+            all += y;
+        }
+        __syncthreads();
+        return b + inc;
+    }
 };
 
-// One cluster per row, its CTAs each holding a contiguous slice of the keys in
-// shared memory (kRes; larger vocabularies compute them again from the logits).
+// One cluster per row, its CTAs each holding a contiguous slice of the row in
+// shared memory as fp32 (kRes; larger vocabularies read the logits again).
+//
+// * Greedy rows, top-k 1: the (logit, index) maximum is the answer.
+// * top-k up to kSampleTop: the k-th largest of the maxima of 512 to 1024 groups
+//   of tokens bounds the k-th largest token from below, so their histogram gives
+//   a threshold that little more than k tokens pass; the first CTA sorts those and
+//   does the rest alone. Rows of at most 512 tokens go there at once.
+// * Otherwise a cut is found by a histogram of 256 bins of z, one of 256 parts
+//   of the bin that it falls in, and sorting what is in that part; equal keys by
+//   the thousand (bf16 logits) are told apart by their index alone.
 template <typename T, bool kRes>
 __global__ void __launch_bounds__(kSampleThreads) sample_kernel(SampleParams p, int slice) {
-    extern __shared__ __align__(16) uint32_t keys[];
+    extern __shared__ __align__(16) float xs[];
     __shared__ SampleShared s;
     SampleTeam team{&s, cg::this_cluster(), 0, 0, 0};
     team.rank = (int)team.cl.block_rank();
@@ -122,120 +239,229 @@ __global__ void __launch_bounds__(kSampleThreads) sample_kernel(SampleParams p, 
     int64_t k = p.top_k ? p.top_k[row] : 0;
     const float tp = p.top_p ? p.top_p[row] : 1.f, mp = p.min_p ? p.min_p[row] : 0.f;
     const float un = p.uniform[row];
-    const bool greedy = !(t > 0.f);
-    if (greedy) t = 1.f;
-    const u64 least = mp > 0.f ? max((u64)ceil((double)mp * (double)kSampleOne), (u64)1) : 1;
+    const u64 least = mp > 0.f ? max((u64)ceil((double)fminf(mp, 1.f) * (double)kSampleOne), (u64)1) : 1;
 
-    // ---- the row's largest logit
+    // Place of the draw in a mass of `total` > 0.
+    auto draw = [&](u64 total) -> u64 {
+        const double ud = floor((double)un * (double)total);
+        const u64 r = ud > 0.0 ? (u64)ud : 0;
+        return r >= total ? total - 1 : r;
+    };
+    // list_if: what f(i) gives of the CTA's tokens, without the kNone, into the
+    // warps' lists in index order; n_list counts them, also past the end. A warp
+    // has a run of tokens.
+    constexpr u64 kNone = ~0ull;
+    const int seg = (n + kSampleWarps - 1) / kSampleWarps, seg_lo = min(warp * seg, n), seg_hi = min(seg_lo + seg, n);
+    auto list_if = [&](auto f) {
+        uint32_t c = 0;
+        for (int i0 = seg_lo; i0 < seg_hi; i0 += 32) {
+            const u64 y = i0 + lane < seg_hi ? f(i0 + lane) : kNone;
+            const uint32_t m = __ballot_sync(0xffffffffu, y != kNone);
+            if (m) {
+                const uint32_t o = c + __popc(m & ((1u << lane) - 1));
+                if (y != kNone && o < kSampleWarpList) s.list[warp][o] = y;
+                c += __popc(m);
+            }
+        }
+        if (lane == 0) s.n_list[warp] = c;
+    };
+    // A thread has a run of an odd number of tokens (odd: neighbours in different banks).
+    const int run = ((n + kSampleThreads - 1) / kSampleThreads) | 1, run_lo = min(tid * run, n), run_hi = min(run_lo + run, n);
+
+    // ---- the row's largest logit and its first index: (order key, ~index)
     float mx = -INFINITY;
-    for (int i = tid; i < n; i += kSampleThreads) {
-        const float f = Act<T>::load(x[i]);
-        if (kRes) keys[i] = __float_as_uint(f);
-        mx = fmaxf(mx, f);
+    int at = 0;
+    {
+        auto see = [&](int i, float f) {  // indices come in ascending order
+            if (kRes) xs[i] = f;
+            if (f > mx) {
+                mx = f;
+                at = i;
+            }
+        };
+        constexpr int V = 16 / sizeof(T);
+        const bool vec = (reinterpret_cast<uintptr_t>(x) & 15) == 0;
+        const int nv = vec ? n / V : 0;
+#pragma unroll 4
+        for (int j = tid; j < nv; j += kSampleThreads) {
+            const uint4 y = ld_stream_u4(x + (int64_t)j * V);
+            const uint32_t w[4] = {y.x, y.y, y.z, y.w};
+#pragma unroll
+            for (int e = 0; e < V; ++e)
+                see(j * V + e, sizeof(T) == 4 ? __uint_as_float(w[e * 4 / V])
+                                              : __uint_as_float(e & 1 ? w[e / 2] & 0xffff0000u : w[e / 2] << 16));
+        }
+#pragma unroll 4
+        for (int i = nv * V + tid; i < n; i += kSampleThreads) see(i, Act<T>::load(x[i]));
+        u64 best = mx > -INFINITY ? ((u64)float_order_key(mx + 0.f) << 32) | (0xffffffffu - (uint32_t)(i0 + at)) : 0;
+        best = warp_max_u64(best);
+        if (lane == 0) s.part[warp] = best;
+        float gm = mx;  // 512 to 1024 group maxima in the cluster
+        const int gs = min(team.C, 8);
+        for (int o = 1; o < gs; o *= 2) gm = fmaxf(gm, __shfl_xor_sync(0xffffffffu, gm, o));
+        if ((tid & (gs - 1)) == 0) s.group[tid / gs] = gm;
+        if (tid < kSampleBins) s.count[0][tid] = 0;
+        __syncthreads();
+        if (warp == 0) {
+            best = warp_max_u64(lane < kSampleWarps ? s.part[lane] : 0);
+            if (lane == 0) s.top = best;
+        }
+        team.cl.sync();
+        best = warp_max_u64(lane < team.C ? team.at(lane, &s.top) : 0);
+        if (best == 0 || !(t > 0.f) || k == 1) {  // nothing to draw from, or nothing to choose
+            if (team.rank == 0 && tid == 0) {
+                p.out[row] = best ? (int64_t)(0xffffffffu - (uint32_t)best) : -1;
+                if (p.prob) p.prob[row] = best ? 1.f : 0.f;
+            }
+            team.cl.sync();  // nobody leaves while its maximum is read
+            return;
+        }
+        const uint32_t o = (uint32_t)(best >> 32);
+        const float all = __uint_as_float(o & 0x80000000u ? o & 0x7fffffffu : ~o);
+        // ---- few tokens to keep (those above the k-th largest group maximum), or few tokens at all
+        const bool few = p.vocab <= kSampleList;
+        if (few || (k > 0 && k <= kSampleTop)) {
+            float edge = -INFINITY;
+            int bin = kSampleBins - 1;
+            if (!few) {
+                const int per = kSampleThreads / gs, groups = per * team.C;
+                for (int q = tid; q < groups; q += kSampleThreads) {
+                    const uint32_t key = sample_key(team.at(q / per, &s.group[q % per]), all, t);
+                    if (key < kSampleNever) atomicAdd(&s.count[0][sample_bin(sample_place(key))], 1u);
+                }
+                if (tid == 0) s.bin = kSampleBins - 1;
+                __syncthreads();
+                const u64 c = tid < kSampleBins ? s.count[0][tid] : 0;
+                u64 any;
+                const u64 inc = team.scan(c, any);
+                if (inc - c < (u64)k && inc >= (u64)k) s.bin = tid;
+                __syncthreads();
+                bin = s.bin;
+                // the bin's far edge as a logit, with room for the roundings: a quick test before the exact one
+                if (bin < kSampleBins - 1 && fabsf(all) < INFINITY)
+                    edge = all - ((float)(bin + 1) / kSampleBinScale * t * 1.0001f + 1e-6f * fabsf(all));
+            }
+            list_if([&](int i) -> u64 {
+                const float f = kRes ? xs[i] : Act<T>::load(x[i]);
+                if (!(f >= edge)) return kNone;
+                const uint32_t key = sample_key(f, all, t);
+                if (key >= kSampleNever || sample_bin(sample_place(key)) > bin || sample_weight(key) < least) return kNone;
+                return ((u64)key << 32) | (u64)(i0 + i);
+            });
+            const int m = team.collect();
+            if (m >= 0) {
+                team.cl.sync();  // the lists are read: the others may leave
+                if (team.rank) return;
+                const u64 me = team.sorted(m);
+                const u64 w = tid < m && (k <= 0 || tid < k) ? sample_weight((uint32_t)(me >> 32)) : 0;
+                u64 total;
+                const u64 before = team.scan(w, total) - w;
+                bool keep = w > 0;
+                if (tp < 1.f) {
+                    const double want = ceil((double)tp * (double)total);
+                    keep = keep && before < (want < 1.0 ? 1 : (u64)want);
+                }
+                if (tid < m) s.weight[(uint32_t)me & (kSampleList - 1)] = keep ? w : 0;
+                __syncthreads();
+                const u64 mine = tid < m ? s.weight[tid] : 0;
+                const u64 inc = team.scan(mine, total);
+                const u64 r = draw(total);
+                if (inc - mine <= r && r < inc) {
+                    p.out[row] = (int64_t)((uint32_t)s.all[tid] >> kSamplePlace);
+                    if (p.prob) p.prob[row] = (float)mine / (float)total;
+                }
+                return;
+            }
+        }
+        mx = all;
     }
-    mx = warp_max(mx);
-    if (lane == 0) s.red[warp] = mx;
-    __syncthreads();
-    if (warp == 0) {
-        mx = warp_max(lane < kSampleWarps ? s.red[lane] : -INFINITY);
-        if (lane == 0) s.mx = mx;
+
+    // ---- the general case
+    if (kRes) {  // logits to keys, in place
+        for (int i = tid; i < n; i += kSampleThreads) xs[i] = __uint_as_float(sample_key(xs[i], mx, t));
     }
     team.cl.sync();
-    mx = warp_max(lane < team.C ? *team.cl.map_shared_rank(&s.mx, lane) : -INFINITY);
-    if (mx == -INFINITY) {  // nothing to draw from
-        if (team.rank == 0 && tid == 0) {
-            p.out[row] = -1;
-            if (p.prob) p.prob[row] = 0.f;
-        }
-        team.cl.sync();  // nobody leaves while its maximum is read
-        return;
-    }
-    if (kRes) {
-        for (int i = tid; i < n; i += kSampleThreads) keys[i] = sample_key(__uint_as_float(keys[i]), mx, t);
-    }
-    __syncthreads();
-    auto key_of = [&](int i) -> uint32_t { return kRes ? keys[i] : sample_key(Act<T>::load(x[i]), mx, t); };
+    auto key_of = [&](int i) -> uint32_t { return kRes ? __float_as_uint(xs[i]) : sample_key(Act<T>::load(x[i]), mx, t); };
     u64 cut = ~0ull;  // tokens up to it in the order of (key, index) are kept
     auto comp_of = [&](uint32_t key, int i) -> u64 { return ((u64)key << 32) | (u64)(i0 + i); };
-    // weight of token i among the kept, 0 if it is not
-    auto kept = [&](int i) -> u64 {
-        const uint32_t key = key_of(i);
+    auto weight_of = [&](uint32_t key, int i) -> u64 {  // 0 where the token is not kept
         if (comp_of(key, i) > cut) return 0;
         const u64 w = sample_weight(key);
         return w >= least ? w : 0;
     };
-    // First local index whose running f() is above `target`; the caller knows there is one.
-    auto locate = [&](auto f, u64 target) -> int {
-        const int seg = (n + kSampleWarps - 1) / kSampleWarps;
-        const int lo = min(warp * seg, n), hi = min(lo + seg, n);
-        u64 v = 0;
-        for (int i = lo + lane; i < hi; i += 32) v += f(i);
-        v = warp_sum_u64(v);
-        if (lane == 0) s.part[warp] = v;
-        __syncthreads();
-        u64 b = 0;
-        for (int w = 0; w < warp; ++w) b += s.part[w];
-        if (target >= b && target < b + v) {
-            for (int c = lo; c < hi; c += 32) {
-                const int i = c + lane;
-                u64 y = i < hi ? f(i) : 0;
-#pragma unroll
-                for (int o = 1; o < 32; o <<= 1) {
-                    const u64 z = __shfl_up_sync(0xffffffffu, y, o);
-                    if (lane >= o) y += z;
-                }
-                const unsigned hit = __ballot_sync(0xffffffffu, b + y > target);
-                if (hit) {
-                    if (lane == 0) s.where = c + __ffs(hit) - 1;
-                    break;
-                }
-                b += __shfl_sync(0xffffffffu, y, 31);
-            }
+    // scan_runs: f's sum over the thread's run, the sums of the threads before it,
+    // and the CTA's total in xchg; walk: the first i of the run whose running f is
+    // above `target`.
+    auto scan_runs = [&](auto f, u64& mine, u64& before) {
+        mine = 0;
+        for (int i = run_lo; i < run_hi; ++i) mine += f(i);
+        u64 all;
+        before = team.scan(mine, all) - mine;
+        if (tid == 0) s.xchg[team.turn & 1] = all;
+    };
+    auto walk = [&](auto f, u64 before, u64 target) -> int {
+        for (int i = run_lo;; ++i) {
+            before += f(i);
+            if (before > target) return i;
         }
-        __syncthreads();
-        return s.where;
     };
 
-    // The least cut at which the kept tokens' count (by_mass false) or mass reaches `need`.
-    auto find_cut = [&](bool by_mass, u64 need) {
-        u64 before = 0;   // of the tokens in earlier bins
+    // The least cut at which the kept tokens' count (by_mass false) or mass
+    // reaches what is asked for: k tokens, or top_p of the mass.
+    auto find_cut = [&](bool by_mass) {
+        u64 before = 0, need = 0;   // before: of the tokens in earlier bins
         int bins[2] = {0, 0};
         uint32_t members = 0;
         for (int level = 0; level < 2; ++level) {
             if (tid < kSampleBins) {
-                s.mass[level][tid] = 0;
+                s.mass[level][0][tid] = s.mass[level][1][tid] = s.mass[level][2][tid] = 0;
                 s.count[level][tid] = 0;
             }
             __syncthreads();
             for (int i = tid; i < n; i += kSampleThreads) {
-                const u64 w = kept(i);
-                if (!w) continue;
-                const float place = sample_place(key_of(i));
+                const uint32_t key = key_of(i);
+                const float place = sample_place(key);
                 int bin = sample_bin(place);
                 if (level == 1) {
                     if (bin != bins[0]) continue;
                     bin = sample_sub(place, bin);
                 }
-                if (by_mass) atomicAdd(&s.mass[level][bin], w);
+                const u64 w = weight_of(key, i);
+                if (!w) continue;
+                if (by_mass) {
+                    const uint32_t lo = (uint32_t)w & 0x3fffu, mid = (uint32_t)(w >> 14) & 0x3fffu, hi = (uint32_t)(w >> 28);
+                    atomicAdd(&s.mass[level][0][bin], lo);
+                    if (mid) atomicAdd(&s.mass[level][1][bin], mid);
+                    if (hi) atomicAdd(&s.mass[level][2][bin], hi);
+                }
                 if (!by_mass || level == 1) atomicAdd(&s.count[level][bin], 1u);
             }
             team.cl.sync();
             u64 v = 0, cnt = 0;
             if (tid < kSampleBins) {
+#pragma unroll 4
                 for (int r = 0; r < team.C; ++r) {
-                    if (by_mass) v += team.at(r, &s.mass[level][tid]);
-                    if (!by_mass || level == 1) cnt += *team.cl.map_shared_rank(&s.count[level][tid], r);
+                    if (by_mass)
+                        v += (u64)team.at(r, &s.mass[level][0][tid]) + ((u64)team.at(r, &s.mass[level][1][tid]) << 14) +
+                             ((u64)team.at(r, &s.mass[level][2][tid]) << 28);
+                    if (!by_mass || level == 1) cnt += team.at(r, &s.count[level][tid]);
                 }
                 if (!by_mass) v = cnt;
             }
-            u64 inc = v;
-#pragma unroll
-            for (int o = 1; o < 32; o <<= 1) {
-                const u64 z = __shfl_up_sync(0xffffffffu, inc, o);
-                if (lane >= o) inc += z;
-            }
+            const u64 inc = warp_scan_u64(v);
             if (lane == 31 && warp < kSampleBins / 32) s.scan[warp] = inc;
             __syncthreads();
+            if (level == 0) {
+                u64 all = 0;
+                for (int w = 0; w < kSampleBins / 32; ++w) all += s.scan[w];
+                if (by_mass) {
+                    const double want = ceil((double)tp * (double)all);
+                    need = want < 1.0 ? 1 : (u64)want;
+                } else {
+                    need = (u64)k;
+                    if (need >= all) return;  // nothing to cut
+                }
+            }
             if (tid < kSampleBins) {
                 u64 b = before;
                 for (int w = 0; w < warp; ++w) b += s.scan[w];
@@ -251,71 +477,53 @@ __global__ void __launch_bounds__(kSampleThreads) sample_kernel(SampleParams p, 
             members = s.members;
         }
         auto in_bin = [&](int i) -> u64 {  // weight of a candidate
-            const float place = sample_place(key_of(i));
-            return sample_bin(place) == bins[0] && sample_sub(place, bins[0]) == bins[1] ? kept(i) : 0;
+            const uint32_t key = key_of(i);
+            const float place = sample_place(key);
+            return sample_bin(place) == bins[0] && sample_sub(place, bins[0]) == bins[1] ? weight_of(key, i) : 0;
         };
-        if (members <= kSampleList) {  // rank them against one another
-            if (tid == 0) s.n_list = 0;
-            __syncthreads();
-            for (int i = tid; i < n; i += kSampleThreads)
-                if (in_bin(i)) s.list[atomicAdd(&s.n_list, 1u)] = comp_of(key_of(i), i);
-            team.cl.sync();
-            int at = 0;
-            for (int r = 0; r < team.C; ++r) {
-                const int m = (int)*team.cl.map_shared_rank(&s.n_list, r);
-                if (tid < m) s.all[at + tid] = team.at(r, &s.list[tid]);
-                at += m;
+        if (members <= kSampleList) {
+            list_if([&](int i) -> u64 { return in_bin(i) ? comp_of(key_of(i), i) : kNone; });
+            const int m = team.collect();
+            if (m >= 0) {
+                const u64 me = team.sorted(m), w = tid < m ? (by_mass ? sample_weight((uint32_t)(me >> 32)) : 1) : 0;
+                u64 all;
+                const u64 inc = before + team.scan(w, all);
+                if (w && inc - w < need && need <= inc)
+                    s.cut = (me & 0xffffffff00000000ull) | ((uint32_t)me >> kSamplePlace);
+                __syncthreads();
+                cut = s.cut;
+                return;
             }
-            __syncthreads();
-            if (tid < at) {
-                const u64 me = s.all[tid];
-                u64 sum = before, own = 1;
-                for (int j = 0; j < at; ++j) {
-                    const u64 c = s.all[j];
-                    const u64 w = by_mass ? sample_weight((uint32_t)(c >> 32)) : 1;
-                    if (c <= me) sum += w;
-                    if (c == me) own = w;
-                }
-                if (sum >= need && sum - own < need) s.cut = me;
-            }
-            __syncthreads();
-            cut = s.cut;
-            return;
         }
         // too many: equal keys as a rule
         uint32_t lo = ~0u, hi = 0;
-        u64 mine = 0;
-        for (int i = tid; i < n; i += kSampleThreads)
-            if (in_bin(i)) {
-                lo = min(lo, key_of(i));
-                hi = max(hi, key_of(i));
-                ++mine;
-            }
-        lo = __reduce_min_sync(0xffffffffu, lo);
-        hi = __reduce_max_sync(0xffffffffu, hi);
         if (tid == 0) {
             s.kmin = ~0u;
             s.kmax = 0;
         }
-        __syncthreads();
+        u64 mine, ahead, earlier;
+        scan_runs([&](int i) -> u64 {
+            if (!in_bin(i)) return 0;
+            lo = min(lo, key_of(i));
+            hi = max(hi, key_of(i));
+            return 1;
+        }, mine, ahead);  // its barrier comes after kmin and kmax are set
+        lo = __reduce_min_sync(0xffffffffu, lo);
+        hi = __reduce_max_sync(0xffffffffu, hi);
         if (lane == 0) {
             atomicMin(&s.kmin, lo);
             atomicMax(&s.kmax, hi);
         }
-        u64 earlier = 0;
-        team.sum(mine, &earlier);  // its barrier also publishes kmin and kmax
-        lo = __reduce_min_sync(0xffffffffu, lane < team.C ? *team.cl.map_shared_rank(&s.kmin, lane) : ~0u);
-        hi = __reduce_max_sync(0xffffffffu, lane < team.C ? *team.cl.map_shared_rank(&s.kmax, lane) : 0u);
-        const u64 here = team.s->xchg[(team.turn - 1) & 1];  // this CTA's candidates
+        team.gather(&earlier);
+        lo = __reduce_min_sync(0xffffffffu, lane < team.C ? team.at(lane, &s.kmin) : ~0u);
+        hi = __reduce_max_sync(0xffffffffu, lane < team.C ? team.at(lane, &s.kmax) : 0u);
         if (lo == hi) {  // the m-th of equal ones, in index order
             const u64 w = by_mass ? sample_weight(lo) : 1, m = (need - before + w - 1) / w;
-            const bool own = earlier < m && m <= earlier + here;
-            if (own) {
-                const int i = locate([&](int j) -> u64 { return in_bin(j) ? 1 : 0; }, m - earlier - 1);
-                if (tid == 0) s.cut = comp_of(lo, i);
-            } else if (tid == 0) {
-                s.cut = 0;
-            }
+            if (tid == 0) s.cut = 0;
+            __syncthreads();
+            ahead += earlier;
+            if (ahead < m && m <= ahead + mine)
+                s.cut = comp_of(lo, walk([&](int j) -> u64 { return in_bin(j) ? 1 : 0; }, ahead, m - 1));
             team.cl.sync();
             const u64 c = lane < team.C ? team.at(lane, &s.cut) : 0;  // one of them is not 0 (or the cut is)
             cut = warp_sum_u64(c);
@@ -337,32 +545,18 @@ __global__ void __launch_bounds__(kSampleThreads) sample_kernel(SampleParams p, 
         cut = a;
     };
 
-    if (greedy) k = 1;
-    auto total_kept = [&](bool count, u64* earlier) {
-        u64 v = 0;
-        for (int i = tid; i < n; i += kSampleThreads) {
-            const u64 w = kept(i);
-            v += count ? (w ? 1 : 0) : w;
-        }
-        return team.sum(v, earlier);
-    };
-    if (k > 0 && (u64)k < total_kept(true, nullptr)) find_cut(false, (u64)k);
-    if (tp < 1.f) {
-        const double want = ceil((double)tp * (double)total_kept(false, nullptr));
-        find_cut(true, want < 1.0 ? 1 : (u64)want);
-    }
-    u64 earlier = 0;
-    const u64 total = total_kept(false, &earlier);
-    const u64 here = s.xchg[(team.turn - 1) & 1];
-    const double ud = floor((double)un * (double)total);
-    u64 r = ud > 0.0 ? (u64)ud : 0;
-    if (r >= total) r = total - 1;
-    if (r >= earlier && r < earlier + here) {
-        const int i = locate(kept, r - earlier);
-        if (tid == 0) {
-            p.out[row] = i0 + i;
-            if (p.prob) p.prob[row] = (float)kept(i) / (float)total;
-        }
+    if (k > 0) find_cut(false);
+    if (tp < 1.f) find_cut(true);
+    auto kept = [&](int i) -> u64 { return weight_of(key_of(i), i); };
+    u64 mine, ahead, earlier;
+    scan_runs(kept, mine, ahead);
+    const u64 total = team.gather(&earlier);
+    const u64 r = draw(total);
+    ahead += earlier;
+    if (r >= ahead && r < ahead + mine) {
+        const int i = walk(kept, ahead, r);
+        p.out[row] = i0 + i;
+        if (p.prob) p.prob[row] = (float)kept(i) / (float)total;
     }
     team.cl.sync();  // nobody leaves while its shared memory is read
 }
@@ -421,7 +615,7 @@ extern "C" am_status_code amcu_sample(const AmcuSampleArgs* a, void* stream) {
     int c = 1;
     while (c < 16 && ceil_div(a->vocab, c) > kSampleSlice) c *= 2;
     while (c < 16 && a->rows * c * 2 <= num_sms() && ceil_div(a->vocab, 2 * c) >= 2048) c *= 2;
-    const int slice = (int)ceil_div(a->vocab, c);
+    const int slice = (int)(ceil_div(a->vocab, 8 * c) * 8);  // the slices of an aligned row are aligned
     const bool res = slice <= kSampleSlice, f32 = a->dtype == AMCU_F32;
     AMCU_REQUIRE(a->rows * c <= INT32_MAX, "amcu_sample: too many rows");
     const size_t smem = res ? (size_t)slice * 4 : 0;

@@ -141,6 +141,42 @@ def test_masked_infinite_and_nan(ops, vocab):
     assert got.tolist() == [int(x[6].argmax())]  # a temperature that is none is greedy
 
 
+@pytest.mark.parametrize("k", [2, 300])
+def test_infinite_and_signed_zero_with_top_k(ops, k):
+    x = np.random.default_rng(4).normal(0, 1, (3, 9000)).astype(np.float32)
+    x[0, [700, 8000, 8999]] = np.inf
+    x[1] = np.where(np.arange(9000) % 2 == 0, -0.0, 0.0).astype(np.float32)  # all equal
+    x[2] = -np.inf
+    got, prob = run(ops, x, [1.0] * 3, [k] * 3, [1.0] * 3, [0.0] * 3, [0.99999] * 3)
+    n = min(k, 3)
+    assert got.tolist() == [[700, 8000, 8999][n - 1], k - 1, -1]
+    np.testing.assert_allclose(prob.cpu().numpy(), [1 / n, 1 / k, 0], rtol=1e-6)
+    got, _ = run(ops, x[1:2], [0.0], [0], [1.0], [0.0], [0.99999])
+    assert got.tolist() == [0]
+
+
+@pytest.mark.parametrize("k", [2, 50, 256, 257, 1000])
+@pytest.mark.parametrize("where", ["first", "last", "one thread", "spread"])
+def test_top_k_wherever_they_are(ops, k, where):
+    """The k largest crowded into one slice, one thread's tokens or spread out, in falling and rising order."""
+    vocab = 128256
+    base = -5.0 - np.abs(np.random.default_rng(k).normal(0, 1, vocab)).astype(np.float32)
+    at = {"first": np.arange(k), "last": vocab - k + np.arange(k), "one thread": 512 * 4 * np.arange(k) % vocab,
+          "spread": (np.arange(k) * 7919) % vocab}[where]
+    x = np.stack([base, base])
+    x[0, at] = 1.0 + 0.001 * np.arange(k)
+    x[1, at] = 1.0 - 0.001 * np.arange(k)
+    x = x[:, :vocab]
+    want = []
+    for i in range(2):
+        kept, _ = ref.sample_kept(x[i], 1.0, k, 1.0, 0.0)
+        ids = np.flatnonzero(kept)
+        assert set(ids) == set(at) or where == "one thread"
+        want.append(int(ids[-1]))
+    got, _ = run(ops, x, [1.0] * 2, [k] * 2, [1.0] * 2, [0.0] * 2, [0.9999999] * 2)
+    assert got.tolist() == want
+
+
 def test_uniform_edges(ops):
     """0, 1 and beyond, and NaN: always a kept token."""
     x = np.array([[0.0, 1.0, -np.inf, 2.0, -np.inf]] * 5, np.float32)
