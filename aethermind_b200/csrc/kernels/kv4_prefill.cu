@@ -288,13 +288,20 @@ __global__ void __launch_bounds__(kPfThreads, 1) kv4_prefill_kernel(Kv4AttnParam
         const int w = t >> 5;
         constexpr int CPT = D / 32;       // 16-byte chunks of codes per token
         const int kmax = lim_last + 1;    // keys past it are zeros
-        auto load = [&](bool is_v, int j) {
+        // pages of a tile's eight 16-key blocks, in lanes 0-7; fetched a tile ahead
+        auto pages_of = [&](int j) {
+            const int key = j * kPfKeys + lane * 16;
+            return lane < 8 && key < kmax ? kv4_page(v, b, key) : -1;
+        };
+        int pages = pages_of(0), pages_next = -1;
+        auto load = [&](bool is_v, int j, int pg) {
             const uint8_t* codes = is_v ? v.vc : v.kc;
             const uint8_t* params = is_v ? v.vp : v.kp;
 #pragma unroll
             for (int i = 0; i < CPT; ++i) {
                 const int e = i * kPfDqThreads + t, tk = e / CPT, c = e % CPT, key = j * kPfKeys + tk;
-                const int page = key < kmax ? kv4_page(v, b, key) : -1;
+                int page = __shfl_sync(0xffffffffu, pg, tk >> 4);
+                if (key >= kmax) page = -1;
                 const int slot = key & ((1 << v.page_shift) - 1);
                 const uint8_t* src = codes + (page >= 0 ? kv4_code_off<D>(v, page, kvh, slot) + 16 * c : 0);
                 uint8_t* dst = is_v ? sm + L::oRawV + (tk >> 3) * L::kVPitch + (tk & 7) * (D / 2) + 16 * c
@@ -304,7 +311,7 @@ __global__ void __launch_bounds__(kPfThreads, 1) kv4_prefill_kernel(Kv4AttnParam
             if (t < L::kParK / 16) {  // parameters: 16 bytes are 2 (D = 128) or 4 tokens
                 constexpr int TPC = 256 / D;
                 const int tk = t * TPC, key = j * kPfKeys + tk;
-                const int page = key < kmax ? kv4_page(v, b, key) : -1;
+                const int page = __shfl_sync(0xffffffffu, pg, tk >> 4);  // whole warps
                 const int slot = key & ((1 << v.page_shift) - 1);
                 const uint8_t* src = params + (page >= 0 ? kv4_param_off<D>(v, page, kvh, slot) : 0);
                 // tokens past the last key may hold anything: leave them out
@@ -315,11 +322,12 @@ __global__ void __launch_bounds__(kPfThreads, 1) kv4_prefill_kernel(Kv4AttnParam
             asm volatile("cp.async.commit_group;" ::: "memory");
         };
         if (nt > 0) {
-            load(false, 0);
-            load(true, 0);
+            load(false, 0, pages);
+            load(true, 0, pages);
         }
         for (int j = 0; j < nt; ++j) {
             const int s = j & 1;
+            pages_next = pages_of(j + 1);
             // K: row t
             asm volatile("cp.async.wait_group 1;" ::: "memory");
             named_bar_sync(1, kPfDqThreads);
@@ -356,7 +364,7 @@ __global__ void __launch_bounds__(kPfThreads, 1) kv4_prefill_kernel(Kv4AttnParam
             }
             asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
             named_bar_sync(1, kPfDqThreads);  // raw K is read out
-            if (j + 1 < nt) load(false, j + 1);
+            if (j + 1 < nt) load(false, j + 1, pages_next);
             else asm volatile("cp.async.commit_group;" ::: "memory");
             __syncwarp();
             if (lane == 0) mbar_arrive(&k_full[s]);
@@ -426,7 +434,7 @@ __global__ void __launch_bounds__(kPfThreads, 1) kv4_prefill_kernel(Kv4AttnParam
             }
             asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
             named_bar_sync(1, kPfDqThreads);  // raw V is read out
-            if (j + 1 < nt) load(true, j + 1);
+            if (j + 1 < nt) load(true, j + 1, pages_next);
             else asm volatile("cp.async.commit_group;" ::: "memory");
             __syncwarp();
             if (lane == 0) mbar_arrive(&v_full[s]);
@@ -441,29 +449,39 @@ __global__ void __launch_bounds__(kPfThreads, 1) kv4_prefill_kernel(Kv4AttnParam
         const int full = (__reduce_min_sync(0xffffffffu, row_live ? lim : 0x7fffffff) + 1) / kPfKeys;
         float ref = -1e30f;  // log2 units
         uint64_t l2 = f2_pack(0.f, 0.f);
+        // pages that are none mask their 16 keys: looked up a tile ahead, one block per lane
+        auto missing = [&](int j) {
+            const int key = j * kPfKeys + lane * 16;
+            return lane < 8 && key <= lim_last && kv4_page(v, b, key) < 0;
+        };
+        bool none = missing(0);
         for (int j = 0; j < nt; ++j) {
-            // pages that are none mask their 16 keys (looked up before the wait: one per lane)
-            const int pk = j * kPfKeys + lane * 16;
-            const unsigned bad = __ballot_sync(0xffffffffu, lane < 8 && pk <= lim_last && kv4_page(v, b, pk) < 0);
+            const unsigned bad = __ballot_sync(0xffffffffu, none);
             wait(&s_full[i], j & 1);
             tc_fence_after();
             const bool mask = j >= full || bad != 0;
-            uint32_t x[32];
+            if (mask) {  // masked scores become -inf in place
+#pragma unroll 1
+                for (int q = 0; q < 4; ++q) {
+                    uint32_t x[32];
+                    tc_ld32_issue(ts + 32 * q, x);
+                    tc_ld32_wait(x);
+#pragma unroll
+                    for (int c = 0; c < 32; ++c)
+                        if (j * kPfKeys + 32 * q + c > lim || ((bad >> (2 * q + (c >> 4))) & 1u)) x[c] = 0xff800000u;
+                    tc_st32(ts + 32 * q, x);
+                }
+            }
+            uint32_t x[2][32];
             float mx = -INFINITY;
-            auto masked = [&](int c) {  // key j * 128 + c
-                return j * kPfKeys + c > lim || ((bad >> (c >> 4)) & 1u);
-            };
+            tc_ld32_issue(ts, x[0]);
 #pragma unroll
             for (int q = 0; q < 4; ++q) {
-                tc_ld32_issue(ts + 32 * q, x);
-                tc_ld32_wait(x);
-                if (!mask) {
+                tc_ld32_wait(x[q & 1]);
+                if (q < 3) tc_ld32_issue(ts + 32 * (q + 1), x[(q + 1) & 1]);
 #pragma unroll
-                    for (int c = 0; c < 32; ++c) mx = fmaxf(mx, __uint_as_float(x[c]));
-                } else {
-#pragma unroll
-                    for (int c = 0; c < 32; ++c) mx = masked(32 * q + c) ? mx : fmaxf(mx, __uint_as_float(x[c]));
-                }
+                for (int c = 0; c < 32; c += 2)
+                    mx = fmaxf(mx, fmaxf(__uint_as_float(x[q & 1][c]), __uint_as_float(x[q & 1][c + 1])));
             }
             mx *= f;  // f > 0: the order stays; -inf stays (f = 0 is a dead row's)
             if (!(mx > -1e30f)) mx = -1e30f;
@@ -475,34 +493,34 @@ __global__ void __launch_bounds__(kPfThreads, 1) kv4_prefill_kernel(Kv4AttnParam
                     l2 = f2_fma(l2, f2_pack(corr, corr), f2_pack(0.f, 0.f));
 #pragma unroll 1
                     for (int q = 0; q < D / 32; ++q) {
-                        tc_ld32_issue(to + 32 * q, x);
-                        tc_ld32_wait(x);
+                        uint32_t y[32];
+                        tc_ld32_issue(to + 32 * q, y);
+                        tc_ld32_wait(y);
 #pragma unroll
-                        for (int c = 0; c < 32; ++c) x[c] = __float_as_uint(__uint_as_float(x[c]) * corr);
-                        tc_st32(to + 32 * q, x);
+                        for (int c = 0; c < 32; ++c) y[c] = __float_as_uint(__uint_as_float(y[c]) * corr);
+                        tc_st32(to + 32 * q, y);
                     }
                 }
             }
+            none = j + 1 < nt && missing(j + 1);
+            tc_ld32_issue(ts, x[0]);
             const uint64_t f2 = f2_pack(f, f), r2 = f2_pack(-ref, -ref);
 #pragma unroll
             for (int q = 0; q < 4; ++q) {
-                tc_ld32_issue(ts + 32 * q, x);
-                tc_ld32_wait(x);
+                tc_ld32_wait(x[q & 1]);
+                if (q < 3) tc_ld32_issue(ts + 32 * (q + 1), x[(q + 1) & 1]);
                 uint32_t pk16[16];
 #pragma unroll
                 for (int c = 0; c < 16; ++c) {
-                    const uint64_t y = f2_fma(f2_pack(__uint_as_float(x[2 * c]), __uint_as_float(x[2 * c + 1])), f2, r2);
+                    const uint64_t y = f2_fma(f2_pack(__uint_as_float(x[q & 1][2 * c]), __uint_as_float(x[q & 1][2 * c + 1])), f2, r2);
                     float a, bb;
                     f2_unpack(y, a, bb);
                     a = pf_ex2(a);
                     bb = pf_ex2(bb);
-                    if (mask) {
-                        a = masked(32 * q + 2 * c) ? 0.f : a;
-                        bb = masked(32 * q + 2 * c + 1) ? 0.f : bb;
-                    }
                     l2 = f2_add(l2, f2_pack(a, bb));
                     pk16[c] = pf_h2u(__floats2half2_rn(a, bb));
                 }
+                // columns 16 q .. + 15 hold scores that are in registers by now (q = 0: columns 0 .. 31 are)
                 tc_st_32x32b_x16_nowait(ts + 16 * q, pk16);
             }
             asm volatile("tcgen05.wait::st.sync.aligned;" ::: "memory");
