@@ -8,9 +8,9 @@
 //               B = K, S in tensor memory (one lane per row)
 //   P = 2^(S f - ref) by one thread per row, in fp16 over S's own columns
 //   O += P V    A = P (tensor memory), B = V^T, O in tensor memory
-// Warps 0-3 and 4-7 are the softmax of the two row tiles, warps 8-11 turn codes
-// into fp16 tiles, warp 12 issues the MMAs and owns the tensor memory. While
-// one row tile's softmax runs, the other's products do.
+// Warps 0-3 and 4-7 are the softmax of the two row tiles, warps 8-11 turn K's
+// codes into fp16 tiles and warps 12-15 V's, warp 16 issues the MMAs and owns the
+// tensor memory. While one row tile's softmax runs, the other's products do.
 //
 // K tile and V^T tile have the 128-byte-swizzled K-major layout. A word of 8
 // codes is one 16-byte chunk of a K row; its nibbles come out in the order
@@ -31,7 +31,8 @@
 namespace amcu {
 
 constexpr int kPfRows = 256, kPfKeys = 128;
-constexpr int kPfThreads = 13 * 32;
+constexpr int kPfThreads = 17 * 32;
+constexpr int kPfMmaWarp = 16;
 constexpr int kPfDqThreads = 128;
 constexpr int32_t kErrKv4Wait = 0x501;
 constexpr float kPfLog2e = 1.4426950408889634f;
@@ -41,14 +42,12 @@ template <int D>
 struct PfLayout {  // shared memory, bytes
     static constexpr int kQ = 128 * D * 2;            // one row tile of Q
     static constexpr int kK = kPfKeys * D * 2;        // a K or V^T stage
-    static constexpr int kRawK = kPfKeys * D / 2;
     static constexpr int kVPitch = 8 * D / 2 + 16;    // 8 tokens of V codes
     static constexpr int kRawV = kPfKeys / 8 * kVPitch;
-    static constexpr int kParK = kPfKeys * D / 16;
     static constexpr int kVParPitch = 8 * D / 16 + 16;
     static constexpr int kParV = kPfKeys / 8 * kVParPitch;
-    static constexpr int oQ = 0, oK = oQ + 2 * kQ, oV = oK + 2 * kK, oRawK = oV + 2 * kK, oRawV = oRawK + kRawK,
-                         oParK = oRawV + kRawV, oParV = oParK + kParK, oBar = oParV + kParV;
+    static constexpr int oQ = 0, oK = oQ + 2 * kQ, oV = oK + 2 * kK, oRawV = oV + 2 * kK, oParV = oRawV + 2 * kRawV,
+                         oBar = oParV + 2 * kParV;
     static constexpr int kTotal = oBar + 256 + 1024;  // + alignment slack
 };
 
@@ -150,7 +149,7 @@ __global__ void __launch_bounds__(kPfThreads, 1) kv4_prefill_kernel(Kv4AttnParam
             s_item[1] = (int)off;
         }
     }
-    if (warp == 12) {
+    if (warp == kPfMmaWarp) {
         if (lane == 0) {
             for (int i = 0; i < 2; ++i) {
                 mbar_init(&k_full[i], 4);
@@ -191,36 +190,40 @@ __global__ void __launch_bounds__(kPfThreads, 1) kv4_prefill_kernel(Kv4AttnParam
     const int tok = row_live ? m / p.grp : 0, head = kvh * p.grp + (row_live ? m - tok * p.grp : 0);
     if (warp < 8) {
         const __nv_bfloat16* qp = static_cast<const __nv_bfloat16*>(p.q) + (int64_t)(row0 + tok) * p.qs + (int64_t)head * D;
-        uint32_t q[D / 2];
-        if (row_live && p.vec) {
+        auto chunk = [&](int c, float (&e)[8]) {  // elements 8 c .. + 7
+            uint32_t w[4] = {0, 0, 0, 0};
+            if (row_live && p.vec) {
+                const uint4 y = *reinterpret_cast<const uint4*>(qp + 8 * c);
+                w[0] = y.x; w[1] = y.y; w[2] = y.z; w[3] = y.w;
+            } else if (row_live) {
+                const uint16_t* qe = reinterpret_cast<const uint16_t*>(qp) + 8 * c;
 #pragma unroll
-            for (int i = 0; i < D / 8; ++i) {
-                const uint4 y = *reinterpret_cast<const uint4*>(qp + 8 * i);
-                q[4 * i] = y.x; q[4 * i + 1] = y.y; q[4 * i + 2] = y.z; q[4 * i + 3] = y.w;
+                for (int i = 0; i < 4; ++i) w[i] = (uint32_t)qe[2 * i] | ((uint32_t)qe[2 * i + 1] << 16);
             }
-        } else {
-            const uint16_t* qe = reinterpret_cast<const uint16_t*>(qp);
 #pragma unroll
-            for (int i = 0; i < D / 2; ++i) q[i] = row_live ? (uint32_t)qe[2 * i] | ((uint32_t)qe[2 * i + 1] << 16) : 0u;
+            for (int i = 0; i < 4; ++i) {
+                e[2 * i] = __uint_as_float(w[i] << 16);
+                e[2 * i + 1] = __uint_as_float(w[i] & 0xffff0000u);
+            }
+        };
+        float amax = 0.f, e[8];
+#pragma unroll 4
+        for (int c = 0; c < D / 8; ++c) {
+            chunk(c, e);
+#pragma unroll
+            for (int i = 0; i < 8; ++i) amax = fmaxf(amax, fabsf(e[i]));
         }
-        float amax = 0.f;
-#pragma unroll
-        for (int i = 0; i < D / 2; ++i)
-            amax = fmaxf(amax, fmaxf(fabsf(__uint_as_float(q[i] << 16)), fabsf(__uint_as_float(q[i] & 0xffff0000u))));
         const uint32_t eb = min(max(__float_as_uint(amax) >> 23, 1u), 253u);
         const float inv = __uint_as_float((254u - eb) << 23);
         f = __uint_as_float(eb << 23) * p.scale * kPfLog2e;
         if (row_live) lim = min(ctx - n + tok, cap - 1);
         uint8_t* Q = sm + L::oQ + (warp >> 2) * L::kQ;
         const int r = threadIdx.x & 127;
+#pragma unroll 4
+        for (int c = 0; c < D / 8; ++c) {  // in the order 0 4 1 5 2 6 3 7
+            chunk(c, e);
 #pragma unroll
-        for (int c = 0; c < D / 8; ++c) {  // elements 0 4 1 5 2 6 3 7 of the chunk
-            float e[8];
-#pragma unroll
-            for (int i = 0; i < 4; ++i) {
-                e[2 * i] = __uint_as_float(q[4 * c + i] << 16) * inv;
-                e[2 * i + 1] = __uint_as_float(q[4 * c + i] & 0xffff0000u) * inv;
-            }
+            for (int i = 0; i < 8; ++i) e[i] *= inv;
             *reinterpret_cast<uint4*>(Q + pf_sw<128>(r, c)) =
                     make_uint4(pf_h2u(__floats2half2_rn(e[0], e[4])), pf_h2u(__floats2half2_rn(e[1], e[5])),
                                pf_h2u(__floats2half2_rn(e[2], e[6])), pf_h2u(__floats2half2_rn(e[3], e[7])));
@@ -239,16 +242,23 @@ __global__ void __launch_bounds__(kPfThreads, 1) kv4_prefill_kernel(Kv4AttnParam
         }
     };
 
-    if (warp == 12) {
+    if (warp == kPfMmaWarp) {
         // ---- MMA issuer
         if (lane == 0 && nt > 0) {
             constexpr uint32_t id_s = tc_idesc_f16(128, kPfKeys), id_o = tc_idesc_f16(128, D);
+            // descriptors of the tiles' starts; a K step adds to the address field (16-byte
+            // units). Built anew for every MMA they cost this one thread more time than
+            // the MMA takes (152 cycles against 64).
+            const uint64_t q_desc = tc_desc_sw128(smem_u32(sm + L::oQ)), k_desc = tc_desc_sw128(smem_u32(sm + L::oK)),
+                           v_desc = tc_desc_sw128(smem_u32(sm + L::oV));
             auto qk = [&](int i, int j) {
-                const uint32_t a = smem_u32(sm + L::oQ + i * L::kQ), bb = smem_u32(sm + L::oK + (j & 1) * L::kK);
+                const uint64_t a = q_desc + (uint64_t)(i * (L::kQ >> 4)), bb = k_desc + (uint64_t)((j & 1) * (L::kK >> 4));
+                const uint32_t d = tmem + (uint32_t)(128 * i);
 #pragma unroll
                 for (int s = 0; s < D / 16; ++s) {
-                    const uint32_t o = (uint32_t)((s >> 2) * 16384 + (s & 3) * 32);
-                    tc_mma(tmem + (uint32_t)(128 * i), tc_desc_sw128(a + o), tc_desc_sw128(bb + o), id_s, s != 0);
+                    constexpr int kHalf = 16384 >> 4;
+                    const uint64_t o = (uint64_t)((s >> 2) * kHalf + (s & 3) * 2);
+                    tc_mma(d, a + o, bb + o, id_s, s != 0);
                 }
             };
             wait(&k_full[0], 0);
@@ -266,12 +276,12 @@ __global__ void __launch_bounds__(kPfThreads, 1) kv4_prefill_kernel(Kv4AttnParam
                     wait(&p_full[i], j & 1);
                     tc_fence_after();
                     if (ok) {
-                        const uint32_t bb = smem_u32(sm + L::oV + (j & 1) * L::kK);
+                        const uint64_t bb = v_desc + (uint64_t)((j & 1) * (L::kK >> 4));
+                        const uint32_t d = tmem + 256u + (uint32_t)(128 * i), a = tmem + (uint32_t)(128 * i);
 #pragma unroll
                         for (int s = 0; s < kPfKeys / 16; ++s) {
-                            const uint32_t o = (uint32_t)((s >> 2) * (D * 128) + (s & 3) * 32);
-                            tc_mma_ts(tmem + 256u + (uint32_t)(128 * i), tmem + (uint32_t)(128 * i + 8 * s),
-                                      tc_desc_sw128(bb + o), id_o, j != 0 || s != 0);
+                            constexpr int kHalf = (D * 128) >> 4;
+                            tc_mma_ts(d, a + (uint32_t)(8 * s), bb + (uint64_t)((s >> 2) * kHalf + (s & 3) * 2), id_o, s != 0 || j != 0);
                         }
                         if (more) qk(i, j + 1);
                     }
@@ -283,67 +293,50 @@ __global__ void __launch_bounds__(kPfThreads, 1) kv4_prefill_kernel(Kv4AttnParam
         }
         __syncwarp();
     } else if (warp >= 8) {
-        // ---- codes to fp16 tiles
-        const int t = threadIdx.x - 256;  // 0..127: the token of a K row
-        const int w = t >> 5;
-        constexpr int CPT = D / 32;       // 16-byte chunks of codes per token
+        // registers from the dequantising warps to the softmax: 8 x 72 + 8 x 120 + 96 = 17 x 96 a lane
+        asm volatile("setmaxnreg.dec.sync.aligned.u32 72;");
+        const int t = threadIdx.x & 127;
         const int kmax = lim_last + 1;    // keys past it are zeros
-        // pages of a tile's eight 16-key blocks, in lanes 0-7; fetched a tile ahead
+        // pages of a tile's eight 16-key blocks, in lanes 0-7; fetched ahead
         auto pages_of = [&](int j) {
             const int key = j * kPfKeys + lane * 16;
             return lane < 8 && key < kmax ? kv4_page(v, b, key) : -1;
         };
-        int pages = pages_of(0), pages_next = -1;
-        auto load = [&](bool is_v, int j, int pg) {
-            const uint8_t* codes = is_v ? v.vc : v.kc;
-            const uint8_t* params = is_v ? v.vp : v.kp;
-#pragma unroll
-            for (int i = 0; i < CPT; ++i) {
-                const int e = i * kPfDqThreads + t, tk = e / CPT, c = e % CPT, key = j * kPfKeys + tk;
-                int page = __shfl_sync(0xffffffffu, pg, tk >> 4);
+        if (warp < 12) {
+            // ---- K codes to fp16: row t of the tile, read straight into registers a tile ahead
+            uint32_t raw[WPR], par[G];
+            auto load = [&](int j, int pg) {
+                const int key = j * kPfKeys + t;
+                int page = __shfl_sync(0xffffffffu, pg, t >> 4);
                 if (key >= kmax) page = -1;
                 const int slot = key & ((1 << v.page_shift) - 1);
-                const uint8_t* src = codes + (page >= 0 ? kv4_code_off<D>(v, page, kvh, slot) + 16 * c : 0);
-                uint8_t* dst = is_v ? sm + L::oRawV + (tk >> 3) * L::kVPitch + (tk & 7) * (D / 2) + 16 * c
-                                    : sm + L::oRawK + tk * (D / 2) + 16 * (D == 128 ? c ^ ((tk >> 1) & 3) : c ^ ((tk >> 2) & 1));
-                pf_cp16(dst, src, page >= 0 ? 16u : 0u);
-            }
-            if (t < L::kParK / 16) {  // parameters: 16 bytes are 2 (D = 128) or 4 tokens
-                constexpr int TPC = 256 / D;
-                const int tk = t * TPC, key = j * kPfKeys + tk;
-                const int page = __shfl_sync(0xffffffffu, pg, tk >> 4);  // whole warps
-                const int slot = key & ((1 << v.page_shift) - 1);
-                const uint8_t* src = params + (page >= 0 ? kv4_param_off<D>(v, page, kvh, slot) : 0);
-                // tokens past the last key may hold anything: leave them out
-                const int live = min(max(kmax - key, 0), TPC);
-                uint8_t* dst = is_v ? sm + L::oParV + (tk >> 3) * L::kVParPitch + (tk & 7) * (D / 16) : sm + L::oParK + tk * (D / 16);
-                pf_cp16(dst, src, page >= 0 ? (uint32_t)(live * (D / 16)) : 0u);
-            }
-            asm volatile("cp.async.commit_group;" ::: "memory");
-        };
-        if (nt > 0) {
-            load(false, 0, pages);
-            load(true, 0, pages);
-        }
-        for (int j = 0; j < nt; ++j) {
-            const int s = j & 1;
-            pages_next = pages_of(j + 1);
-            // K: row t
-            asm volatile("cp.async.wait_group 1;" ::: "memory");
-            named_bar_sync(1, kPfDqThreads);
-            if (j >= 2) wait(&k_empty[s], ((j >> 1) & 1) ^ 1);
-            {
-                uint32_t cw[WPR];
 #pragma unroll
-                for (int c = 0; c < CPT; ++c) {
-                    const uint4 y = lds_u4(sm + L::oRawK + t * (D / 2) + 16 * (D == 128 ? c ^ ((t >> 1) & 3) : c ^ ((t >> 2) & 1)));
-                    cw[4 * c] = y.x; cw[4 * c + 1] = y.y; cw[4 * c + 2] = y.z; cw[4 * c + 3] = y.w;
+                for (int i = 0; i < WPR; ++i) raw[i] = 0;
+#pragma unroll
+                for (int g = 0; g < G; ++g) par[g] = 0;
+                if (page >= 0) {
+                    const uint4* src = reinterpret_cast<const uint4*>(v.kc + kv4_code_off<D>(v, page, kvh, slot));
+#pragma unroll
+                    for (int c = 0; c < WPR / 4; ++c) {
+                        const uint4 y = __ldg(src + c);
+                        raw[4 * c] = y.x; raw[4 * c + 1] = y.y; raw[4 * c + 2] = y.z; raw[4 * c + 3] = y.w;
+                    }
+                    const uint32_t* ps = reinterpret_cast<const uint32_t*>(v.kp + kv4_param_off<D>(v, page, kvh, slot));
+#pragma unroll
+                    for (int g = 0; g < G; ++g) par[g] = __ldg(ps + g);
                 }
+            };
+            int pages = pages_of(0);
+            if (nt > 0) load(0, pages);
+            pages = pages_of(1);
+            for (int j = 0; j < nt; ++j) {
+                const int s = j & 1;
+                if (j >= 2) wait(&k_empty[s], ((j >> 1) & 1) ^ 1);
                 __half2 sc[G], mn[G];
                 bool big = false;
 #pragma unroll
                 for (int g = 0; g < G; ++g) {
-                    const __half2 y = *reinterpret_cast<const __half2*>(sm + L::oParK + t * (D / 16) + 4 * g);
+                    const __half2 y = pf_u2h(par[g]);
                     sc[g] = __low2half2(y);
                     mn[g] = __high2half2(y);
                     big |= __half2float(__high2half(y)) + 15.f * __half2float(__low2half(y)) >= 65504.f;
@@ -352,8 +345,8 @@ __global__ void __launch_bounds__(kPfThreads, 1) kv4_prefill_kernel(Kv4AttnParam
 #pragma unroll
                 for (int i = 0; i < WPR; ++i) {
                     const int g = i % G;
-                    __half2 h[4] = {pf_value(cw[i], false, sc[g], mn[g]), pf_value(cw[i], true, sc[g], mn[g]),
-                                    pf_value(cw[i] >> 8, false, sc[g], mn[g]), pf_value(cw[i] >> 8, true, sc[g], mn[g])};
+                    __half2 h[4] = {pf_value(raw[i], false, sc[g], mn[g]), pf_value(raw[i], true, sc[g], mn[g]),
+                                    pf_value(raw[i] >> 8, false, sc[g], mn[g]), pf_value(raw[i] >> 8, true, sc[g], mn[g])};
                     if (big) {
 #pragma unroll
                         for (int q = 0; q < 4; ++q) h[q] = __hmin2(h[q], __float2half2_rn(65504.f));
@@ -361,62 +354,77 @@ __global__ void __launch_bounds__(kPfThreads, 1) kv4_prefill_kernel(Kv4AttnParam
                     *reinterpret_cast<uint4*>(K + pf_sw<kPfKeys>(t, 8 * g + i / G)) =
                             make_uint4(pf_h2u(h[0]), pf_h2u(h[1]), pf_h2u(h[2]), pf_h2u(h[3]));
                 }
+                asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
+                __syncwarp();
+                if (lane == 0) mbar_arrive(&k_full[s]);
+                if (j + 1 < nt) load(j + 1, pages);
+                pages = pages_of(j + 2);
             }
-            asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
-            named_bar_sync(1, kPfDqThreads);  // raw K is read out
-            if (j + 1 < nt) load(false, j + 1, pages_next);
-            else asm volatile("cp.async.commit_group;" ::: "memory");
-            __syncwarp();
-            if (lane == 0) mbar_arrive(&k_full[s]);
-
-            // V: tokens 8 tg .. + 7, words of 8 elements of one or both groups
-            asm volatile("cp.async.wait_group 1;" ::: "memory");
-            named_bar_sync(1, kPfDqThreads);
-            if (j >= 2) wait(&v_empty[s], ((j >> 1) & 1) ^ 1);
-            {
+        } else {
+            // ---- V codes to fp16, transposed: tokens 8 tg .. + 7, words of 8 elements of one or both groups
+            const int w = warp & 3;
+            constexpr int CPT = D / 32;       // 16-byte chunks of codes per token
+            auto load = [&](int j, int pg) {
+                uint8_t* codes = sm + L::oRawV + (j & 1) * L::kRawV;
+                uint8_t* params = sm + L::oParV + (j & 1) * L::kParV;
+                if (j < nt) {
+#pragma unroll
+                    for (int i = 0; i < CPT; ++i) {
+                        const int e = i * kPfDqThreads + t, tk = e / CPT, c = e % CPT, key = j * kPfKeys + tk;
+                        int page = __shfl_sync(0xffffffffu, pg, tk >> 4);
+                        if (key >= kmax) page = -1;
+                        const int slot = key & ((1 << v.page_shift) - 1);
+                        const uint8_t* src = v.vc + (page >= 0 ? kv4_code_off<D>(v, page, kvh, slot) + 16 * c : 0);
+                        pf_cp16(codes + (tk >> 3) * L::kVPitch + (tk & 7) * (D / 2) + 16 * c, src, page >= 0 ? 16u : 0u);
+                    }
+                    if (t < kPfKeys * D / 256) {  // parameters: 16 bytes are 2 (D = 128) or 4 tokens; whole warps
+                        constexpr int TPC = 256 / D;
+                        const int tk = t * TPC, key = j * kPfKeys + tk;
+                        const int page = __shfl_sync(0xffffffffu, pg, tk >> 4);
+                        const int slot = key & ((1 << v.page_shift) - 1);
+                        const uint8_t* src = v.vp + (page >= 0 ? kv4_param_off<D>(v, page, kvh, slot) : 0);
+                        // tokens past the last key may hold anything: leave them out
+                        const int live = min(max(kmax - key, 0), TPC);
+                        pf_cp16(params + (tk >> 3) * L::kVParPitch + (tk & 7) * (D / 16), src,
+                                page >= 0 ? (uint32_t)(live * (D / 16)) : 0u);
+                    }
+                }
+                asm volatile("cp.async.commit_group;" ::: "memory");
+            };
+            int pages = pages_of(0);
+            load(0, pages);
+            pages = pages_of(1);
+            for (int j = 0; j < nt; ++j) {
+                const int s = j & 1;
+                load(j + 1, pages);  // its buffer was read out before the barrier of tile j - 1's end
+                pages = pages_of(j + 2);
+                asm volatile("cp.async.wait_group 1;" ::: "memory");
+                named_bar_sync(1, kPfDqThreads);
+                if (j >= 2) wait(&v_empty[s], ((j >> 1) & 1) ^ 1);
                 const int tg = (lane & 7) + 8 * (w & 1), q8 = (lane >> 3) + 4 * (w >> 1);  // token group, word (pair)
-                uint32_t cw[8][G];
-                const uint8_t* src = sm + L::oRawV + tg * L::kVPitch + q8 * (4 * G);
-#pragma unroll
-                for (int i = 0; i < 8; ++i) {
-                    if (G == 2) {
-                        const uint2 y = *reinterpret_cast<const uint2*>(src + i * (D / 2));
-                        cw[i][0] = y.x;
-                        cw[i][G - 1] = y.y;
-                    } else {
-                        cw[i][0] = *reinterpret_cast<const uint32_t*>(src + i * (D / 2));
-                    }
-                }
-                uint32_t par[8][G];
-#pragma unroll
-                for (int i = 0; i < 8 * G / 4; ++i) {
-                    const uint4 y = lds_u4(sm + L::oParV + tg * L::kVParPitch + 16 * i);
-                    const uint32_t yy[4] = {y.x, y.y, y.z, y.w};
-#pragma unroll
-                    for (int e = 0; e < 4; ++e) par[(4 * i + e) / G][(4 * i + e) % G] = yy[e];
-                }
-                bool big = false;
-#pragma unroll
-                for (int i = 0; i < 8; ++i)
-#pragma unroll
-                    for (int g = 0; g < G; ++g) {
-                        const float2 y = __half22float2(pf_u2h(par[i][g]));
-                        big |= y.y + 15.f * y.x >= 65504.f;
-                    }
+                const uint8_t* src = sm + L::oRawV + s * L::kRawV + tg * L::kVPitch + q8 * (4 * G);
+                const uint8_t* ps = sm + L::oParV + s * L::kParV + tg * L::kVParPitch;
                 uint8_t* V = sm + L::oV + s * L::kK;
 #pragma unroll
                 for (int g = 0; g < G; ++g) {
                     __half2 sc[4], mn[4];
+                    bool big = false;
 #pragma unroll
                     for (int y = 0; y < 4; ++y) {
-                        sc[y] = pf_u2h(__byte_perm(par[2 * y][g], par[2 * y + 1][g], 0x5410));
-                        mn[y] = pf_u2h(__byte_perm(par[2 * y][g], par[2 * y + 1][g], 0x7632));
+                        const uint32_t p0 = lds_u32(ps + (2 * y) * (4 * G) + 4 * g), p1 = lds_u32(ps + (2 * y + 1) * (4 * G) + 4 * g);
+                        sc[y] = pf_u2h(__byte_perm(p0, p1, 0x5410));
+                        mn[y] = pf_u2h(__byte_perm(p0, p1, 0x7632));
+                        const float2 top = __half22float2(mn[y]), step = __half22float2(sc[y]);
+                        big |= top.x + 15.f * step.x >= 65504.f || top.y + 15.f * step.y >= 65504.f;
                     }
+                    uint32_t cw[8];
+#pragma unroll
+                    for (int i = 0; i < 8; ++i) cw[i] = lds_u32(src + i * (D / 2) + 4 * g);
 #pragma unroll
                     for (int part = 0; part < 2; ++part) {
                         uint32_t ww[4];
 #pragma unroll
-                        for (int y = 0; y < 4; ++y) ww[y] = __byte_perm(cw[2 * y][g], cw[2 * y + 1][g], part ? 0x7632 : 0x5410);
+                        for (int y = 0; y < 4; ++y) ww[y] = __byte_perm(cw[2 * y], cw[2 * y + 1], part ? 0x7632 : 0x5410);
 #pragma unroll
                         for (int e = 0; e < 4; ++e) {  // element 4 part + e
                             __half2 h[4];
@@ -431,16 +439,16 @@ __global__ void __launch_bounds__(kPfThreads, 1) kv4_prefill_kernel(Kv4AttnParam
                         }
                     }
                 }
+                asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
+                __syncwarp();
+                if (lane == 0) mbar_arrive(&v_full[s]);
+                named_bar_sync(1, kPfDqThreads);  // the codes of this tile are read out
             }
-            asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
-            named_bar_sync(1, kPfDqThreads);  // raw V is read out
-            if (j + 1 < nt) load(true, j + 1, pages_next);
-            else asm volatile("cp.async.commit_group;" ::: "memory");
-            __syncwarp();
-            if (lane == 0) mbar_arrive(&v_full[s]);
+            asm volatile("cp.async.wait_group 0;" ::: "memory");
         }
-        asm volatile("cp.async.wait_group 0;" ::: "memory");
-    } else if (warp / 4 < ni) {
+    } else {
+        asm volatile("setmaxnreg.inc.sync.aligned.u32 120;");
+        if (warp / 4 < ni) {
         // ---- softmax of row tile i: thread = row
         const int i = warp >> 2;
         const uint32_t lane_base = (uint32_t)((warp & 3) * 32) << 16;
@@ -449,14 +457,16 @@ __global__ void __launch_bounds__(kPfThreads, 1) kv4_prefill_kernel(Kv4AttnParam
         const int full = (__reduce_min_sync(0xffffffffu, row_live ? lim : 0x7fffffff) + 1) / kPfKeys;
         float ref = -1e30f;  // log2 units
         uint64_t l2 = f2_pack(0.f, 0.f);
-        // pages that are none mask their 16 keys: looked up a tile ahead, one block per lane
-        auto missing = [&](int j) {
+        // pages that are none mask their 16 keys: looked up a tile ahead, one block per
+        // lane (positions up to lim_last are inside the page table)
+        auto page_at = [&](int j) {  // past the last key: a valid one
             const int key = j * kPfKeys + lane * 16;
-            return lane < 8 && key <= lim_last && kv4_page(v, b, key) < 0;
+            return lane < 8 && key <= lim_last ? v.table[b * v.table_stride + (key >> v.page_shift)] : 0;
         };
-        bool none = missing(0);
+        int page = page_at(0);
         for (int j = 0; j < nt; ++j) {
-            const unsigned bad = __ballot_sync(0xffffffffu, none);
+            const unsigned bad = __ballot_sync(0xffffffffu, page < 0 || page >= v.num_pages);
+            page = page_at(j + 1);
             wait(&s_full[i], j & 1);
             tc_fence_after();
             const bool mask = j >= full || bad != 0;
@@ -502,7 +512,6 @@ __global__ void __launch_bounds__(kPfThreads, 1) kv4_prefill_kernel(Kv4AttnParam
                     }
                 }
             }
-            none = j + 1 < nt && missing(j + 1);
             tc_ld32_issue(ts, x[0]);
             const uint64_t f2 = f2_pack(f, f), r2 = f2_pack(-ref, -ref);
 #pragma unroll
@@ -563,10 +572,11 @@ __global__ void __launch_bounds__(kPfThreads, 1) kv4_prefill_kernel(Kv4AttnParam
                     reinterpret_cast<uint16_t*>(op)[32 * q + c] = (uint16_t)(y[c / 2] >> (16 * (c & 1)));
             }
         }
+        }
     }
     tc_fence_before();
     __syncthreads();
-    if (warp == 12) {
+    if (warp == kPfMmaWarp) {
         tc_fence_after();
         asm volatile("tcgen05.dealloc.cta_group::1.sync.aligned.b32 %0, %1;" ::"r"(tmem), "r"(512) : "memory");
     }
