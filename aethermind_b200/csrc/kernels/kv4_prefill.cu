@@ -10,7 +10,10 @@
 //   O += P V    A = P (tensor memory), B = V^T, O in tensor memory
 // Warps 0-3 and 4-7 are the softmax of the two row tiles, warps 8-11 turn K's
 // codes into fp16 tiles and warps 12-15 V's, warp 16 issues the MMAs and owns the
-// tensor memory. While one row tile's softmax runs, the other's products do.
+// tensor memory. While one row tile's softmax runs, the other's products do. (An
+// issuing warp for each row tile measured 469 against 432 us, the issuer as the
+// block's first warp 442, polling waits with a sleep 472: 2 x 2048 rows over 8192
+// keys, 32 / 8 heads of 128.)
 //
 // K tile and V^T tile have the 128-byte-swizzled K-major layout. A word of 8
 // codes is one 16-byte chunk of a K row; its nibbles come out in the order
@@ -19,9 +22,11 @@
 // m + s c in fp16: (1024 + c) - 1024 exactly, then one fused multiply-add
 // rounded once to 11 bits (an element beyond fp16 becomes 65504).
 //
-// The softmax reference of a row moves (and O and the sum are rescaled) only
-// when the tile's maximum passes it by 2^8: p stays inside fp16, whose relative
-// precision does not depend on the reference.
+// The softmax reference of a row moves only when a score passes it by 2^8 (p
+// stays inside fp16, whose relative precision does not depend on the
+// reference), and to a whole power of two: the sum, O and what the tile has of P
+// already are then rescaled exactly. So the scores are read once, without
+// knowing their tile's maximum first.
 //
 // Waits are bounded: one that runs out records an error code, and the CTA goes
 // through its control flow without waiting again.
@@ -78,6 +83,16 @@ __device__ __forceinline__ void tc_ld32_wait(uint32_t (&r)[32]) {
                    "+r"(r[22]), "+r"(r[23]), "+r"(r[24]), "+r"(r[25]), "+r"(r[26]), "+r"(r[27]), "+r"(r[28]),
                    "+r"(r[29]), "+r"(r[30]), "+r"(r[31])::"memory");
 }
+// 32 lanes x 16 columns, complete on return.
+__device__ __forceinline__ void tc_ld16(uint32_t taddr, uint32_t (&r)[16]) {
+    asm volatile(
+            "tcgen05.ld.sync.aligned.32x32b.x16.b32 {%0,%1,%2,%3,%4,%5,%6,%7,%8,%9,%10,%11,%12,%13,%14,%15}, [%16];\n"
+            "tcgen05.wait::ld.sync.aligned;"
+            : "=r"(r[0]), "=r"(r[1]), "=r"(r[2]), "=r"(r[3]), "=r"(r[4]), "=r"(r[5]), "=r"(r[6]), "=r"(r[7]),
+              "=r"(r[8]), "=r"(r[9]), "=r"(r[10]), "=r"(r[11]), "=r"(r[12]), "=r"(r[13]), "=r"(r[14]), "=r"(r[15])
+            : "r"(taddr)
+            : "memory");
+}
 __device__ __forceinline__ void tc_st32(uint32_t taddr, const uint32_t (&r)[32]) {
     tc_st_32x32b_x32(taddr, r);
 }
@@ -124,9 +139,9 @@ __global__ void __launch_bounds__(kPfThreads, 1) kv4_prefill_kernel(Kv4AttnParam
     uint8_t* sm = reinterpret_cast<uint8_t*>((reinterpret_cast<uintptr_t>(pf_raw) + 1023) & ~(uintptr_t)1023);
     uint64_t* bar = reinterpret_cast<uint64_t*>(sm + L::oBar);
     uint64_t *k_full = bar, *k_empty = bar + 2, *v_full = bar + 4, *v_empty = bar + 6, *s_full = bar + 8,
-             *p_full = bar + 10, *o_full = bar + 12;
-    uint32_t* tmem_slot = reinterpret_cast<uint32_t*>(bar + 14);
-    int* s_item = reinterpret_cast<int*>(bar + 15);  // b, item of b
+             *p_full = bar + 10, *o_full = bar + 12, *q_full = bar + 14;
+    uint32_t* tmem_slot = reinterpret_cast<uint32_t*>(bar + 16);
+    int* s_item = reinterpret_cast<int*>(bar + 17);  // b, item of b
 
     const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
     pdl_wait();
@@ -159,6 +174,7 @@ __global__ void __launch_bounds__(kPfThreads, 1) kv4_prefill_kernel(Kv4AttnParam
                 mbar_init(&s_full[i], 1);
                 mbar_init(&p_full[i], 4);
                 mbar_init(&o_full[i], 1);
+                mbar_init(&q_full[i], 4);
             }
             fence_mbar_init();
         }
@@ -168,7 +184,9 @@ __global__ void __launch_bounds__(kPfThreads, 1) kv4_prefill_kernel(Kv4AttnParam
                      : "memory");
         asm volatile("tcgen05.relinquish_alloc_permit.cta_group::1.sync.aligned;" ::: "memory");
     }
+    tc_fence_before();
     __syncthreads();
+    tc_fence_after();
     const int b = s_item[0];
     int row0, n;
     kv4_rows(v, b, row0, n);
@@ -182,57 +200,6 @@ __global__ void __launch_bounds__(kPfThreads, 1) kv4_prefill_kernel(Kv4AttnParam
     const int ni = m_end - m0 > 128 ? 2 : 1;                              // row tiles
     if (ctx > cap && v.status && threadIdx.x == 0) *v.status = (int32_t)AM_STATUS_OUT_OF_RANGE;
 
-    // ---- Q: one thread per row
-    float f = 0.f;           // 2^e scale log2(e) of this thread's row
-    int lim = -1;            // its last key
-    const int m = m0 + threadIdx.x;
-    const bool row_live = threadIdx.x < kPfRows && m < m_end;
-    const int tok = row_live ? m / p.grp : 0, head = kvh * p.grp + (row_live ? m - tok * p.grp : 0);
-    if (warp < 8) {
-        const __nv_bfloat16* qp = static_cast<const __nv_bfloat16*>(p.q) + (int64_t)(row0 + tok) * p.qs + (int64_t)head * D;
-        auto chunk = [&](int c, float (&e)[8]) {  // elements 8 c .. + 7
-            uint32_t w[4] = {0, 0, 0, 0};
-            if (row_live && p.vec) {
-                const uint4 y = *reinterpret_cast<const uint4*>(qp + 8 * c);
-                w[0] = y.x; w[1] = y.y; w[2] = y.z; w[3] = y.w;
-            } else if (row_live) {
-                const uint16_t* qe = reinterpret_cast<const uint16_t*>(qp) + 8 * c;
-#pragma unroll
-                for (int i = 0; i < 4; ++i) w[i] = (uint32_t)qe[2 * i] | ((uint32_t)qe[2 * i + 1] << 16);
-            }
-#pragma unroll
-            for (int i = 0; i < 4; ++i) {
-                e[2 * i] = __uint_as_float(w[i] << 16);
-                e[2 * i + 1] = __uint_as_float(w[i] & 0xffff0000u);
-            }
-        };
-        float amax = 0.f, e[8];
-#pragma unroll 4
-        for (int c = 0; c < D / 8; ++c) {
-            chunk(c, e);
-#pragma unroll
-            for (int i = 0; i < 8; ++i) amax = fmaxf(amax, fabsf(e[i]));
-        }
-        const uint32_t eb = min(max(__float_as_uint(amax) >> 23, 1u), 253u);
-        const float inv = __uint_as_float((254u - eb) << 23);
-        f = __uint_as_float(eb << 23) * p.scale * kPfLog2e;
-        if (row_live) lim = min(ctx - n + tok, cap - 1);
-        uint8_t* Q = sm + L::oQ + (warp >> 2) * L::kQ;
-        const int r = threadIdx.x & 127;
-#pragma unroll 4
-        for (int c = 0; c < D / 8; ++c) {  // in the order 0 4 1 5 2 6 3 7
-            chunk(c, e);
-#pragma unroll
-            for (int i = 0; i < 8; ++i) e[i] *= inv;
-            *reinterpret_cast<uint4*>(Q + pf_sw<128>(r, c)) =
-                    make_uint4(pf_h2u(__floats2half2_rn(e[0], e[4])), pf_h2u(__floats2half2_rn(e[1], e[5])),
-                               pf_h2u(__floats2half2_rn(e[2], e[6])), pf_h2u(__floats2half2_rn(e[3], e[7])));
-        }
-        asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
-    }
-    tc_fence_before();
-    __syncthreads();
-    tc_fence_after();
     const uint32_t tmem = *tmem_slot;
     bool ok = true;
     auto wait = [&](uint64_t* w, uint32_t parity) {
@@ -262,8 +229,9 @@ __global__ void __launch_bounds__(kPfThreads, 1) kv4_prefill_kernel(Kv4AttnParam
                 }
             };
             wait(&k_full[0], 0);
-            tc_fence_after();
             for (int i = 0; i < ni; ++i) {
+                wait(&q_full[i], 0);
+                tc_fence_after();
                 if (ok) qk(i, 0);
                 tc_commit(&s_full[i]);
             }
@@ -297,10 +265,16 @@ __global__ void __launch_bounds__(kPfThreads, 1) kv4_prefill_kernel(Kv4AttnParam
         asm volatile("setmaxnreg.dec.sync.aligned.u32 72;");
         const int t = threadIdx.x & 127;
         const int kmax = lim_last + 1;    // keys past it are zeros
-        // pages of a tile's eight 16-key blocks, in lanes 0-7; fetched ahead
+        // pages of a tile's eight 16-key blocks, in lanes 0-7; fetched two tiles ahead
+        // (positions below kmax are inside the page table) and checked when used
         auto pages_of = [&](int j) {
             const int key = j * kPfKeys + lane * 16;
-            return lane < 8 && key < kmax ? kv4_page(v, b, key) : -1;
+            return lane < 8 && key < kmax ? v.table[b * v.table_stride + (key >> v.page_shift)] : 0;
+        };
+        auto checked = [&](int pg) {
+            if (pg >= 0 && pg < v.num_pages) return pg;
+            if (v.status) *v.status = (int32_t)AM_STATUS_OUT_OF_RANGE;
+            return -1;
         };
         if (warp < 12) {
             // ---- K codes to fp16: row t of the tile, read straight into registers a tile ahead
@@ -326,9 +300,10 @@ __global__ void __launch_bounds__(kPfThreads, 1) kv4_prefill_kernel(Kv4AttnParam
                     for (int g = 0; g < G; ++g) par[g] = __ldg(ps + g);
                 }
             };
-            int pages = pages_of(0);
-            if (nt > 0) load(0, pages);
-            pages = pages_of(1);
+            int pages = pages_of(0), ahead = pages_of(1);
+            if (nt > 0) load(0, checked(pages));
+            pages = ahead;
+            ahead = pages_of(2);
             for (int j = 0; j < nt; ++j) {
                 const int s = j & 1;
                 if (j >= 2) wait(&k_empty[s], ((j >> 1) & 1) ^ 1);
@@ -357,8 +332,9 @@ __global__ void __launch_bounds__(kPfThreads, 1) kv4_prefill_kernel(Kv4AttnParam
                 asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
                 __syncwarp();
                 if (lane == 0) mbar_arrive(&k_full[s]);
-                if (j + 1 < nt) load(j + 1, pages);
-                pages = pages_of(j + 2);
+                if (j + 1 < nt) load(j + 1, checked(pages));
+                pages = ahead;
+                ahead = pages_of(j + 3);
             }
         } else {
             // ---- V codes to fp16, transposed: tokens 8 tg .. + 7, words of 8 elements of one or both groups
@@ -391,13 +367,15 @@ __global__ void __launch_bounds__(kPfThreads, 1) kv4_prefill_kernel(Kv4AttnParam
                 }
                 asm volatile("cp.async.commit_group;" ::: "memory");
             };
-            int pages = pages_of(0);
-            load(0, pages);
-            pages = pages_of(1);
+            int pages = pages_of(0), ahead = pages_of(1);
+            load(0, checked(pages));
+            pages = ahead;
+            ahead = pages_of(2);
             for (int j = 0; j < nt; ++j) {
                 const int s = j & 1;
-                load(j + 1, pages);  // its buffer was read out before the barrier of tile j - 1's end
-                pages = pages_of(j + 2);
+                load(j + 1, checked(pages));  // its buffer was read out before the barrier of tile j - 1's end
+                pages = ahead;
+                ahead = pages_of(j + 3);
                 asm volatile("cp.async.wait_group 1;" ::: "memory");
                 named_bar_sync(1, kPfDqThreads);
                 if (j >= 2) wait(&v_empty[s], ((j >> 1) & 1) ^ 1);
@@ -453,10 +431,70 @@ __global__ void __launch_bounds__(kPfThreads, 1) kv4_prefill_kernel(Kv4AttnParam
         const int i = warp >> 2;
         const uint32_t lane_base = (uint32_t)((warp & 3) * 32) << 16;
         const uint32_t ts = tmem + lane_base + (uint32_t)(128 * i), to = tmem + lane_base + 256u + (uint32_t)(128 * i);
+        const int m = m0 + threadIdx.x;
+        const bool row_live = m < m_end;
+        const int tok = row_live ? m / p.grp : 0, head = kvh * p.grp + (row_live ? m - tok * p.grp : 0);
+        const int lim = row_live ? min(ctx - n + tok, cap - 1) : -1;  // the row's last key
+        const int64_t q_off = (int64_t)(row0 + tok) * p.qs + (int64_t)head * D;
+        // Q into shared memory, 16 bytes a lane, CPR lanes to a row
+        float f;  // 2^e scale log2(e) of this thread's row
+        {
+            constexpr int CPR = D / 8, RPW = 32 / CPR;  // chunks of a row, rows at a time
+            uint8_t* Q = sm + L::oQ + i * L::kQ;
+            const int c = lane % CPR;
+            uint32_t eb_mine = 1;
+            constexpr int B = 8;  // loads in flight
+#pragma unroll 1
+            for (int st0 = 0; st0 < 32 / RPW; st0 += B) {
+                uint32_t w[B][4];
+#pragma unroll
+                for (int u = 0; u < B; ++u) {
+                    const int src = (st0 + u) * RPW + lane / CPR;  // lane whose row this is
+                    const int64_t off = __shfl_sync(0xffffffffu, q_off, src);
+                    const bool live = __shfl_sync(0xffffffffu, (int)row_live, src);
+                    const __nv_bfloat16* qp = static_cast<const __nv_bfloat16*>(p.q) + off + 8 * c;
+                    w[u][0] = w[u][1] = w[u][2] = w[u][3] = 0;
+                    if (live && p.vec) {
+                        const uint4 y = *reinterpret_cast<const uint4*>(qp);
+                        w[u][0] = y.x; w[u][1] = y.y; w[u][2] = y.z; w[u][3] = y.w;
+                    } else if (live) {
+                        const uint16_t* qe = reinterpret_cast<const uint16_t*>(qp);
+#pragma unroll
+                        for (int k = 0; k < 4; ++k) w[u][k] = (uint32_t)qe[2 * k] | ((uint32_t)qe[2 * k + 1] << 16);
+                    }
+                }
+#pragma unroll
+                for (int u = 0; u < B; ++u) {
+                    float e[8], amax = 0.f;
+#pragma unroll
+                    for (int k = 0; k < 4; ++k) {
+                        e[2 * k] = __uint_as_float(w[u][k] << 16);
+                        e[2 * k + 1] = __uint_as_float(w[u][k] & 0xffff0000u);
+                        amax = fmaxf(amax, fmaxf(fabsf(e[2 * k]), fabsf(e[2 * k + 1])));
+                    }
+#pragma unroll
+                    for (int o = CPR / 2; o > 0; o >>= 1) amax = fmaxf(amax, __shfl_xor_sync(0xffffffffu, amax, o));
+                    const uint32_t eb = min(max(__float_as_uint(amax) >> 23, 1u), 253u);
+                    const float inv = __uint_as_float((254u - eb) << 23);
+#pragma unroll
+                    for (int k = 0; k < 8; ++k) e[k] *= inv;
+                    // in the order 0 4 1 5 2 6 3 7
+                    *reinterpret_cast<uint4*>(Q + pf_sw<128>((warp & 3) * 32 + (st0 + u) * RPW + lane / CPR, c)) =
+                            make_uint4(pf_h2u(__floats2half2_rn(e[0], e[4])), pf_h2u(__floats2half2_rn(e[1], e[5])),
+                                       pf_h2u(__floats2half2_rn(e[2], e[6])), pf_h2u(__floats2half2_rn(e[3], e[7])));
+                    const uint32_t got = __shfl_sync(0xffffffffu, eb, (lane % RPW) * CPR);
+                    if (lane / RPW == st0 + u) eb_mine = got;
+                }
+            }
+            f = __uint_as_float(eb_mine << 23) * p.scale * kPfLog2e;
+            asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
+            __syncwarp();
+            if (lane == 0) mbar_arrive(&q_full[i]);
+        }
         // tiles below `full` need no mask in this warp
-        const int full = (__reduce_min_sync(0xffffffffu, row_live ? lim : 0x7fffffff) + 1) / kPfKeys;
-        float ref = -1e30f;  // log2 units
-        uint64_t l2 = f2_pack(0.f, 0.f);
+        const int full = __reduce_min_sync(0xffffffffu, row_live ? lim + 1 : 0x7fffffff) / kPfKeys;
+        float ref = -1e30f;  // log2 units; a whole number once a key was seen
+        uint64_t l2 = f2_pack(0.f, 0.f), l3 = l2;
         // pages that are none mask their 16 keys: looked up a tile ahead, one block per
         // lane (positions up to lim_last are inside the page table)
         auto page_at = [&](int j) {  // past the last key: a valid one
@@ -464,13 +502,13 @@ __global__ void __launch_bounds__(kPfThreads, 1) kv4_prefill_kernel(Kv4AttnParam
             return lane < 8 && key <= lim_last ? v.table[b * v.table_stride + (key >> v.page_shift)] : 0;
         };
         int page = page_at(0);
+        const uint64_t f2 = f2_pack(f, f);
         for (int j = 0; j < nt; ++j) {
             const unsigned bad = __ballot_sync(0xffffffffu, page < 0 || page >= v.num_pages);
             page = page_at(j + 1);
             wait(&s_full[i], j & 1);
             tc_fence_after();
-            const bool mask = j >= full || bad != 0;
-            if (mask) {  // masked scores become -inf in place
+            if (j >= full || bad != 0) {  // masked scores become -inf in place
 #pragma unroll 1
                 for (int q = 0; q < 4; ++q) {
                     uint32_t x[32];
@@ -483,53 +521,63 @@ __global__ void __launch_bounds__(kPfThreads, 1) kv4_prefill_kernel(Kv4AttnParam
                 }
             }
             uint32_t x[2][32];
-            float mx = -INFINITY;
             tc_ld32_issue(ts, x[0]);
 #pragma unroll
             for (int q = 0; q < 4; ++q) {
-                tc_ld32_wait(x[q & 1]);
-                if (q < 3) tc_ld32_issue(ts + 32 * (q + 1), x[(q + 1) & 1]);
+                uint32_t(&z)[32] = x[q & 1];
+                tc_ld32_wait(z);
+                // the reference moves only for a score that passes it by kPfLift
+                float m4[4];
 #pragma unroll
-                for (int c = 0; c < 32; c += 2)
-                    mx = fmaxf(mx, fmaxf(__uint_as_float(x[q & 1][c]), __uint_as_float(x[q & 1][c + 1])));
-            }
-            mx *= f;  // f > 0: the order stays; -inf stays (f = 0 is a dead row's)
-            if (!(mx > -1e30f)) mx = -1e30f;
-            const bool over = j == 0 || mx > ref + kPfLift;
-            if (__any_sync(0xffffffffu, over)) {
-                const float nref = fmaxf(ref, mx), corr = pf_ex2(ref - nref);
-                ref = nref;
-                if (j > 0) {
+                for (int c = 0; c < 4; ++c) m4[c] = fmaxf(__uint_as_float(z[c]), __uint_as_float(z[c + 4]));
+#pragma unroll
+                for (int c = 8; c < 32; c += 8)
+#pragma unroll
+                    for (int k = 0; k < 4; ++k)
+                        m4[k] = fmaxf(fmaxf(m4[k], __uint_as_float(z[c + k])), __uint_as_float(z[c + k + 4]));
+                const float mx = fmaxf(fmaxf(m4[0], m4[1]), fmaxf(m4[2], m4[3])) * f;
+                if (__any_sync(0xffffffffu, mx > ref + kPfLift)) {
+                    // to a whole number, so that every rescaling is by a power of two
+                    const float nref = mx > ref ? ceilf(fminf(mx, 1e30f)) : ref, corr = pf_ex2(ref - nref);
+                    ref = nref;
                     l2 = f2_fma(l2, f2_pack(corr, corr), f2_pack(0.f, 0.f));
+                    l3 = f2_fma(l3, f2_pack(corr, corr), f2_pack(0.f, 0.f));
+                    const __half2 corr2 = __float2half2_rn(corr);
+                    asm volatile("tcgen05.wait::st.sync.aligned;" ::: "memory");
 #pragma unroll 1
-                    for (int q = 0; q < D / 32; ++q) {
-                        uint32_t y[32];
-                        tc_ld32_issue(to + 32 * q, y);
-                        tc_ld32_wait(y);
+                    for (int k = 0; k < q; ++k) {  // P of this tile's earlier columns
+                        uint32_t y[16];
+                        tc_ld16(ts + 16 * k, y);
 #pragma unroll
-                        for (int c = 0; c < 32; ++c) y[c] = __float_as_uint(__uint_as_float(y[c]) * corr);
-                        tc_st32(to + 32 * q, y);
+                        for (int c = 0; c < 16; ++c) y[c] = pf_h2u(__hmul2(pf_u2h(y[c]), corr2));
+                        tc_st_32x32b_x16(ts + 16 * k, y);
+                    }
+                    if (j > 0) {  // products of earlier tiles are complete: this tile's scores were committed after them
+#pragma unroll 1
+                        for (int k = 0; k < D / 16; ++k) {
+                            uint32_t y[16];
+                            tc_ld16(to + 16 * k, y);
+#pragma unroll
+                            for (int c = 0; c < 16; ++c) y[c] = __float_as_uint(__uint_as_float(y[c]) * corr);
+                            tc_st_32x32b_x16(to + 16 * k, y);
+                        }
                     }
                 }
-            }
-            tc_ld32_issue(ts, x[0]);
-            const uint64_t f2 = f2_pack(f, f), r2 = f2_pack(-ref, -ref);
-#pragma unroll
-            for (int q = 0; q < 4; ++q) {
-                tc_ld32_wait(x[q & 1]);
                 if (q < 3) tc_ld32_issue(ts + 32 * (q + 1), x[(q + 1) & 1]);
+                const uint64_t r2 = f2_pack(-ref, -ref);
                 uint32_t pk16[16];
 #pragma unroll
                 for (int c = 0; c < 16; ++c) {
-                    const uint64_t y = f2_fma(f2_pack(__uint_as_float(x[q & 1][2 * c]), __uint_as_float(x[q & 1][2 * c + 1])), f2, r2);
+                    const uint64_t y = f2_fma(f2_pack(__uint_as_float(z[2 * c]), __uint_as_float(z[2 * c + 1])), f2, r2);
                     float a, bb;
                     f2_unpack(y, a, bb);
                     a = pf_ex2(a);
                     bb = pf_ex2(bb);
-                    l2 = f2_add(l2, f2_pack(a, bb));
+                    if (c & 1) l3 = f2_add(l3, f2_pack(a, bb));
+                    else l2 = f2_add(l2, f2_pack(a, bb));
                     pk16[c] = pf_h2u(__floats2half2_rn(a, bb));
                 }
-                // columns 16 q .. + 15 hold scores that are in registers by now (q = 0: columns 0 .. 31 are)
+                // columns 16 q .. + 15 hold scores that are in registers by now
                 tc_st_32x32b_x16_nowait(ts + 16 * q, pk16);
             }
             asm volatile("tcgen05.wait::st.sync.aligned;" ::: "memory");
@@ -539,7 +587,7 @@ __global__ void __launch_bounds__(kPfThreads, 1) kv4_prefill_kernel(Kv4AttnParam
         }
         // ---- out = O / l
         float la, lb;
-        f2_unpack(l2, la, lb);
+        f2_unpack(f2_add(l2, l3), la, lb);
         const float l = la + lb, inv = l > 0.f ? 1.f / l : 0.f;
         if (nt > 0) {
             wait(&o_full[i], 0);
