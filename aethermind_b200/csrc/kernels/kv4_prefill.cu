@@ -96,6 +96,28 @@ __device__ __forceinline__ void tc_ld16(uint32_t taddr, uint32_t (&r)[16]) {
 __device__ __forceinline__ void tc_st32(uint32_t taddr, const uint32_t (&r)[32]) {
     tc_st_32x32b_x32(taddr, r);
 }
+// The products and commits are issued by one elected lane of a warp that runs
+// its loop as a whole.
+__device__ __forceinline__ void pf_mma_ss(uint32_t d, uint64_t a, uint64_t b, uint32_t idesc, uint32_t acc) {
+    asm volatile(
+            "{\n .reg .pred p, e;\n setp.ne.b32 p, %4, 0;\n elect.sync _|e, 0xffffffff;\n"
+            " @e tcgen05.mma.cta_group::1.kind::f16 [%0], %1, %2, %3, p;\n}" ::"r"(d),
+            "l"(a), "l"(b), "r"(idesc), "r"(acc)
+            : "memory");
+}
+__device__ __forceinline__ void pf_mma_ts(uint32_t d, uint32_t a, uint64_t b, uint32_t idesc, uint32_t acc) {
+    asm volatile(
+            "{\n .reg .pred p, e;\n setp.ne.b32 p, %4, 0;\n elect.sync _|e, 0xffffffff;\n"
+            " @e tcgen05.mma.cta_group::1.kind::f16 [%0], [%1], %2, %3, p;\n}" ::"r"(d),
+            "r"(a), "l"(b), "r"(idesc), "r"(acc)
+            : "memory");
+}
+__device__ __forceinline__ void pf_commit(uint64_t* bar) {
+    asm volatile(
+            "{\n .reg .pred e;\n elect.sync _|e, 0xffffffff;\n"
+            " @e tcgen05.commit.cta_group::1.mbarrier::arrive::one.shared::cluster.b64 [%0];\n}" ::"r"(smem_u32(bar))
+            : "memory");
+}
 __device__ __forceinline__ float pf_ex2(float x) {
     float r;
     asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(r) : "f"(x));
@@ -143,7 +165,7 @@ __global__ void __launch_bounds__(kPfThreads, 1) kv4_prefill_kernel(Kv4AttnParam
     uint32_t* tmem_slot = reinterpret_cast<uint32_t*>(bar + 16);
     int* s_item = reinterpret_cast<int*>(bar + 17);  // b, item of b
 
-    const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+    const int warp = __shfl_sync(0xffffffffu, threadIdx.x >> 5, 0), lane = threadIdx.x & 31;
     pdl_wait();
     pdl_trigger();
 
@@ -200,7 +222,7 @@ __global__ void __launch_bounds__(kPfThreads, 1) kv4_prefill_kernel(Kv4AttnParam
     const int ni = m_end - m0 > 128 ? 2 : 1;                              // row tiles
     if (ctx > cap && v.status && threadIdx.x == 0) *v.status = (int32_t)AM_STATUS_OUT_OF_RANGE;
 
-    const uint32_t tmem = *tmem_slot;
+    const uint32_t tmem = __shfl_sync(0xffffffffu, *tmem_slot, 0);
     bool ok = true;
     auto wait = [&](uint64_t* w, uint32_t parity) {
         if (ok && !mbar_wait(w, parity)) {
@@ -211,7 +233,9 @@ __global__ void __launch_bounds__(kPfThreads, 1) kv4_prefill_kernel(Kv4AttnParam
 
     if (warp == kPfMmaWarp) {
         // ---- MMA issuer
-        if (lane == 0 && nt > 0) {
+        // nt and ni the same in every lane also to the compiler: branches and descriptors stay uniform
+        const int nt_ = __shfl_sync(0xffffffffu, nt, 0), ni_ = __shfl_sync(0xffffffffu, ni, 0);
+        if (nt_ > 0) {
             constexpr uint32_t id_s = tc_idesc_f16(128, kPfKeys), id_o = tc_idesc_f16(128, D);
             // descriptors of the tiles' starts; a K step adds to the address field (16-byte
             // units). Built anew for every MMA they cost this one thread more time than
@@ -225,38 +249,38 @@ __global__ void __launch_bounds__(kPfThreads, 1) kv4_prefill_kernel(Kv4AttnParam
                 for (int s = 0; s < D / 16; ++s) {
                     constexpr int kHalf = 16384 >> 4;
                     const uint64_t o = (uint64_t)((s >> 2) * kHalf + (s & 3) * 2);
-                    tc_mma(d, a + o, bb + o, id_s, s != 0);
+                    pf_mma_ss(d, a + o, bb + o, id_s, s != 0);
                 }
             };
             wait(&k_full[0], 0);
-            for (int i = 0; i < ni; ++i) {
+            for (int i = 0; i < ni_; ++i) {
                 wait(&q_full[i], 0);
                 tc_fence_after();
-                if (ok) qk(i, 0);
-                tc_commit(&s_full[i]);
+                qk(i, 0);
+                pf_commit(&s_full[i]);
             }
-            tc_commit(&k_empty[0]);
-            for (int j = 0; j < nt; ++j) {
-                const bool more = j + 1 < nt;
+            pf_commit(&k_empty[0]);
+            for (int j = 0; j < nt_; ++j) {
+                const bool more = j + 1 < nt_;
                 wait(&v_full[j & 1], (j >> 1) & 1);
                 if (more) wait(&k_full[(j + 1) & 1], ((j + 1) >> 1) & 1);
-                for (int i = 0; i < ni; ++i) {
+                for (int i = 0; i < ni_; ++i) {
                     wait(&p_full[i], j & 1);
                     tc_fence_after();
-                    if (ok) {
+                    {
                         const uint64_t bb = v_desc + (uint64_t)((j & 1) * (L::kK >> 4));
                         const uint32_t d = tmem + 256u + (uint32_t)(128 * i), a = tmem + (uint32_t)(128 * i);
 #pragma unroll
                         for (int s = 0; s < kPfKeys / 16; ++s) {
                             constexpr int kHalf = (D * 128) >> 4;
-                            tc_mma_ts(d, a + (uint32_t)(8 * s), bb + (uint64_t)((s >> 2) * kHalf + (s & 3) * 2), id_o, s != 0 || j != 0);
+                            pf_mma_ts(d, a + (uint32_t)(8 * s), bb + (uint64_t)((s >> 2) * kHalf + (s & 3) * 2), id_o, s != 0 || j != 0);
                         }
                         if (more) qk(i, j + 1);
                     }
-                    tc_commit(more ? &s_full[i] : &o_full[i]);
+                    pf_commit(more ? &s_full[i] : &o_full[i]);
                 }
-                tc_commit(&v_empty[j & 1]);
-                if (more) tc_commit(&k_empty[(j + 1) & 1]);
+                pf_commit(&v_empty[j & 1]);
+                if (more) pf_commit(&k_empty[(j + 1) & 1]);
             }
         }
         __syncwarp();
