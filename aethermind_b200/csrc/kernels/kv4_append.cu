@@ -26,6 +26,8 @@ am_status_code kv4_check(const char* what, const AmcuKv4Cache& c, const AmcuKv4B
                  "%s: codes_page_stride must be a multiple of 16 and hold a page", what);
     AMCU_REQUIRE(c.params_page_stride == 0 || (c.params_page_stride >= params && c.params_page_stride % 16 == 0),
                  "%s: params_page_stride must be a multiple of 16 and hold a page", what);
+    AMCU_REQUIRE(codes <= UINT32_MAX && c.codes_page_stride <= UINT32_MAX && c.params_page_stride <= UINT32_MAX,
+                 "%s: pages must be smaller than 4 GB", what);
     AMCU_REQUIRE(b.table_stride == 0 || b.table_stride >= b.max_pages || b.n_seq <= 1,
                  "%s: table_stride below max_pages", what);
     if (b.rows > 0 && b.n_seq > 0) {

@@ -21,15 +21,20 @@ namespace amcu {
 // in turn, each through a cp.async ring of its own. An item cut between CTAs
 // leaves partial sums that kv4_combine_kernel adds in the order of the CTAs.
 //
-// Codes enter the MMA without any conversion: a nibble in bits 0-3 of a half
-// is the fp16 subnormal c * 2^-24, one in bits 4-7 is c * 2^-20. q is scaled
+// Codes enter both products without any conversion: a nibble in bits 0-3 of a
+// half is the fp16 subnormal c * 2^-24, one in bits 4-7 is c * 2^-20. q is scaled
 // by a power of two to [1, 2) and its elements at the low nibbles by 16 more,
 // which makes the integer dot product exact up to fp32 sums; scale and minimum
-// of a key's group are applied to the 64-element sums (m through sum(q)).
-// For V the contraction runs over keys, so c * s is formed before the product:
-// (1024 + c) s - 1024 s in one fp16x2 FMA, rounded once to 11 bits (fp32: the
-// rounding's remainder in a second product). The minima and the softmax
-// denominator are three more rows of the same product.
+// of a key's group are applied to the 64-element sums (m through sum(q)). In the
+// second product the rows that come from low nibbles are 2^-4 of the others until
+// the end, the scales of V go into p (p s, rounded to 11 bits; fp32: as a high and
+// a low half), and the minima and the softmax denominator are three more rows of
+// the product. p s is fp16: where a warp's scales are below 2^-5 (fp32: always)
+// they are lifted by a power of two, so precision is relative to the largest scales
+// that the warp meets, not to 6e-8. The MMA aligns its products by their operands'
+// exponents, subnormals' by that of 2^-14: sums with such codes are good to 2^-17 of
+// their largest term, which bf16 does not see; fp32 calls turn codes into normal
+// halves first ((1024 + c) - 1024).
 constexpr int kDecWarps = 8;
 constexpr int kDecThreads = kDecWarps * 32;
 constexpr int kDecStages = 5;
@@ -81,6 +86,14 @@ template <int D>
 __device__ __forceinline__ int dec_chunk(int tk, int c) {
     return D == 128 ? (tk >> 1) * 8 + ((((tk & 1) << 2) + c) ^ (((tk >> 1) & 3) << 1))
                     : (tk >> 2) * 8 + ((((tk & 3) << 1) + c) ^ (((tk >> 2) & 1) << 1));
+}
+
+// Codes in bits 0-3 (high: 4-7) of both halves as an MMA operand.
+template <bool kNormal>
+__device__ __forceinline__ uint32_t dec_code(uint32_t w, bool high) {
+    if (!kNormal) return high ? w & 0x00F000F0u : w & 0x000F000Fu;
+    return h2u(high ? __hadd2(u2h((w & 0x00F000F0u) | 0x54005400u), __float2half2_rn(-64.f))
+                    : __hadd2(u2h((w & 0x000F000Fu) | 0x64006400u), __float2half2_rn(-1024.f)));
 }
 
 // Cost of sequence b in units, and what a segment needs of it.
@@ -202,12 +215,12 @@ __global__ void __launch_bounds__(kDecThreads, 2) kv4_decode_kernel(Kv4AttnParam
                         a = (r & 1) ? a - ah : ah;
                         c = (r & 1) ? c - ch : ch;
                     }
-                    const float lift = e == 0 ? 16.f : 1.f;
+                    const float lift = !kWide && e == 0 ? 16.f : 1.f;
                     qf[j][hh][e] = h2u(__floats2half2_rn(a * lift, c * lift));
                 }
         // results: factor of the integer sums, sum(q) per group, last visible position
         const float sl = p.scale * kLog2e;
-        const float f_op = __uint_as_float(eb << 23) * sl * 1048576.f;
+        const float f_op = __uint_as_float(eb << 23) * sl * (kWide ? 1.f : 1048576.f);
         const int lim_op = c_live ? min(sq.ctx - sq.n + c_row, cap - 1) : -1;
         float f[2], qg[G][2];
         int lim[2];
@@ -228,38 +241,39 @@ __global__ void __launch_bounds__(kDecThreads, 2) kv4_decode_kernel(Kv4AttnParam
         // ---- ring: unit k of this warp is u0 + warp + 8 k
         const int nk = u_end > u0 + warp ? (u_end - u0 - warp + kDecWarps - 1) / kDecWarps : 0;
         int pages = -1;
+        bool holes = false;   // a page that is none was met
+        const int64_t head_c = ((int64_t)kvh << v.page_shift) * (D / 2), head_p = ((int64_t)kvh << v.page_shift) * (D / 16);
+        constexpr int PC = kParams / 16;
+        const uint8_t* const k_src = v.kc + head_c + lane * 16;
+        const uint8_t* const v_src = v.vc + head_c + lane * 16;
+        const uint8_t* const p_src = lane < PC ? v.kp + head_p + lane * 16 : v.vp + head_p + (lane - PC) * 16;
+        const uint32_t c_dst = ring + (uint32_t)dec_chunk<D>(lane / (D / 32), lane % (D / 32)) * 16;
+        const uint32_t p_dst = ring + 2 * kCodes + lane * 16;
+        const uint32_t slot_mask = (1u << page_units_shift) - 1;
         auto fetch = [&](int k) {
             if (k < nk) {
                 if ((k & 31) == 0) {  // page ids of the next 32 units, one per lane
                     const int u = u0 + warp + kDecWarps * (k + lane);
-                    pages = u < u_end ? kv4_page(v, b, u * kDecUnit) : -1;
+                    pages = u < u_end ? kv4_page(v, b, u * kDecUnit) : 0;
+                    holes |= __any_sync(0xffffffffu, pages < 0);
                 }
-                const int u = u0 + warp + kDecWarps * k;
                 const int page = __shfl_sync(0xffffffffu, pages, k & 31);
-                const uint32_t st = ring + (k % S) * kStage;
-                const uint32_t ok = page >= 0 ? 16u : 0u;
-                const int slot = (u & ((1 << page_units_shift) - 1)) * kDecUnit;
-                const int64_t co = page >= 0 ? kv4_code_off<D>(v, page, kvh, slot) : 0;
-                const int64_t po = page >= 0 ? kv4_param_off<D>(v, page, kvh, slot) : 0;
-                constexpr int CPT = D / 32;  // 16-byte chunks per token
+                const uint32_t st = (uint32_t)(k % S) * kStage, ok = page >= 0 ? 16u : 0u, pg = page >= 0 ? page : 0;
+                const uint32_t slot = (uint32_t)(u0 + warp + kDecWarps * k) & slot_mask;
+                const uint64_t co = pg * (uint64_t)(uint32_t)v.cps + slot * kCodes;  // pages are below 4 GB
 #pragma unroll
-                for (int i = 0; i < kCodes / 512; ++i) {
-                    const int c = i * 32 + lane;
-                    const uint32_t d = (uint32_t)dec_chunk<D>(c / CPT, c % CPT) * 16;
-                    cp16(st + d, v.kc + co + c * 16, ok);
-                    cp16(st + kCodes + d, v.vc + co + c * 16, ok);
+                for (int i = 0; i < kCodes / 512; ++i) {  // 512 bytes are whole swizzled lines
+                    cp16(c_dst + st + i * 512, k_src + co + i * 512, ok);
+                    cp16(c_dst + st + kCodes + i * 512, v_src + co + i * 512, ok);
                 }
-                constexpr int PC = kParams / 16;
-                if (lane < 2 * PC) {
-                    const bool is_v = lane >= PC;
-                    cp16(st + 2 * kCodes + lane * 16, (is_v ? v.vp + po + (lane - PC) * 16 : v.kp + po + lane * 16), ok);
-                }
-                if (lane == 0) *reinterpret_cast<int*>(const_cast<uint8_t*>(ring_p) + (k % S) * kStage + 2 * (kCodes + kParams)) = page;
+                if (lane < 2 * PC) cp16(p_dst + st, p_src + pg * (uint64_t)(uint32_t)v.pps + slot * kParams, ok);
+                if (lane == 0) *reinterpret_cast<int*>(const_cast<uint8_t*>(ring_p) + st + 2 * (kCodes + kParams)) = page;
             }
             asm volatile("cp.async.commit_group;" ::: "memory");
         };
 
         float ref[2] = {-1e30f, -1e30f};
+        float lift = kWide ? 0.f : 1.f;  // V's scales are multiplied by it (0: not chosen yet)
         float o[G][4][4], xa[4] = {};
 #pragma unroll
         for (int g = 0; g < G; ++g)
@@ -298,10 +312,12 @@ __global__ void __launch_bounds__(kDecThreads, 2) kv4_decode_kernel(Kv4AttnParam
             }
 #pragma unroll
             for (int j = 0; j < 2 * G; ++j) {
-                const uint32_t lo[4] = {k0[j] & 0x000F000Fu, k1[j] & 0x000F000Fu, k0[j] & 0x00F000F0u, k1[j] & 0x00F000F0u};
+                const uint32_t lo[4] = {dec_code<kWide>(k0[j], false), dec_code<kWide>(k1[j], false), dec_code<kWide>(k0[j], true),
+                                        dec_code<kWide>(k1[j], true)};
                 mma_f16_16816(a[j % G], lo, qf[j][0][0], qf[j][0][1]);
                 const uint32_t s0 = k0[j] >> 8, s1 = k1[j] >> 8;
-                const uint32_t hi[4] = {s0 & 0x000F000Fu, s1 & 0x000F000Fu, s0 & 0x00F000F0u, s1 & 0x00F000F0u};
+                const uint32_t hi[4] = {dec_code<kWide>(s0, false), dec_code<kWide>(s1, false), dec_code<kWide>(s0, true),
+                                        dec_code<kWide>(s1, true)};
                 mma_f16_16816(a[j % G], hi, qf[j][1][0], qf[j][1][1]);
             }
             float sc[4];  // (key r: columns 2t, 2t + 1), (key r + 8: ...); fp32: one head, in [0] and [2]
@@ -343,14 +359,14 @@ __global__ void __launch_bounds__(kDecThreads, 2) kv4_decode_kernel(Kv4AttnParam
                     vm[hh][g] = __byte_perm(w[g], w[G + g], 0x7632);
                 }
             }
-            const int page = *reinterpret_cast<const int*>(st + 2 * (kCodes + kParams));
-            if (u >= full || page < 0) {  // masks; nothing of an unseen key may reach a product
+            if (u >= full || holes) {  // masks; nothing of an unseen key may reach a product
+                const bool none = *reinterpret_cast<const int*>(st + 2 * (kCodes + kParams)) < 0;
                 const int key = u * kDecUnit + r;
 #pragma unroll
                 for (int hh = 0; hh < 2; ++hh) {
 #pragma unroll
                     for (int j = 0; j < 2; ++j)
-                        if (page < 0 || key + 8 * hh > lim[j]) sc[2 * hh + j] = -INFINITY;
+                        if (none || key + 8 * hh > lim[j]) sc[2 * hh + j] = -INFINITY;
                     const int vk = u * kDecUnit + 2 * t + 8 * hh;
                     const uint32_t keep = (vk <= lim_last ? 0x0000FFFFu : 0u) | (vk + 1 <= lim_last ? 0xFFFF0000u : 0u);
 #pragma unroll
@@ -360,9 +376,32 @@ __global__ void __launch_bounds__(kDecThreads, 2) kv4_decode_kernel(Kv4AttnParam
                     }
                 }
             }
+            // ---- scales of V to where p s keeps its bits: at the warp's first unit, and again for much larger ones
+            if (k == 0 || lift != 1.f) {
+                __half2 m2 = __hmax2(u2h(vs[0][0]), u2h(vs[1][0]));
+                if (G == 2) m2 = __hmax2(m2, __hmax2(u2h(vs[0][G - 1]), u2h(vs[1][G - 1])));
+                float top = fmaxf(__low2float(m2), __high2float(m2));  // over the unit's 16 keys: t tells them apart
+                top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, 1));
+                top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, 2));
+                const float fits = __uint_as_float((260u - (__float_as_uint(fmaxf(top, 6e-8f)) >> 23)) << 23);  // to [64, 128)
+                if (k == 0) {
+                    if (kWide || (top > 0.f && top < 0.03125f)) lift = fits;
+                } else if (top * lift >= 4096.f) {
+                    const float corr = fits / lift;
+                    lift = fits;
+#pragma unroll
+                    for (int g = 0; g < G; ++g)
+#pragma unroll
+                        for (int i = 0; i < 4; ++i)
+#pragma unroll
+                            for (int c = 0; c < 4; ++c) o[g][i][c] *= corr;
+                }
+            }
             // ---- softmax: the reference moves only when a score passes it by kDecLift
-            const bool over = fmaxf(sc[0], sc[2]) > ref[0] + kDecLift || fmaxf(sc[1], sc[3]) > ref[1] + kDecLift;
-            if (__any_sync(0xffffffffu, over)) {
+            float pr[4];
+#pragma unroll
+            for (int c = 0; c < 4; ++c) pr[c] = sc[c] - ref[c & 1];
+            if (__any_sync(0xffffffffu, fmaxf(fmaxf(pr[0], pr[1]), fmaxf(pr[2], pr[3])) > kDecLift)) {
 #pragma unroll
                 for (int j = 0; j < 2; ++j) {
                     float m = fmaxf(sc[j], sc[2 + j]);
@@ -372,6 +411,8 @@ __global__ void __launch_bounds__(kDecThreads, 2) kv4_decode_kernel(Kv4AttnParam
                     m = fmaxf(m, ref[j]);
                     const float corr = ex2(ref[j] - m);
                     ref[j] = m;
+                    pr[j] = sc[j] - m;
+                    pr[2 + j] = sc[2 + j] - m;
                     xa[j] *= corr;
                     xa[2 + j] *= corr;
 #pragma unroll
@@ -383,50 +424,42 @@ __global__ void __launch_bounds__(kDecThreads, 2) kv4_decode_kernel(Kv4AttnParam
                         }
                 }
             }
-            float pr[4];
 #pragma unroll
-            for (int c = 0; c < 4; ++c) pr[c] = ex2(sc[c] - ref[c & 1]);
-            // scales of 64 and more: 1024 s would leave fp16
-            uint32_t one = 0x3C003C00u;
-            {
-                bool big = false;
-#pragma unroll
-                for (int hh = 0; hh < 2; ++hh)
-#pragma unroll
-                    for (int g = 0; g < G; ++g)
-                        big |= (vs[hh][g] & 0x7FFFu) >= 0x5380u || (vs[hh][g] & 0x7FFF0000u) >= 0x53800000u;
-                if (__any_sync(0xffffffffu, big)) {
-                    const __half2 down = __float2half2_rn(0.0078125f);
-                    one = h2u(down);
-#pragma unroll
-                    for (int hh = 0; hh < 2; ++hh)
-#pragma unroll
-                        for (int g = 0; g < G; ++g) {
-                            vs[hh][g] = h2u(__hmul2(u2h(vs[hh][g]), down));
-                            vm[hh][g] = h2u(__hmul2(u2h(vm[hh][g]), down));
-                        }
-#pragma unroll
-                    for (int c = 0; c < 4; ++c) pr[c] *= 128.f;
-                }
-            }
-            uint32_t pb[2];
+            for (int c = 0; c < 4; ++c) pr[c] = ex2(pr[c]);
+            uint32_t pb[2], ps[2][G];  // p, and p times the groups' scales
 #pragma unroll
             for (int hh = 0; hh < 2; ++hh) {
-                __half2 h;
                 if (kWide) {
-                    const __half ph = __float2half_rn(pr[2 * hh]);
-                    h = __halves2half2(ph, __float2half_rn(pr[2 * hh] - __half2float(ph)));
+                    auto two = [](float x) {
+                        const __half h = __float2half_rn(x);
+                        return movm_trans(h2u(__halves2half2(h, __float2half_rn(x - __half2float(h)))));
+                    };
+                    pb[hh] = two(pr[2 * hh]);
+#pragma unroll
+                    for (int g = 0; g < G; ++g) {  // this lane's key is r or r + 8
+                        const __half sv = *reinterpret_cast<const __half*>(vpar + (r + 8 * hh) * (4 * G) + 4 * g);
+                        const bool seen = u * kDecUnit + r + 8 * hh <= lim_last;
+                        ps[hh][g] = two(seen ? pr[2 * hh] * (__half2float(sv) * lift) : 0.f);
+                    }
                 } else {
-                    h = __floats2half2_rn(pr[2 * hh], pr[2 * hh + 1]);
+                    pb[hh] = movm_trans(h2u(__floats2half2_rn(pr[2 * hh], pr[2 * hh + 1])));
+                    if (lift != 1.f) {
+#pragma unroll
+                        for (int g = 0; g < G; ++g) {
+                            const float2 y = __half22float2(u2h(vs[hh][g]));
+                            vs[hh][g] = h2u(__floats2half2_rn(y.x * lift, y.y * lift));
+                        }
+                    }
+#pragma unroll
+                    for (int g = 0; g < G; ++g) ps[hh][g] = h2u(__hmul2(u2h(pb[hh]), u2h(vs[hh][g])));
                 }
-                pb[hh] = movm_trans(h2u(h));
             }
             // ---- rows: minima of the groups, ones
             {
                 uint32_t e[4] = {0, 0, 0, 0};
 #pragma unroll
                 for (int hh = 0; hh < 2; ++hh) {
-                    uint32_t w = r == G ? one : 0u;
+                    uint32_t w = r == G ? 0x3C003C00u : 0u;
 #pragma unroll
                     for (int g = 0; g < G; ++g) w = r == g ? vm[hh][g] : w;
                     e[2 * hh] = w;
@@ -448,12 +481,8 @@ __global__ void __launch_bounds__(kDecThreads, 2) kv4_decode_kernel(Kv4AttnParam
                         vw[hh][y][0] = *reinterpret_cast<const uint32_t*>(st + kCodes + dec_chunk<D>(tk, r >> 2) * 16 + (r & 3) * 4);
                     }
                 }
-            const __half2 k1024 = __float2half2_rn(-1024.f), k64 = __float2half2_rn(-64.f);
 #pragma unroll
             for (int g = 0; g < G; ++g) {
-                const __half2 s2[2] = {u2h(vs[0][g]), u2h(vs[1][g])};
-                const __half2 n1[2] = {__hmul2(s2[0], k1024), __hmul2(s2[1], k1024)};
-                const __half2 n2[2] = {__hmul2(s2[0], k64), __hmul2(s2[1], k64)};
 #pragma unroll
                 for (int part = 0; part < 2; ++part) {  // elements 4 part .. 4 part + 3
                     uint32_t w[2];
@@ -462,22 +491,10 @@ __global__ void __launch_bounds__(kDecThreads, 2) kv4_decode_kernel(Kv4AttnParam
                         w[hh] = __byte_perm(vw[hh][0][g], vw[hh][1][g], part ? 0x7632 : 0x5410);
 #pragma unroll
                     for (int q2 = 0; q2 < 2; ++q2) {
-                        uint32_t hi[4], lo[4];
-#pragma unroll
-                        for (int hh = 0; hh < 2; ++hh) {
-                            const uint32_t ww = q2 ? w[hh] >> 8 : w[hh];
-                            const __half2 x0 = u2h((ww & 0x000F000Fu) | 0x64006400u);
-                            const __half2 x1 = u2h((ww & 0x00F000F0u) | 0x54005400u);
-                            const __half2 y0 = __hfma2(x0, s2[hh], n1[hh]), y1 = __hfma2(x1, s2[hh], n2[hh]);
-                            hi[2 * hh] = h2u(y0);
-                            hi[2 * hh + 1] = h2u(y1);
-                            if (kWide) {
-                                lo[2 * hh] = h2u(__hfma2(__hadd2(x0, k1024), s2[hh], __hneg2(y0)));
-                                lo[2 * hh + 1] = h2u(__hfma2(__hadd2(x1, k64), s2[hh], __hneg2(y1)));
-                            }
-                        }
-                        mma_f16_16816(o[g][2 * part + q2], hi, pb[0], pb[1]);
-                        if (kWide) mma_f16_16816(o[g][2 * part + q2], lo, pb[0], pb[1]);
+                        const uint32_t wa = q2 ? w[0] >> 8 : w[0], wb = q2 ? w[1] >> 8 : w[1];
+                        const uint32_t e[4] = {dec_code<kWide>(wa, false), dec_code<kWide>(wa, true), dec_code<kWide>(wb, false),
+                                               dec_code<kWide>(wb, true)};
+                        mma_f16_16816(o[g][2 * part + q2], e, ps[0][g], ps[1][g]);
                     }
                 }
             }
@@ -488,6 +505,9 @@ __global__ void __launch_bounds__(kDecThreads, 2) kv4_decode_kernel(Kv4AttnParam
         __syncthreads();  // the rings are read out
         float* mo = reinterpret_cast<float*>(smem);
         float* mx = mo + kDecWarps * 8 * kMS;  // [warp][column][4]
+        // low nibbles are in units of 2^-24, high ones of 2^-20 (fp32: of 1), both times lift
+        const float unlift = nk > 0 ? 1.f / lift : 0.f;
+        const float lo_unit = (kWide ? 1.f : 16777216.f) * unlift, hi_unit = (kWide ? 1.f : 1048576.f) * unlift;
         if (kWide) {  // high and low columns of one head
 #pragma unroll
             for (int c = 0; c < 4; c += 2) {
@@ -506,7 +526,7 @@ __global__ void __launch_bounds__(kDecThreads, 2) kv4_decode_kernel(Kv4AttnParam
             for (int g = 0; g < G; ++g)
 #pragma unroll
                 for (int i = 0; i < 4; ++i)
-                    *reinterpret_cast<float2*>(dst + g * kKv4Group + 8 * r + 2 * i) = make_float2(o[g][i][j], o[g][i][2 + j]);
+                    *reinterpret_cast<float2*>(dst + g * kKv4Group + 8 * r + 2 * i) = make_float2(o[g][i][j] * lo_unit, o[g][i][2 + j] * hi_unit);
             if (r <= G) mx[(warp * 8 + col) * 4 + (r == G ? 1 : 2 + r)] = xa[j];
             if (r == 0) mx[(warp * 8 + col) * 4] = ref[j];
         }
