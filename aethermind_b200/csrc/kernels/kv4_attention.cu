@@ -37,7 +37,7 @@ namespace amcu {
 // halves first ((1024 + c) - 1024).
 constexpr int kDecWarps = 8;
 constexpr int kDecThreads = kDecWarps * 32;
-constexpr int kDecStages = 5;
+constexpr int kDecStages = 4;  // 3, 5 and 6 measure within 2%
 constexpr int kDecUnit = 16;       // keys per unit
 constexpr int kDecMinUnits = 8;    // units of a CTA at least: one for each warp
 constexpr float kLog2e = 1.4426950408889634f;
@@ -54,7 +54,8 @@ template <int D> constexpr int dec_smem_bytes() {
 
 struct DecMeta {   // for the CTA that holds an item's last unit but not its first
     int32_t first;   // CTA of the first unit; -1: nothing to combine
-    int32_t b, kvh, ct;
+    int32_t row0, head0, col0, cols;  // the sequence's first row, the kv head's first q head, the tile's columns
+    int32_t pad[3];
 };
 struct DecWork {
     float2* ml;    // [CTA][2][8] (reference, denominator)
@@ -185,53 +186,7 @@ __global__ void __launch_bounds__(kDecThreads, 2) kv4_decode_kernel(Kv4AttnParam
         for (int g = 0; g < G; ++g)
 #pragma unroll
             for (int i = 0; i < 16; ++i) qv[g][i] = c_live ? Act<T>::load(qp[g * kKv4Group + i]) : 0.f;
-        float amax = 0.f, qsum[G];
-#pragma unroll
-        for (int g = 0; g < G; ++g) {
-            qsum[g] = 0.f;
-#pragma unroll
-            for (int i = 0; i < 16; ++i) {
-                amax = fmaxf(amax, fabsf(qv[g][i]));
-                qsum[g] += qv[g][i];
-            }
-            qsum[g] += __shfl_xor_sync(0xffffffffu, qsum[g], 1);
-            qsum[g] += __shfl_xor_sync(0xffffffffu, qsum[g], 2);
-        }
-        amax = fmaxf(amax, __shfl_xor_sync(0xffffffffu, amax, 1));
-        amax = fmaxf(amax, __shfl_xor_sync(0xffffffffu, amax, 2));
-        const uint32_t eb = min(max(__float_as_uint(amax) >> 23, 1u), 253u);
-        const float inv = __uint_as_float((254u - eb) << 23);
-        uint32_t qf[2 * G][2][2];  // [word][half of the word][b0, b1]
-#pragma unroll
-        for (int j = 0; j < 2 * G; ++j)
-#pragma unroll
-            for (int hh = 0; hh < 2; ++hh)
-#pragma unroll
-                for (int e = 0; e < 2; ++e) {  // nibbles 2 hh + e and 2 hh + e + 4
-                    const int i = 8 * (j / G) + 2 * hh + e;
-                    float a = qv[j % G][i] * inv, c = qv[j % G][i + 4] * inv;
-                    if (kWide) {
-                        const float ah = __half2float(__float2half_rn(a)), ch = __half2float(__float2half_rn(c));
-                        a = (r & 1) ? a - ah : ah;
-                        c = (r & 1) ? c - ch : ch;
-                    }
-                    const float lift = !kWide && e == 0 ? 16.f : 1.f;
-                    qf[j][hh][e] = h2u(__floats2half2_rn(a * lift, c * lift));
-                }
-        // results: factor of the integer sums, sum(q) per group, last visible position
-        const float sl = p.scale * kLog2e;
-        const float f_op = __uint_as_float(eb << 23) * sl * (kWide ? 1.f : 1048576.f);
-        const int lim_op = c_live ? min(sq.ctx - sq.n + c_row, cap - 1) : -1;
-        float f[2], qg[G][2];
-        int lim[2];
-#pragma unroll
-        for (int j = 0; j < 2; ++j) {
-            const int src = kWide ? 8 * t : 8 * t + 4 * j;
-            f[j] = __shfl_sync(0xffffffffu, f_op, src);
-            lim[j] = __shfl_sync(0xffffffffu, lim_op, src);
-#pragma unroll
-            for (int g = 0; g < G; ++g) qg[g][j] = __shfl_sync(0xffffffffu, qsum[g] * sl, src);
-        }
+        const int lim_op = c_live ? min(sq.ctx - sq.n + c_row, cap - 1) : -1;  // last visible position
         // keys past the last column's limit need no unit; before the first one's, no mask
         const int lim_last = __shfl_sync(0xffffffffu, lim_op, kWide ? 8 * (cols - 1) : 4 * (cols - 1));
         const int lim_first = __shfl_sync(0xffffffffu, lim_op, 0);
@@ -272,6 +227,56 @@ __global__ void __launch_bounds__(kDecThreads, 2) kv4_decode_kernel(Kv4AttnParam
             asm volatile("cp.async.commit_group;" ::: "memory");
         };
 
+        // on their way while q is prepared
+#pragma unroll
+        for (int k = 0; k < S - 1; ++k) fetch(k);
+
+        float amax = 0.f, qsum[G];
+#pragma unroll
+        for (int g = 0; g < G; ++g) {
+            qsum[g] = 0.f;
+#pragma unroll
+            for (int i = 0; i < 16; ++i) {
+                amax = fmaxf(amax, fabsf(qv[g][i]));
+                qsum[g] += qv[g][i];
+            }
+            qsum[g] += __shfl_xor_sync(0xffffffffu, qsum[g], 1);
+            qsum[g] += __shfl_xor_sync(0xffffffffu, qsum[g], 2);
+        }
+        amax = fmaxf(amax, __shfl_xor_sync(0xffffffffu, amax, 1));
+        amax = fmaxf(amax, __shfl_xor_sync(0xffffffffu, amax, 2));
+        const uint32_t eb = min(max(__float_as_uint(amax) >> 23, 1u), 253u);
+        const float inv = __uint_as_float((254u - eb) << 23);
+        uint32_t qf[2 * G][2][2];  // [word][half of the word][b0, b1]
+#pragma unroll
+        for (int j = 0; j < 2 * G; ++j)
+#pragma unroll
+            for (int hh = 0; hh < 2; ++hh)
+#pragma unroll
+                for (int e = 0; e < 2; ++e) {  // nibbles 2 hh + e and 2 hh + e + 4
+                    const int i = 8 * (j / G) + 2 * hh + e;
+                    float a = qv[j % G][i] * inv, c = qv[j % G][i + 4] * inv;
+                    if (kWide) {
+                        const float ah = __half2float(__float2half_rn(a)), ch = __half2float(__float2half_rn(c));
+                        a = (r & 1) ? a - ah : ah;
+                        c = (r & 1) ? c - ch : ch;
+                    }
+                    const float lift = !kWide && e == 0 ? 16.f : 1.f;
+                    qf[j][hh][e] = h2u(__floats2half2_rn(a * lift, c * lift));
+                }
+        // results: factor of the integer sums, sum(q) per group, last visible position
+        const float sl = p.scale * kLog2e;
+        const float f_op = __uint_as_float(eb << 23) * sl * (kWide ? 1.f : 1048576.f);
+        float f[2], qg[G][2];
+        int lim[2];
+#pragma unroll
+        for (int j = 0; j < 2; ++j) {
+            const int src = kWide ? 8 * t : 8 * t + 4 * j;
+            f[j] = __shfl_sync(0xffffffffu, f_op, src);
+            lim[j] = __shfl_sync(0xffffffffu, lim_op, src);
+#pragma unroll
+            for (int g = 0; g < G; ++g) qg[g][j] = __shfl_sync(0xffffffffu, qsum[g] * sl, src);
+        }
         float ref[2] = {-1e30f, -1e30f};
         float lift = kWide ? 0.f : 1.f;  // V's scales are multiplied by it (0: not chosen yet)
         float o[G][4][4], xa[4] = {};
@@ -281,9 +286,6 @@ __global__ void __launch_bounds__(kDecThreads, 2) kv4_decode_kernel(Kv4AttnParam
             for (int i = 0; i < 4; ++i)
 #pragma unroll
                 for (int c = 0; c < 4; ++c) o[g][i][c] = 0.f;
-#pragma unroll
-        for (int k = 0; k < S - 1; ++k) fetch(k);
-
         for (int k = 0; k < nk; ++k) {
             asm volatile("cp.async.wait_group %0;" ::"n"(S - 2) : "memory");
             __syncwarp();
@@ -534,7 +536,7 @@ __global__ void __launch_bounds__(kDecThreads, 2) kv4_decode_kernel(Kv4AttnParam
         const bool whole = u0 == 0 && u1 == sq.units;
         const int slot = blockIdx.x * 2 + (u0 == 0 ? 1 : 0);
         if (!whole && threadIdx.x == 0 && u0 > 0 && u1 == sq.units)
-            ws.meta[blockIdx.x] = {(int)((x - u0) / share), b, kvh, ct};
+            ws.meta[blockIdx.x] = {(int)((x - u0) / share), sq.row0, kvh * p.grp, ct * CT, cols, {}};
         for (int e = threadIdx.x; e < cols * D; e += kDecThreads) {
             const int col = e / D, d = e % D;
             float m = -1e30f;
@@ -564,49 +566,68 @@ __global__ void __launch_bounds__(kDecThreads, 2) kv4_decode_kernel(Kv4AttnParam
 }
 
 // Partial sums of an item that was cut between CTAs, one column per CTA row.
+// Bound by latency: a warp's partials are loaded together, four at a time (37
+// partials of 8 items one after another took 6 us, so 3).
+constexpr int kCombineWarps = 8;
 template <typename T, int D>
-__global__ void __launch_bounds__(128) kv4_combine_kernel(Kv4AttnParams p, DecWork ws) {
-    constexpr int CT = dec_cols<T>(), E = D / 32;
-    __shared__ float so[4][D];
-    __shared__ float2 sm[4];
+__global__ void __launch_bounds__(kCombineWarps * 32) kv4_combine_kernel(Kv4AttnParams p, DecWork ws) {
+    constexpr int E = D / 32, B = 4;
+    __shared__ float so[kCombineWarps][D];
+    __shared__ float2 sm[kCombineWarps];
     pdl_wait();
     pdl_trigger();
     const DecMeta me = ws.meta[blockIdx.x];
-    if (me.first < 0) return;
-    int row0, n;
-    kv4_rows(p.v, me.b, row0, n);
-    const int col = blockIdx.y, fcol = me.ct * CT + col;
-    if (fcol >= n * p.grp) return;
+    const int col = blockIdx.y, last = blockIdx.x;
+    if (me.first < 0 || col >= me.cols) return;
     const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
     float m = -1e30f, l = 0.f, acc[E] = {};
-    for (int c = me.first + warp; c <= (int)blockIdx.x; c += 4) {
-        const int slot = 2 * c + (c == me.first ? 1 : 0);
-        const float2 y = ws.ml[slot * 8 + col];
-        float val[E];
+    for (int c0 = me.first + warp; c0 <= last; c0 += B * kCombineWarps) {
+        float2 y[B];
+        float val[B][E];
 #pragma unroll
-        for (int i = 0; i < E; ++i) val[i] = ws.o[((int64_t)slot * 8 + col) * D + lane * E + i];
-        const float nm = fmaxf(m, y.x), fa = ex2(m - nm), fb = ex2(y.x - nm);
-        l = l * fa + y.y * fb;
+        for (int q = 0; q < B; ++q) {
+            const int c = c0 + q * kCombineWarps, slot = 2 * c + (c == me.first ? 1 : 0);
+            y[q] = make_float2(-1e30f, 0.f);
 #pragma unroll
-        for (int i = 0; i < E; ++i) acc[i] = acc[i] * fa + val[i] * fb;
-        m = nm;
+            for (int i = 0; i < E; ++i) val[q][i] = 0.f;
+            if (c <= last) {
+                y[q] = ws.ml[slot * 8 + col];
+                const float* o = ws.o + ((int64_t)slot * 8 + col) * D + lane * E;
+                if (E == 4) {
+                    const float4 z = *reinterpret_cast<const float4*>(o);
+                    val[q][0] = z.x; val[q][1] = z.y; val[q][E - 2] = z.z; val[q][E - 1] = z.w;
+                } else {
+                    const float2 z = *reinterpret_cast<const float2*>(o);
+                    val[q][0] = z.x; val[q][1] = z.y;
+                }
+            }
+        }
+#pragma unroll
+        for (int q = 0; q < B; ++q) {
+            const float nm = fmaxf(m, y[q].x), fa = ex2(m - nm), fb = ex2(y[q].x - nm);
+            l = l * fa + y[q].y * fb;
+#pragma unroll
+            for (int i = 0; i < E; ++i) acc[i] = acc[i] * fa + val[q][i] * fb;
+            m = nm;
+        }
     }
     if (lane == 0) sm[warp] = make_float2(m, l);
 #pragma unroll
     for (int i = 0; i < E; ++i) so[warp][lane * E + i] = acc[i];
     __syncthreads();
-    for (int d = threadIdx.x; d < D; d += 128) {
-        const float mm = fmaxf(fmaxf(sm[0].x, sm[1].x), fmaxf(sm[2].x, sm[3].x));
-        float ls = 0.f, vs = 0.f;
+    const int d = threadIdx.x;
+    if (d >= D) return;
+    float mm = -1e30f, ls = 0.f, vs = 0.f;
 #pragma unroll
-        for (int w = 0; w < 4; ++w) {
-            const float fw = ex2(sm[w].x - mm);
-            ls = fmaf(fw, sm[w].y, ls);
-            vs = fmaf(fw, so[w][d], vs);
-        }
-        const int rw = fcol / p.grp, hd = me.kvh * p.grp + fcol - rw * p.grp;
-        static_cast<T*>(p.out)[(int64_t)(row0 + rw) * p.os + (int64_t)hd * D + d] = Act<T>::store(ls > 0.f ? vs / ls : 0.f);
+    for (int w = 0; w < kCombineWarps; ++w) mm = fmaxf(mm, sm[w].x);
+#pragma unroll
+    for (int w = 0; w < kCombineWarps; ++w) {
+        const float fw = ex2(sm[w].x - mm);
+        ls = fmaf(fw, sm[w].y, ls);
+        vs = fmaf(fw, so[w][d], vs);
     }
+    const int fcol = me.col0 + col, rw = fcol / p.grp, hd = me.head0 + fcol - rw * p.grp;
+    static_cast<T*>(p.out)[(int64_t)(me.row0 + rw) * p.os + (int64_t)hd * D + d] = Act<T>::store(ls > 0.f ? vs / ls : 0.f);
 }
 
 }  // namespace amcu
@@ -615,7 +636,15 @@ using namespace amcu;
 
 namespace {
 
-int dec_ctas() { return 2 * num_sms(); }
+// CTAs of a call: two to an SM, fewer where the page table cannot hold that many units.
+int64_t dec_ctas(const AmcuKv4AttentionArgs* a) {
+    const int64_t cols = a->dtype == AMCU_F32 ? dec_cols<float>() : dec_cols<__nv_bfloat16>();
+    const int64_t tiles = ceil_div(a->batch.rows * (a->n_q_heads / a->cache.n_kv_heads), cols) + a->batch.n_seq;
+    const int64_t units = ceil_div(a->batch.max_pages * a->cache.page_size, kDecUnit);
+    const double bound = (double)tiles * (double)a->cache.n_kv_heads * (double)(units > 0 ? units : 1) / kDecMinUnits;
+    const int64_t most = 2 * num_sms();
+    return bound >= (double)most ? most : (int64_t)bound + 1;
+}
 
 // The decode workspace: partial sums and their bookkeeping, 16-byte aligned parts.
 size_t dec_layout(int64_t ctas, int64_t d, uint8_t* base, DecWork* w) {
@@ -629,20 +658,21 @@ size_t dec_layout(int64_t ctas, int64_t d, uint8_t* base, DecWork* w) {
 }
 
 template <typename T, int D>
-void launch_decode(const Kv4AttnParams& p, const DecWork& w, cudaStream_t s) {
+void launch_decode(const Kv4AttnParams& p, const DecWork& w, unsigned ctas, cudaStream_t s) {
     constexpr int smem = dec_smem_bytes<D>();
     set_func_attr_once(reinterpret_cast<const void*>(&kv4_decode_kernel<T, D>),
                        cudaFuncAttributeMaxDynamicSharedMemorySize, smem);
-    const unsigned ctas = (unsigned)dec_ctas();
     launch_pdl(kv4_decode_kernel<T, D>, dim3(ctas), dim3(kDecThreads), smem, s, p, w);
-    launch_pdl(kv4_combine_kernel<T, D>, dim3(ctas, dec_cols<T>()), dim3(128), 0, s, p, w);
+    launch_pdl(kv4_combine_kernel<T, D>, dim3(ctas, dec_cols<T>()), dim3(kCombineWarps * 32), 0, s, p, w);
 }
 
 }  // namespace
 
 extern "C" size_t amcu_attn_kv4_workspace_bytes(const AmcuKv4AttentionArgs* a) {
-    if (!a || a->batch.rows <= 0 || a->batch.n_seq <= 0) return 0;
-    return dec_layout(dec_ctas(), a->cache.head_dim, nullptr, nullptr);
+    if (!a || a->batch.rows <= 0 || a->batch.n_seq <= 0 || a->n_q_heads <= 0 || a->cache.n_kv_heads <= 0 ||
+        a->batch.max_pages < 0 || a->cache.page_size <= 0)
+        return 0;
+    return dec_layout(dec_ctas(a), a->cache.head_dim, nullptr, nullptr);
 }
 
 extern "C" am_status_code amcu_attn_kv4(const AmcuKv4AttentionArgs* a, void* stream) {
@@ -670,13 +700,14 @@ extern "C" am_status_code amcu_attn_kv4(const AmcuKv4AttentionArgs* a, void* str
     AMCU_REQUIRE(a->workspace && a->workspace_size >= need && aligned(a->workspace, 16),
                  "amcu_attn_kv4: needs a 16-byte aligned workspace of %zu bytes", need);
     DecWork w;
-    dec_layout(dec_ctas(), a->cache.head_dim, static_cast<uint8_t*>(a->workspace), &w);
+    const unsigned ctas = (unsigned)dec_ctas(a);
+    dec_layout(ctas, a->cache.head_dim, static_cast<uint8_t*>(a->workspace), &w);
     const bool f32 = a->dtype == AMCU_F32;
     cudaStream_t s = as_stream(stream);
     if (prompts) return kv4_prefill_launch(p, a->cache.head_dim, s);
     if (a->cache.head_dim == 64)
-        f32 ? launch_decode<float, 64>(p, w, s) : launch_decode<__nv_bfloat16, 64>(p, w, s);
+        f32 ? launch_decode<float, 64>(p, w, ctas, s) : launch_decode<__nv_bfloat16, 64>(p, w, ctas, s);
     else
-        f32 ? launch_decode<float, 128>(p, w, s) : launch_decode<__nv_bfloat16, 128>(p, w, s);
+        f32 ? launch_decode<float, 128>(p, w, ctas, s) : launch_decode<__nv_bfloat16, 128>(p, w, ctas, s);
     return check_launch("amcu_attn_kv4");
 }
