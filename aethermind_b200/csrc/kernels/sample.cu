@@ -53,7 +53,8 @@ __device__ __forceinline__ u64 sample_weight(uint32_t key) {
     const int sh = (int)(f >> 23) - 110;
     return sh >= 0 ? (u64)m << sh : (u64)(sh > -24 ? m >> -sh : 0u);
 }
-// Position of a key on a scale of 256 bins; bin and sub-bin are monotone in the key.
+// Position of a key on a scale of 256 bins (a weight above 0 is below 254); bin
+// and sub-bin are monotone in the key.
 __device__ __forceinline__ float sample_place(uint32_t key) { return __fmul_rn(__uint_as_float(key), kSampleBinScale); }
 __device__ __forceinline__ int sample_bin(float place) { return (int)fminf(place, (float)(kSampleBins - 1)); }
 __device__ __forceinline__ int sample_sub(float place, int bin) {
@@ -254,12 +255,16 @@ __global__ void __launch_bounds__(kSampleThreads) sample_kernel(SampleParams p, 
     const int seg = (n + kSampleWarps - 1) / kSampleWarps, seg_lo = min(warp * seg, n), seg_hi = min(seg_lo + seg, n);
     auto list_if = [&](auto f) {
         uint32_t c = 0;
-        for (int i0 = seg_lo; i0 < seg_hi; i0 += 32) {
-            const u64 y = i0 + lane < seg_hi ? f(i0 + lane) : kNone;
-            const uint32_t m = __ballot_sync(0xffffffffu, y != kNone);
-            if (m) {
+        for (int at = seg_lo; at < seg_hi; at += 128) {  // four independent tokens a lane
+            u64 y[4];
+#pragma unroll
+            for (int e = 0; e < 4; ++e) y[e] = at + 32 * e + lane < seg_hi ? f(at + 32 * e + lane) : kNone;
+            if (__ballot_sync(0xffffffffu, (y[0] & y[1] & y[2] & y[3]) != kNone) == 0) continue;
+#pragma unroll
+            for (int e = 0; e < 4; ++e) {
+                const uint32_t m = __ballot_sync(0xffffffffu, y[e] != kNone);
                 const uint32_t o = c + __popc(m & ((1u << lane) - 1));
-                if (y != kNone && o < kSampleWarpList) s.list[warp][o] = y;
+                if (y[e] != kNone && o < kSampleWarpList) s.list[warp][o] = y[e];
                 c += __popc(m);
             }
         }
@@ -378,6 +383,7 @@ __global__ void __launch_bounds__(kSampleThreads) sample_kernel(SampleParams p, 
 
     // ---- the general case
     if (kRes) {  // logits to keys, in place
+#pragma unroll 4
         for (int i = tid; i < n; i += kSampleThreads) xs[i] = __uint_as_float(sample_key(xs[i], mx, t));
     }
     team.cl.sync();
@@ -394,6 +400,7 @@ __global__ void __launch_bounds__(kSampleThreads) sample_kernel(SampleParams p, 
     // above `target`.
     auto scan_runs = [&](auto f, u64& mine, u64& before) {
         mine = 0;
+#pragma unroll 4
         for (int i = run_lo; i < run_hi; ++i) mine += f(i);
         u64 all;
         before = team.scan(mine, all) - mine;
@@ -418,16 +425,14 @@ __global__ void __launch_bounds__(kSampleThreads) sample_kernel(SampleParams p, 
                 s.count[level][tid] = 0;
             }
             __syncthreads();
-            for (int i = tid; i < n; i += kSampleThreads) {
+            const float bin_lo = (float)bins[0], bin_hi = bin_lo + 1.f;
+            auto add = [&](int i) {
                 const uint32_t key = key_of(i);
                 const float place = sample_place(key);
-                int bin = sample_bin(place);
-                if (level == 1) {
-                    if (bin != bins[0]) continue;
-                    bin = sample_sub(place, bin);
-                }
+                if (level == 1 && !(place >= bin_lo && place < bin_hi)) return;
+                const int bin = level == 1 ? sample_sub(place, bins[0]) : sample_bin(place);
                 const u64 w = weight_of(key, i);
-                if (!w) continue;
+                if (!w) return;
                 if (by_mass) {
                     const uint32_t lo = (uint32_t)w & 0x3fffu, mid = (uint32_t)(w >> 14) & 0x3fffu, hi = (uint32_t)(w >> 28);
                     atomicAdd(&s.mass[level][0][bin], lo);
@@ -435,7 +440,9 @@ __global__ void __launch_bounds__(kSampleThreads) sample_kernel(SampleParams p, 
                     if (hi) atomicAdd(&s.mass[level][2][bin], hi);
                 }
                 if (!by_mass || level == 1) atomicAdd(&s.count[level][bin], 1u);
-            }
+            };
+#pragma unroll 4
+            for (int i = tid; i < n; i += kSampleThreads) add(i);
             team.cl.sync();
             u64 v = 0, cnt = 0;
             if (tid < kSampleBins) {
@@ -476,10 +483,11 @@ __global__ void __launch_bounds__(kSampleThreads) sample_kernel(SampleParams p, 
             before = s.before;
             members = s.members;
         }
+        const float bin_lo = (float)bins[0], bin_hi = bin_lo + 1.f;
         auto in_bin = [&](int i) -> u64 {  // weight of a candidate
             const uint32_t key = key_of(i);
             const float place = sample_place(key);
-            return sample_bin(place) == bins[0] && sample_sub(place, bins[0]) == bins[1] ? weight_of(key, i) : 0;
+            return place >= bin_lo && place < bin_hi && sample_sub(place, bins[0]) == bins[1] ? weight_of(key, i) : 0;
         };
         if (members <= kSampleList) {
             list_if([&](int i) -> u64 { return in_bin(i) ? comp_of(key_of(i), i) : kNone; });
