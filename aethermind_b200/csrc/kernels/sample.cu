@@ -33,6 +33,7 @@ constexpr int kSampleWarps = kSampleThreads / 32;
 constexpr int kSampleBins = 256;
 constexpr int kSampleList = kSampleThreads;       // most candidates that are sorted
 constexpr int kSampleWarpList = 64;               // of one warp's tokens
+constexpr int kSampleQueue = 128;                 // tokens of a cut's bin that a warp keeps the indices of
 constexpr int kSamplePlace = 9;                   // bits of a place among them
 constexpr int kSampleTop = 256;                   // largest top-k whose tokens are gathered
 constexpr int kSampleSlice = 16384;               // most logits that a CTA keeps in shared memory
@@ -67,6 +68,7 @@ struct SampleShared {
     float group[kSampleThreads];       // maxima of the threads, or of 2, 4 or 8 neighbours
     u64 list[kSampleWarps][kSampleWarpList];  // each warp's candidates
     uint32_t n_list[kSampleWarps];
+    uint32_t queue[kSampleWarps][kSampleQueue];
     u64 all[kSampleList];        // every CTA's
     u64 weight[kSampleList];     // by place: weights of the kept
     u64 tmp[kSampleList];
@@ -250,23 +252,40 @@ __global__ void __launch_bounds__(kSampleThreads) sample_kernel(SampleParams p, 
     };
     // list_if: what f(i) gives of the CTA's tokens, without the kNone, into the
     // warps' lists in index order; n_list counts them, also past the end. A warp
-    // has a run of tokens.
+    // has a run of tokens, a lane four neighbours at a time; quick(i) may rule out
+    // tokens i .. i + 3 (i a multiple of 4) together.
     constexpr u64 kNone = ~0ull;
-    const int seg = (n + kSampleWarps - 1) / kSampleWarps, seg_lo = min(warp * seg, n), seg_hi = min(seg_lo + seg, n);
-    auto list_if = [&](auto f) {
+    const int seg = ((n + 4 * kSampleWarps - 1) / (4 * kSampleWarps)) * 4, seg_lo = min(warp * seg, n), seg_hi = min(seg_lo + seg, n);
+    auto list_if = [&](auto quick, auto f) {
         uint32_t c = 0;
-        for (int at = seg_lo; at < seg_hi; at += 128) {  // four independent tokens a lane
+#pragma unroll 2
+        for (int at = seg_lo; at < seg_hi; at += 128) {
+            const int i = at + 4 * lane;
+            const bool maybe = i < seg_hi && quick(i);
+            if (__ballot_sync(0xffffffffu, maybe) == 0) continue;
             u64 y[4];
-#pragma unroll
-            for (int e = 0; e < 4; ++e) y[e] = at + 32 * e + lane < seg_hi ? f(at + 32 * e + lane) : kNone;
-            if (__ballot_sync(0xffffffffu, (y[0] & y[1] & y[2] & y[3]) != kNone) == 0) continue;
+            uint32_t mine = 0;
 #pragma unroll
             for (int e = 0; e < 4; ++e) {
-                const uint32_t m = __ballot_sync(0xffffffffu, y[e] != kNone);
-                const uint32_t o = c + __popc(m & ((1u << lane) - 1));
-                if (y[e] != kNone && o < kSampleWarpList) s.list[warp][o] = y[e];
-                c += __popc(m);
+                y[e] = maybe && i + e < seg_hi ? f(i + e) : kNone;
+                mine += y[e] != kNone;
             }
+            if (__ballot_sync(0xffffffffu, mine) == 0) continue;
+            uint32_t o = mine;
+#pragma unroll
+            for (int d = 1; d < 32; d <<= 1) {
+                const uint32_t z = __shfl_up_sync(0xffffffffu, o, d);
+                if (lane >= d) o += z;
+            }
+            const uint32_t all = __shfl_sync(0xffffffffu, o, 31);
+            o += c - mine;
+#pragma unroll
+            for (int e = 0; e < 4; ++e)
+                if (y[e] != kNone) {
+                    if (o < kSampleWarpList) s.list[warp][o] = y[e];
+                    ++o;
+                }
+            c += all;
         }
         if (lane == 0) s.n_list[warp] = c;
     };
@@ -277,27 +296,41 @@ __global__ void __launch_bounds__(kSampleThreads) sample_kernel(SampleParams p, 
     float mx = -INFINITY;
     int at = 0;
     {
-        auto see = [&](int i, float f) {  // indices come in ascending order
+        constexpr int V = 16 / sizeof(T);
+        const bool vec = (reinterpret_cast<uintptr_t>(x) & 15) == 0;
+        const int nv = vec ? n / V : 0;
+#pragma unroll 4
+        for (int j = tid; j < nv; j += kSampleThreads) {  // a thread's indices ascend
+            const uint4 y = ld_stream_u4(x + (int64_t)j * V);
+            const uint32_t w[4] = {y.x, y.y, y.z, y.w};
+            float f[V];
+#pragma unroll
+            for (int e = 0; e < V; ++e)
+                f[e] = sizeof(T) == 4 ? __uint_as_float(w[e * 4 / V]) : __uint_as_float(e & 1 ? w[e / 2] & 0xffff0000u : w[e / 2] << 16);
+            float top = f[0];
+#pragma unroll
+            for (int e = 1; e < V; ++e) top = fmaxf(top, f[e]);
+            if (kRes) {
+#pragma unroll
+                for (int e = 0; e < V; e += 4)
+                    *reinterpret_cast<float4*>(xs + j * V + e) = make_float4(f[e], f[e + 1], f[e + 2], f[e + 3]);
+            }
+            if (top > mx) {  // a few times per thread
+                mx = top;
+#pragma unroll
+                for (int e = V - 1; e >= 0; --e)
+                    if (f[e] == top) at = j * V + e;
+            }
+        }
+#pragma unroll 4
+        for (int i = nv * V + tid; i < n; i += kSampleThreads) {
+            const float f = Act<T>::load(x[i]);
             if (kRes) xs[i] = f;
             if (f > mx) {
                 mx = f;
                 at = i;
             }
-        };
-        constexpr int V = 16 / sizeof(T);
-        const bool vec = (reinterpret_cast<uintptr_t>(x) & 15) == 0;
-        const int nv = vec ? n / V : 0;
-#pragma unroll 4
-        for (int j = tid; j < nv; j += kSampleThreads) {
-            const uint4 y = ld_stream_u4(x + (int64_t)j * V);
-            const uint32_t w[4] = {y.x, y.y, y.z, y.w};
-#pragma unroll
-            for (int e = 0; e < V; ++e)
-                see(j * V + e, sizeof(T) == 4 ? __uint_as_float(w[e * 4 / V])
-                                              : __uint_as_float(e & 1 ? w[e / 2] & 0xffff0000u : w[e / 2] << 16));
         }
-#pragma unroll 4
-        for (int i = nv * V + tid; i < n; i += kSampleThreads) see(i, Act<T>::load(x[i]));
         u64 best = mx > -INFINITY ? ((u64)float_order_key(mx + 0.f) << 32) | (0xffffffffu - (uint32_t)(i0 + at)) : 0;
         best = warp_max_u64(best);
         if (lane == 0) s.part[warp] = best;
@@ -346,7 +379,11 @@ __global__ void __launch_bounds__(kSampleThreads) sample_kernel(SampleParams p, 
                 if (bin < kSampleBins - 1 && fabsf(all) < INFINITY)
                     edge = all - ((float)(bin + 1) / kSampleBinScale * t * 1.0001f + 1e-6f * fabsf(all));
             }
-            list_if([&](int i) -> u64 {
+            list_if([&](int i) -> bool {  // four neighbours: does any of them reach the edge?
+                if (!kRes || i + 4 > n) return true;
+                const float4 y = *reinterpret_cast<const float4*>(xs + i);
+                return fmaxf(fmaxf(y.x, y.y), fmaxf(y.z, y.w)) >= edge;
+            }, [&](int i) -> u64 {
                 const float f = kRes ? xs[i] : Act<T>::load(x[i]);
                 if (!(f >= edge)) return kNone;
                 const uint32_t key = sample_key(f, all, t);
@@ -382,16 +419,17 @@ __global__ void __launch_bounds__(kSampleThreads) sample_kernel(SampleParams p, 
     }
 
     // ---- the general case
-    if (kRes) {  // logits to keys, in place
-#pragma unroll 4
-        for (int i = tid; i < n; i += kSampleThreads) xs[i] = __uint_as_float(sample_key(xs[i], mx, t));
-    }
-    team.cl.sync();
-    auto key_of = [&](int i) -> uint32_t { return kRes ? __float_as_uint(xs[i]) : sample_key(Act<T>::load(x[i]), mx, t); };
+    team.cl.sync();  // lists of an attempt above are read
+    bool keyed = false;  // xs holds keys: the first pass over the tokens makes them
+    auto key_of = [&](int i) -> uint32_t {
+        if (kRes && keyed) return __float_as_uint(xs[i]);
+        return sample_key(kRes ? xs[i] : Act<T>::load(x[i]), mx, t);
+    };
+    bool any_cut = false;
     u64 cut = ~0ull;  // tokens up to it in the order of (key, index) are kept
     auto comp_of = [&](uint32_t key, int i) -> u64 { return ((u64)key << 32) | (u64)(i0 + i); };
     auto weight_of = [&](uint32_t key, int i) -> u64 {  // 0 where the token is not kept
-        if (comp_of(key, i) > cut) return 0;
+        if (any_cut && comp_of(key, i) > cut) return 0;
         const u64 w = sample_weight(key);
         return w >= least ? w : 0;
     };
@@ -413,12 +451,15 @@ __global__ void __launch_bounds__(kSampleThreads) sample_kernel(SampleParams p, 
         }
     };
 
+    bool known = false;  // whether `local`, summed over the CTA, is its kept mass
+    u64 local = 0;
     // The least cut at which the kept tokens' count (by_mass false) or mass
     // reaches what is asked for: k tokens, or top_p of the mass.
     auto find_cut = [&](bool by_mass) {
         u64 before = 0, need = 0;   // before: of the tokens in earlier bins
         int bins[2] = {0, 0};
         uint32_t members = 0;
+        int queued = -1;  // this warp's tokens of the first level's bin, in s.queue; -1: too many
         for (int level = 0; level < 2; ++level) {
             if (tid < kSampleBins) {
                 s.mass[level][0][tid] = s.mass[level][1][tid] = s.mass[level][2][tid] = 0;
@@ -426,8 +467,7 @@ __global__ void __launch_bounds__(kSampleThreads) sample_kernel(SampleParams p, 
             }
             __syncthreads();
             const float bin_lo = (float)bins[0], bin_hi = bin_lo + 1.f;
-            auto add = [&](int i) {
-                const uint32_t key = key_of(i);
+            auto add = [&](int i, uint32_t key) {
                 const float place = sample_place(key);
                 if (level == 1 && !(place >= bin_lo && place < bin_hi)) return;
                 const int bin = level == 1 ? sample_sub(place, bins[0]) : sample_bin(place);
@@ -441,8 +481,37 @@ __global__ void __launch_bounds__(kSampleThreads) sample_kernel(SampleParams p, 
                 }
                 if (!by_mass || level == 1) atomicAdd(&s.count[level][bin], 1u);
             };
-#pragma unroll 4
-            for (int i = tid; i < n; i += kSampleThreads) add(i);
+            if (level == 0) {
+                if (kRes && !keyed) {
+#pragma unroll 2
+                    for (int i = tid; i < n; i += kSampleThreads) {
+                        xs[i] = __uint_as_float(sample_key(xs[i], mx, t));
+                        add(i, __float_as_uint(xs[i]));
+                    }
+                    keyed = true;
+                    __syncthreads();
+                } else {
+#pragma unroll 2
+                    for (int i = tid; i < n; i += kSampleThreads) add(i, key_of(i));
+                }
+            } else {
+                // the bin's tokens first, so that they are looked at by full warps
+                uint32_t c = 0;
+#pragma unroll 2
+                for (int at = seg_lo; at < seg_hi; at += 32) {
+                    const float place = at + lane < seg_hi ? sample_place(key_of(at + lane)) : -1.f;
+                    const uint32_t m = __ballot_sync(0xffffffffu, place >= bin_lo && place < bin_hi);
+                    const uint32_t o = c + __popc(m & ((1u << lane) - 1));
+                    if (((m >> lane) & 1u) && o < kSampleQueue) s.queue[warp][o] = (uint32_t)(at + lane);
+                    c += __popc(m);
+                }
+                __syncwarp();
+                queued = c <= kSampleQueue ? (int)c : -1;
+                if (queued >= 0)
+                    for (int j = lane; j < queued; j += 32) add((int)s.queue[warp][j], key_of((int)s.queue[warp][j]));
+                else
+                    for (int i = seg_lo + lane; i < seg_hi; i += 32) add(i, key_of(i));
+            }
             team.cl.sync();
             u64 v = 0, cnt = 0;
             if (tid < kSampleBins) {
@@ -490,7 +559,19 @@ __global__ void __launch_bounds__(kSampleThreads) sample_kernel(SampleParams p, 
             return place >= bin_lo && place < bin_hi && sample_sub(place, bins[0]) == bins[1] ? weight_of(key, i) : 0;
         };
         if (members <= kSampleList) {
-            list_if([&](int i) -> u64 { return in_bin(i) ? comp_of(key_of(i), i) : kNone; });
+            if (queued >= 0) {
+                uint32_t c = 0;
+                for (int j0 = 0; j0 < queued; j0 += 32) {
+                    const int i = j0 + lane < queued ? (int)s.queue[warp][j0 + lane] : -1;
+                    const bool hit = i >= 0 && in_bin(i);
+                    const uint32_t m = __ballot_sync(0xffffffffu, hit), o = c + __popc(m & ((1u << lane) - 1));
+                    if (hit && o < kSampleWarpList) s.list[warp][o] = comp_of(key_of(i), i);
+                    c += __popc(m);
+                }
+                if (lane == 0) s.n_list[warp] = c;
+            } else {
+                list_if([](int) { return true; }, [&](int i) -> u64 { return in_bin(i) ? comp_of(key_of(i), i) : kNone; });
+            }
             const int m = team.collect();
             if (m >= 0) {
                 const u64 me = team.sorted(m), w = tid < m ? (by_mass ? sample_weight((uint32_t)(me >> 32)) : 1) : 0;
@@ -500,9 +581,24 @@ __global__ void __launch_bounds__(kSampleThreads) sample_kernel(SampleParams p, 
                     s.cut = (me & 0xffffffff00000000ull) | ((uint32_t)me >> kSamplePlace);
                 __syncthreads();
                 cut = s.cut;
+                any_cut = true;
+                // this CTA's kept mass: earlier bins, earlier parts of the bin, its own listed tokens
+                u64 part = 0;
+                if (by_mass) {
+#pragma unroll
+                    for (int level = 0; level < 2; ++level)
+                        if (tid < bins[level])
+                            part += (u64)s.mass[level][0][tid] + ((u64)s.mass[level][1][tid] << 14) + ((u64)s.mass[level][2][tid] << 28);
+                    for (int j = lane; j < (int)s.n_list[warp]; j += 32)
+                        if (s.list[warp][j] <= cut) part += sample_weight((uint32_t)(s.list[warp][j] >> 32));
+                }
+                known = by_mass;
+                local = part;
                 return;
             }
         }
+        known = false;
+        any_cut = true;
         // too many: equal keys as a rule
         uint32_t lo = ~0u, hi = 0;
         if (tid == 0) {
@@ -556,15 +652,28 @@ __global__ void __launch_bounds__(kSampleThreads) sample_kernel(SampleParams p, 
     if (k > 0) find_cut(false);
     if (tp < 1.f) find_cut(true);
     auto kept = [&](int i) -> u64 { return weight_of(key_of(i), i); };
-    u64 mine, ahead, earlier;
-    scan_runs(kept, mine, ahead);
-    const u64 total = team.gather(&earlier);
-    const u64 r = draw(total);
-    ahead += earlier;
-    if (r >= ahead && r < ahead + mine) {
-        const int i = walk(kept, ahead, r);
-        p.out[row] = i0 + i;
-        if (p.prob) p.prob[row] = (float)kept(i) / (float)total;
+    u64 mine = 0, ahead = 0, earlier, total;
+    if (known) {  // only the CTA that the draw falls into looks at its tokens again
+        total = team.sum(local, &earlier);
+    } else {
+        scan_runs(kept, mine, ahead);
+        total = team.gather(&earlier);
+    }
+    const u64 here = s.xchg[(team.turn - 1) & 1], r = draw(total);
+    if (r >= earlier && r < earlier + here) {  // the whole CTA
+        if (known) {
+            mine = 0;
+#pragma unroll 4
+            for (int i = run_lo; i < run_hi; ++i) mine += kept(i);
+            u64 all;
+            ahead = team.scan(mine, all) - mine;
+        }
+        ahead += earlier;
+        if (r >= ahead && r < ahead + mine) {
+            const int i = walk(kept, ahead, r);
+            p.out[row] = i0 + i;
+            if (p.prob) p.prob[row] = (float)kept(i) / (float)total;
+        }
     }
     team.cl.sync();  // nobody leaves while its shared memory is read
 }
