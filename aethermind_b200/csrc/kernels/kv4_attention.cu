@@ -27,14 +27,16 @@ namespace amcu {
 // which makes the integer dot product exact up to fp32 sums; scale and minimum
 // of a key's group are applied to the 64-element sums (m through sum(q)). In the
 // second product the rows that come from low nibbles are 2^-4 of the others until
-// the end, the scales of V go into p (p s, rounded to 11 bits; fp32: as a high and
-// a low half), and the minima and the softmax denominator are three more rows of
-// the product. p s is fp16: where a warp's scales are below 2^-5 (fp32: always)
-// they are lifted by a power of two, so precision is relative to the largest scales
+// the end, the scales of V go into p (p s, rounded to 11 bits), and the minima and the softmax denominator are three more rows of
+// the product. p s is fp16: where a warp's scales are below 2^-5 they are lifted by a power of two, so precision is relative to the largest scales
 // that the warp meets, not to 6e-8. The MMA aligns its products by their operands'
 // exponents, subnormals' by that of 2^-14: sums with such codes are good to 2^-17 of
-// their largest term, which bf16 does not see; fp32 calls turn codes into normal
-// halves first ((1024 + c) - 1024).
+// their largest term, which bf16 does not see.
+//
+// fp32 calls work with normal halves around zero, c - 8 = (1024 + c) - 1032, and 8 s
+// more in the minimum. An average over many keys is small beside its terms, so
+// there V's elements are formed whole, m + s c in fp32, and go into the product as
+// a high and a low half; p, times 2^12 to keep its low half normal, does too.
 constexpr int kDecWarps = 8;
 constexpr int kDecThreads = kDecWarps * 32;
 constexpr int kDecStages = 4;  // 3, 5 and 6 measure within 2%
@@ -89,12 +91,12 @@ __device__ __forceinline__ int dec_chunk(int tk, int c) {
                     : (tk >> 2) * 8 + ((((tk & 3) << 1) + c) ^ (((tk >> 2) & 1) << 1));
 }
 
-// Codes in bits 0-3 (high: 4-7) of both halves as an MMA operand.
+// Codes in bits 0-3 (high: 4-7) of both halves as an MMA operand; kNormal: code - 8.
 template <bool kNormal>
 __device__ __forceinline__ uint32_t dec_code(uint32_t w, bool high) {
     if (!kNormal) return high ? w & 0x00F000F0u : w & 0x000F000Fu;
-    return h2u(high ? __hadd2(u2h((w & 0x00F000F0u) | 0x54005400u), __float2half2_rn(-64.f))
-                    : __hadd2(u2h((w & 0x000F000Fu) | 0x64006400u), __float2half2_rn(-1024.f)));
+    return h2u(high ? __hadd2(u2h((w & 0x00F000F0u) | 0x54005400u), __float2half2_rn(-72.f))
+                    : __hadd2(u2h((w & 0x000F000Fu) | 0x64006400u), __float2half2_rn(-1032.f)));
 }
 
 // Cost of sequence b in units, and what a segment needs of it.
@@ -328,7 +330,10 @@ __global__ void __launch_bounds__(kDecThreads, 2) kv4_decode_kernel(Kv4AttnParam
                 float2 sm[G];
                 const uint8_t* kr = kpar + (r + 8 * hh) * (4 * G);
 #pragma unroll
-                for (int g = 0; g < G; ++g) sm[g] = __half22float2(*reinterpret_cast<const __half2*>(kr + 4 * g));
+                for (int g = 0; g < G; ++g) {
+                    sm[g] = __half22float2(*reinterpret_cast<const __half2*>(kr + 4 * g));
+                    if (kWide) sm[g].y = fmaf(8.f, sm[g].x, sm[g].y);  // codes are 8 less
+                }
 #pragma unroll
                 for (int j = 0; j < (kWide ? 1 : 2); ++j) {
                     float dot = 0.f, add = 0.f;
@@ -380,15 +385,23 @@ __global__ void __launch_bounds__(kDecThreads, 2) kv4_decode_kernel(Kv4AttnParam
             }
             // ---- scales of V to where p s keeps its bits: at the warp's first unit, and again for much larger ones
             if (k == 0 || lift != 1.f) {
-                __half2 m2 = __hmax2(u2h(vs[0][0]), u2h(vs[1][0]));
-                if (G == 2) m2 = __hmax2(m2, __hmax2(u2h(vs[0][G - 1]), u2h(vs[1][G - 1])));
-                float top = fmaxf(__low2float(m2), __high2float(m2));  // over the unit's 16 keys: t tells them apart
+                float top = 0.f;  // over the unit's 16 keys: the largest scale, fp32: the largest element
+#pragma unroll
+                for (int hh = 0; hh < 2; ++hh)
+#pragma unroll
+                    for (int g = 0; g < G; ++g) {
+                        const float2 sv = __half22float2(u2h(vs[hh][g])), mv = __half22float2(u2h(vm[hh][g]));
+                        top = fmaxf(top, kWide ? fmaxf(fmaxf(fabsf(mv.x), fabsf(fmaf(15.f, sv.x, mv.x))),
+                                                       fmaxf(fabsf(mv.y), fabsf(fmaf(15.f, sv.y, mv.y))))
+                                               : fmaxf(sv.x, sv.y));
+                    }
                 top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, 1));
                 top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, 2));
-                const float fits = __uint_as_float((260u - (__float_as_uint(fmaxf(top, 6e-8f)) >> 23)) << 23);  // to [64, 128)
+                // to [64, 128), fp32: [1024, 2048)
+                const float fits = __uint_as_float(((kWide ? 264u : 260u) - (__float_as_uint(fmaxf(top, 6e-8f)) >> 23)) << 23);
                 if (k == 0) {
                     if (kWide || (top > 0.f && top < 0.03125f)) lift = fits;
-                } else if (top * lift >= 4096.f) {
+                } else if (top * lift >= (kWide ? 32768.f : 4096.f)) {
                     const float corr = fits / lift;
                     lift = fits;
 #pragma unroll
@@ -427,8 +440,8 @@ __global__ void __launch_bounds__(kDecThreads, 2) kv4_decode_kernel(Kv4AttnParam
                 }
             }
 #pragma unroll
-            for (int c = 0; c < 4; ++c) pr[c] = ex2(pr[c]);
-            uint32_t pb[2], ps[2][G];  // p, and p times the groups' scales
+            for (int c = 0; c < 4; ++c) pr[c] = kWide ? ex2(pr[c]) * 4096.f : ex2(pr[c]);
+            uint32_t pb[2], ps[2][G];  // p, and p times the groups' scales (bf16)
 #pragma unroll
             for (int hh = 0; hh < 2; ++hh) {
                 if (kWide) {
@@ -437,12 +450,6 @@ __global__ void __launch_bounds__(kDecThreads, 2) kv4_decode_kernel(Kv4AttnParam
                         return movm_trans(h2u(__halves2half2(h, __float2half_rn(x - __half2float(h)))));
                     };
                     pb[hh] = two(pr[2 * hh]);
-#pragma unroll
-                    for (int g = 0; g < G; ++g) {  // this lane's key is r or r + 8
-                        const __half sv = *reinterpret_cast<const __half*>(vpar + (r + 8 * hh) * (4 * G) + 4 * g);
-                        const bool seen = u * kDecUnit + r + 8 * hh <= lim_last;
-                        ps[hh][g] = two(seen ? pr[2 * hh] * (__half2float(sv) * lift) : 0.f);
-                    }
                 } else {
                     pb[hh] = movm_trans(h2u(__floats2half2_rn(pr[2 * hh], pr[2 * hh + 1])));
                     if (lift != 1.f) {
@@ -456,14 +463,14 @@ __global__ void __launch_bounds__(kDecThreads, 2) kv4_decode_kernel(Kv4AttnParam
                     for (int g = 0; g < G; ++g) ps[hh][g] = h2u(__hmul2(u2h(pb[hh]), u2h(vs[hh][g])));
                 }
             }
-            // ---- rows: minima of the groups, ones
+            // ---- rows: minima of the groups (fp32: none), ones
             {
                 uint32_t e[4] = {0, 0, 0, 0};
 #pragma unroll
                 for (int hh = 0; hh < 2; ++hh) {
                     uint32_t w = r == G ? 0x3C003C00u : 0u;
 #pragma unroll
-                    for (int g = 0; g < G; ++g) w = r == g ? vm[hh][g] : w;
+                    for (int g = 0; g < G; ++g) w = !kWide && r == g ? vm[hh][g] : w;
                     e[2 * hh] = w;
                 }
                 mma_f16_16816(xa, e, pb[0], pb[1]);
@@ -496,7 +503,24 @@ __global__ void __launch_bounds__(kDecThreads, 2) kv4_decode_kernel(Kv4AttnParam
                         const uint32_t wa = q2 ? w[0] >> 8 : w[0], wb = q2 ? w[1] >> 8 : w[1];
                         const uint32_t e[4] = {dec_code<kWide>(wa, false), dec_code<kWide>(wa, true), dec_code<kWide>(wb, false),
                                                dec_code<kWide>(wb, true)};
-                        mma_f16_16816(o[g][2 * part + q2], e, ps[0][g], ps[1][g]);
+                        if (kWide) {
+                            uint32_t hi[4], lo[4];
+#pragma unroll
+                            for (int i = 0; i < 4; ++i) {  // tokens 2t, 2t + 1 (i < 2) or 2t + 8, 2t + 9
+                                const float2 c = __half22float2(u2h(e[i])), sv = __half22float2(u2h(vs[i >> 1][g])),
+                                             mv = __half22float2(u2h(vm[i >> 1][g]));
+                                const float v0 = fmaf(c.x, sv.x, fmaf(8.f, sv.x, mv.x)) * lift;
+                                const float v1 = fmaf(c.y, sv.y, fmaf(8.f, sv.y, mv.y)) * lift;
+                                const __half2 h = __floats2half2_rn(v0, v1);
+                                const float2 hf = __half22float2(h);
+                                hi[i] = h2u(h);
+                                lo[i] = h2u(__floats2half2_rn(v0 - hf.x, v1 - hf.y));
+                            }
+                            mma_f16_16816(o[g][2 * part + q2], hi, pb[0], pb[1]);
+                            mma_f16_16816(o[g][2 * part + q2], lo, pb[0], pb[1]);
+                        } else {
+                            mma_f16_16816(o[g][2 * part + q2], e, ps[0][g], ps[1][g]);
+                        }
                     }
                 }
             }
