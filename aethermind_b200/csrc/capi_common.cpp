@@ -36,10 +36,15 @@ am_status_code set_error(am_status_code code, const char* fmt, ...) {
 void clear_error() { g_last_error.clear(); }
 
 int num_sms() {
-    int dev = 0, n = 0;
-    if (cudaGetDevice(&dev) != cudaSuccess) return 148;
-    if (cudaDeviceGetAttribute(&n, cudaDevAttrMultiProcessorCount, dev) != cudaSuccess || n <= 0) return 148;
-    return n;
+    static int per_dev[64] = {};
+    int dev = 0;
+    if (cudaGetDevice(&dev) != cudaSuccess || dev < 0 || dev >= 64) return 148;
+    if (per_dev[dev] == 0) {  // benign race: every writer stores the same value
+        int n = 0;
+        if (cudaDeviceGetAttribute(&n, cudaDevAttrMultiProcessorCount, dev) != cudaSuccess || n <= 0) return 148;
+        per_dev[dev] = n;
+    }
+    return per_dev[dev];
 }
 
 bool pdl_enabled() {

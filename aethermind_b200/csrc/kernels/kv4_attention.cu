@@ -709,6 +709,7 @@ extern "C" am_status_code amcu_attn_kv4(const AmcuKv4AttentionArgs* a, void* str
     AMCU_REQUIRE(a->n_q_heads > 0 && a->n_q_heads <= 65536 && a->n_q_heads % a->cache.n_kv_heads == 0,
                  "amcu_attn_kv4: n_q_heads must be a positive multiple of n_kv_heads");
     AMCU_REQUIRE(a->scale >= 0.f && a->scale < INFINITY, "amcu_attn_kv4: scale must be finite and not negative");
+    AMCU_REQUIRE(a->batch.rows * a->n_q_heads <= (1 << 28), "amcu_attn_kv4: rows * n_q_heads must be at most 2^28");
     if (a->batch.rows == 0 || a->batch.n_seq == 0) return AM_STATUS_OK;
     AMCU_REQUIRE(a->q && a->out, "amcu_attn_kv4: null pointer");
     p.q = a->q;

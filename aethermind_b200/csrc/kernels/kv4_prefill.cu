@@ -662,12 +662,13 @@ static void launch_prefill(const Kv4AttnParams& p, unsigned ctas, cudaStream_t s
 }
 
 bool kv4_prefill_wanted(const Kv4View& v, int64_t grp) {
-    const int64_t cols = v.rows * grp, tiles = (cols / kPfRows + v.n_seq) * v.nkv;
-    // One wave of row tiles takes about as long per key as 1.5 eight-column
-    // tiles of the other kernel on every SM (2500 cycles per 128 keys against
-    // 207 per 16): take it once there are more columns than that.
-    const int64_t sms = num_sms();
-    return ceil_div(cols, 8) * v.nkv * 2 > 3 * sms * ceil_div(tiles, sms);
+    // A wave of row tiles (one to an SM) takes about as long as 2.5 eight-column
+    // tiles of the other kernel on every SM: this kernel once there are more columns.
+    // Measured (us, this / the other; 32 / 8 heads of 128, one sequence): 4096 keys, 96
+    // rows 90 / 80, 128 rows 91 / 97, 256 rows 89 / 170; 1000 keys, 64 rows 38 / 39, 128
+    // rows 37 / 52. Four sequences of 16 rows over 4096 keys: 81 / 62, of 32: 81 / 97.
+    const int64_t cols = v.rows * grp, tiles = (cols / kPfRows + v.n_seq) * v.nkv, sms = num_sms();
+    return ceil_div(cols, 8) * v.nkv * 2 > 5 * sms * ceil_div(tiles, sms);
 }
 
 am_status_code kv4_prefill_launch(const Kv4AttnParams& p, int64_t d, cudaStream_t s) {

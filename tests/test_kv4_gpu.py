@@ -151,6 +151,68 @@ def test_attention_prompts(ops, lens, nq, nkv, d, page):
     assert torch.equal(got, again)
 
 
+MORE_PROMPTS = [  # the kernel of prompts takes over at some 400 columns (row, q head of the group) of 8 kv heads
+    ([(160, 160)], 32, 8, 128, 16),
+    ([(300, 128), (301, 129)], 32, 8, 64, 64),
+    ([(513, 200)], 16, 16, 64, 128),
+    ([(257, 130)], 32, 8, 128, 256),
+    ([(128, 128), (0, 0), (2, 2)], 40, 8, 128, 32),
+]
+
+
+@pytest.mark.parametrize("lens,nq,nkv,d,page", MORE_PROMPTS)
+def test_attention_more_prompts(ops, lens, nq, nkv, d, page):
+    test_attention_prompts(ops, lens, nq, nkv, d, page)
+
+
+@pytest.mark.parametrize("rows", [128, 150])
+def test_attention_prompts_moving_reference(ops, rows):
+    """Scores that grow along the keys, in the kernel of prompts."""
+    rng = np.random.default_rng(41)
+    nq, nkv, d, page = 32, 8, 128, 64
+    table, start, ctx, total = make_batch([(600, rows)], page, rng)
+    kc, kp, vc, vp = random_cache(total, nkv, page, d, rng)
+    for i in range(600):
+        kp[table[0, i // page], :, i % page, :, 1] += np.float16(0.002 * i)
+    q = bf16(np.abs(rng.normal(0, 1, (rows, nq * d))))
+    want = ref.attention(q.double().numpy(), (kc, kp, vc, vp), table, start, ctx, nq, nkv, d)
+    got = ops.attention_kv4(q.cuda(), dev((kc, kp, vc, vp)), di(table), di(start), di(ctx), nq, nkv, d)
+    got = got.double().cpu().numpy()
+    # scores up to 100 from keys rounded to 11 bits: 2^-12 of them in the exponent, shared by a key's terms
+    assert np.linalg.norm(got - want) <= 2.0 ** -4 * np.linalg.norm(want)
+
+
+def test_attention_prompts_largest_elements(ops):
+    """Elements at and beyond fp16's largest value in the kernel of prompts."""
+    rng = np.random.default_rng(43)
+    nq, nkv, d, page = 32, 8, 128, 16
+    table, start, ctx, total = make_batch([(200, 140)], page, rng)
+    kc, kp, vc, vp = random_cache(total, nkv, page, d, rng)
+    vp[..., 0], vp[..., 1] = np.float16(4366), np.float16(0)
+    kp[..., 0], kp[..., 1] = np.float16(4000), np.float16(-30000)
+    q = bf16(rng.normal(0, 1e-5, (140, nq * d)))
+    want = ref.attention(q.double().numpy(), (kc, kp, vc, vp), table, start, ctx, nq, nkv, d)
+    got = ops.attention_kv4(q.cuda(), dev((kc, kp, vc, vp)), di(table), di(start), di(ctx), nq, nkv, d)
+    assert np.linalg.norm(got.double().cpu().numpy() - want) <= 2.0 ** -7 * np.linalg.norm(want)
+    vp[..., 1] = np.float16(30000)  # 30000 + 15 * 4366 is beyond fp16: taken as 65504
+    got = ops.attention_kv4(q.cuda(), dev((kc, kp, vc, vp)), di(table), di(start), di(ctx), nq, nkv, d)
+    assert torch.isfinite(got).all()
+
+
+@pytest.mark.parametrize("lens", [[(32768, 1)], [(20000, 2), (9, 1)]])
+def test_attention_fp32_flat_average(ops, lens):
+    """An average over many keys is small beside its terms; it is held to 2e-6 of itself (p and the sums in 22 to 24
+    bits, a result 2^-7 of its terms)."""
+    rng = np.random.default_rng(44)
+    nq, nkv, d, page = 4, 2, 64, 64
+    table, start, ctx, total = make_batch(lens, page, rng)
+    cache = random_cache(total, nkv, page, d, rng)
+    q = torch.from_numpy(rng.normal(0, 0.3, (start[-1], nq * d)).astype(np.float32))
+    want = ref.attention(q.double().numpy(), cache, table, start, ctx, nq, nkv, d)
+    got = ops.attention_kv4(q.cuda(), dev(cache), di(table), di(start), di(ctx), nq, nkv, d).double().cpu().numpy()
+    assert np.linalg.norm(got - want) <= 2e-6 * np.linalg.norm(want)
+
+
 def test_attention_prompts_rising_scores(ops):
     """Scores that grow along the keys, so that the softmax reference moves many times."""
     rng = np.random.default_rng(31)
