@@ -153,9 +153,8 @@ __device__ __forceinline__ uint32_t kv4_codes(const float (&x)[4], float s, floa
 // Bound by instruction issue for prompts (260 per warp and step of 8 elements a
 // lane; DRAM at a third of its rate): the row's sequence, cos / sin and norm
 // weights are fetched once for U steps, whose loads are all in flight together.
-// 9188 rows of 32 + 16 heads of 64 with norms: 66 us with one step a warp and
-// two elements a load, 51 with this layout, 37 with the division avoided and the
-// sums of four elements shared out over the lanes.
+// 9188 rows of 32 + 16 heads of 64 with norms: 51 us with this layout, 37 with
+// the division avoided and the sums of four elements shared out over the lanes.
 template <typename T, int D, int U>
 __global__ void __launch_bounds__(128) kv4_append_kernel(Kv4AppendParams p) {
     constexpr int LPH = D / 8, HPW = 32 / LPH, half = D / 2;

@@ -15,7 +15,8 @@ namespace amcu {
 
 struct SampleParams {
     const void* logits;
-    int64_t stride, vocab;
+    int64_t stride, vocab, rows;
+    int64_t ahead;  // rows between one that runs and the one that takes its place
     const float* uniform;
     const float* temperature;
     const int32_t* top_k;
@@ -47,31 +48,76 @@ __device__ __forceinline__ uint32_t sample_key(float x, float mx, float t) {
     const float z = __fdiv_rn(__fsub_rn(x, mx), t);
     return z <= 0.f ? __float_as_uint(-z) & 0x7fffffffu : kSampleNever;  // NaN: comparison is false
 }
-// floor(expf(-|z|) * 2^40), from the float's fields (a 64-bit conversion is slow).
-__device__ __forceinline__ u64 sample_weight(uint32_t key) {
-    const uint32_t f = __float_as_uint(expf(-__uint_as_float(key)));
-    const uint32_t m = (f & 0x007fffffu) | 0x00800000u;
-    const int sh = (int)(f >> 23) - 110;
-    return sh >= 0 ? (u64)m << sh : (u64)(sh > -24 ? m >> -sh : 0u);
+// The same for rows in whose whole range no step leaves the normal numbers
+// (sample_plain): two corrections of the quotient by its exact remainder with a
+// correctly rounded reciprocal give the correctly rounded quotient (Markstein,
+// IBM J. Res. Dev. 34, 1990), without a branch.
+__device__ __forceinline__ uint32_t sample_key_plain(float x, float mx, float t, float inv) {
+    const float a = __fsub_rn(x, mx);
+    float z = __fmul_rn(a, inv);
+    z = __fmaf_rn(__fmaf_rn(-z, t, a), inv, z);
+    z = __fmaf_rn(__fmaf_rn(-z, t, a), inv, z);
+    return __float_as_uint(z) & 0x7fffffffu;  // masked tokens: NaN, whose weight is 0 and whose bin is the last
 }
+// The largest logit is not tiny (differences from it are then 0 or above 2^-85)
+// nor infinite, and the temperature is within 2^+-40.
+__device__ __forceinline__ bool sample_plain(float mx, float t) {
+    return fabsf(mx) >= 0x1p-60f && fabsf(mx) <= 0x1p120f && t >= 0x1p-40f && t <= 0x1p40f;
+}
+// floor(e * 2^40) of an e in [0, 1], its upper 21 and lower 20 bits, each added to
+// a sum together with kSampleHi, kSampleLo (an addition that truncates at 2^-20,
+// one of the exact rest at 2^-40; 64-bit conversions and shifts are slow).
+constexpr uint32_t kSampleHi = 0x41000000u, kSampleLo = 0x37000000u;  // 8 and 2^-17
+__device__ __forceinline__ void sample_split(float e, uint32_t& hi, uint32_t& lo) {
+    const float a = __fadd_rz(e, 8.f);
+    hi += __float_as_uint(a);
+    lo += __float_as_uint(__fadd_rz(__fsub_rn(e, __fsub_rn(a, 8.f)), 0x1p-17f));
+}
+__device__ __forceinline__ u64 sample_whole(float e) {
+    uint32_t hi = 0u - kSampleHi, lo = 0u - kSampleLo;
+    sample_split(e, hi, lo);
+    return ((u64)hi << 20) + lo;
+}
+__device__ __forceinline__ float sample_exp(uint32_t key) { return expf(-__uint_as_float(key)); }
+__device__ __forceinline__ u64 sample_weight(uint32_t key) { return sample_whole(sample_exp(key)); }
 // Position of a key on a scale of 256 bins (a weight above 0 is below 254); bin
 // and sub-bin are monotone in the key.
 __device__ __forceinline__ float sample_place(uint32_t key) { return __fmul_rn(__uint_as_float(key), kSampleBinScale); }
-__device__ __forceinline__ int sample_bin(float place) { return (int)fminf(place, (float)(kSampleBins - 1)); }
+__device__ __forceinline__ int sample_bin(float place) {  // truncated by an addition; NaN is in the last bin
+    return (int)(__float_as_uint(__fadd_rz(fminf(place, (float)(kSampleBins - 1)), 0x1p23f)) - 0x4b000000u);
+}
 __device__ __forceinline__ int sample_sub(float place, int bin) {
     return min((int)__fmul_rn(__fsub_rn(place, (float)bin), 256.f), kSampleBins - 1);
 }
 
+// A weight's bits for 32-bit sums (64-bit shared atomics are far slower): two
+// fields of 20 bits and 21 for slices of up to 2^14 tokens, three of 14 for slices
+// up to 2^18. Lanes with the same low bits share a copy of the histogram, which
+// so gets 2^11 tokens (2^16) at most.
+template <bool kRes> struct SampleSplit {
+    static constexpr int kFields = kRes ? 2 : 3, kBits = kRes ? 20 : 14, kCopies = kRes ? 8 : 4;
+    static __device__ __forceinline__ int at(int field, int bin, int copy) {
+        return (field * kSampleBins + bin) * kCopies + copy;
+    }
+};
+constexpr int kSampleHist = 2 * kSampleBins * 8;
+
 struct SampleShared {
-    uint32_t mass[2][3][kSampleBins];  // a weight's bits 0-13, 14-27 and 28-40 (64-bit shared atomics are far slower)
+    u64 mass[2][kSampleBins];  // of the tokens in a bin: weights, or their number
     uint32_t count[2][kSampleBins];
     float group[kSampleThreads];       // maxima of the threads, or of 2, 4 or 8 neighbours
     u64 list[kSampleWarps][kSampleWarpList];  // each warp's candidates
     uint32_t n_list[kSampleWarps];
+    uint32_t n_queue[kSampleWarps];
+    union {
+        alignas(16) uint32_t hist[kSampleHist];
+        struct {
+            u64 all[kSampleList];        // every CTA's
+            u64 weight[kSampleList];     // by place: weights of the kept
+            u64 tmp[kSampleList];
+        };
+    };
     uint32_t queue[kSampleWarps][kSampleQueue];
-    u64 all[kSampleList];        // every CTA's
-    u64 weight[kSampleList];     // by place: weights of the kept
-    u64 tmp[kSampleList];
     u64 part[kSampleWarps];
     u64 scan[kSampleBins / 32];
     u64 xchg[2];
@@ -157,7 +203,8 @@ struct SampleTeam {
 
     // all[0 .. m) in ascending order, one per thread (~0 past the end): up to 128
     // by counting the smaller ones; more are put into the 256 bins of z first and
-    // counted within their bin (512 tokens of a row: 1 us, a bitonic sort 4).
+    // counted within their bin (33 rows of 509 tokens: 9.9 us a call, by a bitonic
+    // sort 12.4).
     __device__ u64 sorted(int m) {
         const int tid = threadIdx.x;
         const u64 me = tid < m ? s->all[tid] : ~0ull;
@@ -226,8 +273,17 @@ struct SampleTeam {
 // * Otherwise a cut is found by a histogram of 256 bins of z, one of 256 parts
 //   of the bin that it falls in, and sorting what is in that part; equal keys by
 //   the thousand (bf16 logits) are told apart by their index alone.
+//
+// Bound by latency (exchanges of the cluster, barriers) and, without top-k, by
+// the instructions per token (22 for the mass, 30 and two shared atomics for the
+// histogram). The next row of these SMs is fetched into L2 meanwhile. 192 fp32
+// rows of 128256: 45 us if all are greedy, 88 with top-k 40, 92 with the
+// temperature alone, 178 with top-p 0.95, 165 with top-k 1000. Before the
+// division without a branch, split sums, copies of the histogram and the
+// drawn run walked by a warp: 50, 91, 139, 265, 227.
 template <typename T, bool kRes>
 __global__ void __launch_bounds__(kSampleThreads) sample_kernel(SampleParams p, int slice) {
+    using Split = SampleSplit<kRes>;
     extern __shared__ __align__(16) float xs[];
     __shared__ SampleShared s;
     SampleTeam team{&s, cg::this_cluster(), 0, 0, 0};
@@ -245,7 +301,9 @@ __global__ void __launch_bounds__(kSampleThreads) sample_kernel(SampleParams p, 
     int64_t k = p.top_k ? p.top_k[row] : 0;
     const float tp = p.top_p ? p.top_p[row] : 1.f, mp = p.min_p ? p.min_p[row] : 0.f;
     const float un = p.uniform[row];
-    const u64 least = mp > 0.f ? max((u64)ceil((double)fminf(mp, 1.f) * (double)kSampleOne), (u64)1) : 1;
+    // the least e whose weight floor(e * 2^40) is above 0 and reaches min_p
+    const float least = mp > 0.f ? __double2float_ru(fmax(ceil((double)fminf(mp, 1.f) * (double)kSampleOne), 1.0) / (double)kSampleOne)
+                                 : 1.f / kSampleOne;
 
     // Place of the draw in a mass of `total` > 0.
     auto draw = [&](u64 total) -> u64 {
@@ -334,6 +392,12 @@ __global__ void __launch_bounds__(kSampleThreads) sample_kernel(SampleParams p, 
                 at = i;
             }
         }
+        if (kRes && tid < ((-n) & 3)) xs[n + tid] = -INFINITY;
+        if (tid == 0 && vec && n * (int)sizeof(T) >= 16 && row + p.ahead < p.rows) {
+            const T* next = x + p.ahead * p.stride;
+            if ((reinterpret_cast<uintptr_t>(next) & 15) == 0)
+                asm volatile("cp.async.bulk.prefetch.L2.global [%0], %1;" ::"l"(next), "r"(n * (int)sizeof(T) & ~15) : "memory");
+        }
         u64 best = mx > -INFINITY ? ((u64)float_order_key(mx + 0.f) << 32) | (0xffffffffu - (uint32_t)(i0 + at)) : 0;
         best = warp_max_u64(best);
         if (lane == 0) s.part[warp] = best;
@@ -390,7 +454,7 @@ __global__ void __launch_bounds__(kSampleThreads) sample_kernel(SampleParams p, 
                 const float f = kRes ? xs[i] : Act<T>::load(x[i]);
                 if (!(f >= edge)) return kNone;
                 const uint32_t key = sample_key(f, all, t);
-                if (key >= kSampleNever || sample_bin(sample_place(key)) > bin || sample_weight(key) < least) return kNone;
+                if (key >= kSampleNever || sample_bin(sample_place(key)) > bin || !(sample_exp(key) >= least)) return kNone;
                 return ((u64)key << 32) | (u64)(i0 + i);
             });
             const int m = team.collect();
@@ -423,34 +487,63 @@ __global__ void __launch_bounds__(kSampleThreads) sample_kernel(SampleParams p, 
 
     // ---- the general case
     team.cl.sync();  // lists of an attempt above are read
-    bool keyed = false;  // xs holds keys: the first pass over the tokens makes them
+    bool keyed = false;  // xs holds keys: the first histogram makes them
+    const bool plain = sample_plain(mx, t);
+    const float inv = __frcp_rn(t);
+    if (kRes && !plain) {
+        for (int i = tid; i < ((n + 3) & ~3); i += kSampleThreads) xs[i] = __uint_as_float(sample_key(xs[i], mx, t));
+        keyed = true;
+        __syncthreads();
+    }
     auto key_of = [&](int i) -> uint32_t {
-        if (kRes && keyed) return __float_as_uint(xs[i]);
-        return sample_key(kRes ? xs[i] : Act<T>::load(x[i]), mx, t);
+        if (kRes) return keyed ? __float_as_uint(xs[i]) : sample_key_plain(xs[i], mx, t, inv);
+        const float f = Act<T>::load(x[i]);
+        return plain ? sample_key_plain(f, mx, t, inv) : sample_key(f, mx, t);
     };
     bool any_cut = false;
     u64 cut = ~0ull;  // tokens up to it in the order of (key, index) are kept
     auto comp_of = [&](uint32_t key, int i) -> u64 { return ((u64)key << 32) | (u64)(i0 + i); };
-    auto weight_of = [&](uint32_t key, int i) -> u64 {  // 0 where the token is not kept
-        if (any_cut && comp_of(key, i) > cut) return 0;
-        const u64 w = sample_weight(key);
-        return w >= least ? w : 0;
+    auto exp_of = [&](uint32_t key, int i) -> float {  // 0 where the token is not kept
+        if (any_cut && comp_of(key, i) > cut) return 0.f;
+        const float e = sample_exp(key);
+        return e >= least ? e : 0.f;
     };
-    // scan_runs: f's sum over the thread's run, the sums of the threads before it,
-    // and the CTA's total in xchg; walk: the first i of the run whose running f is
-    // above `target`.
-    auto scan_runs = [&](auto f, u64& mine, u64& before) {
-        mine = 0;
+    auto weight_of = [&](uint32_t key, int i) -> u64 { return sample_whole(exp_of(key, i)); };
+    // The kept mass of the thread's run.
+    auto run_mass = [&]() -> u64 {
+        const uint32_t c = (uint32_t)(run_hi - run_lo);
+        uint32_t hi = 0u - c * kSampleHi, lo = 0u - c * kSampleLo;
+        if (kRes && !keyed) {
 #pragma unroll 4
-        for (int i = run_lo; i < run_hi; ++i) mine += f(i);
+            for (int i = run_lo; i < run_hi; ++i) sample_split(exp_of(sample_key_plain(xs[i], mx, t, inv), i), hi, lo);
+        } else {
+#pragma unroll 4
+            for (int i = run_lo; i < run_hi; ++i) sample_split(exp_of(key_of(i), i), hi, lo);
+        }
+        return ((u64)hi << 20) + lo;  // runs are 512 tokens at most
+    };
+    // scan_runs: the sum over the thread's run, those of the threads before it, and
+    // the CTA's total in xchg; walk: the first token of the CTA with a running f
+    // above `target`, given to `hit` by the lane that finds it (`before` and `mine`
+    // as scan_runs left them, plus what other CTAs have): the warp whose thread's
+    // run it is in goes through that run together.
+    auto scan_runs = [&](auto f, u64& mine, u64& before) {
+        mine = f();
         u64 all;
         before = team.scan(mine, all) - mine;
         if (tid == 0) s.xchg[team.turn & 1] = all;
     };
-    auto walk = [&](auto f, u64 before, u64 target) -> int {
-        for (int i = run_lo;; ++i) {
-            before += f(i);
-            if (before > target) return i;
+    auto walk = [&](auto f, u64 before, u64 mine, u64 target, auto hit) {
+        const uint32_t owner = __ballot_sync(0xffffffffu, before <= target && target - before < mine);
+        if (!owner) return;
+        const int src = __ffs(owner) - 1;
+        const int lo = __shfl_sync(0xffffffffu, run_lo, src), hi = __shfl_sync(0xffffffffu, run_hi, src);
+        before = __shfl_sync(0xffffffffu, before, src);
+        for (int at = lo; at < hi; at += 32) {
+            const u64 v = at + lane < hi ? f(at + lane) : 0, inc = before + warp_scan_u64(v);
+            if (inc - v <= target && target < inc) hit(at + lane);
+            before = __shfl_sync(0xffffffffu, inc, 31);
+            if (target < before) return;
         }
     };
 
@@ -464,68 +557,114 @@ __global__ void __launch_bounds__(kSampleThreads) sample_kernel(SampleParams p, 
         uint32_t members = 0;
         int queued = -1;  // this warp's tokens of the first level's bin, in s.queue; -1: too many
         for (int level = 0; level < 2; ++level) {
-            if (tid < kSampleBins) {
-                s.mass[level][0][tid] = s.mass[level][1][tid] = s.mass[level][2][tid] = 0;
-                s.count[level][tid] = 0;
-            }
+            for (int j = tid; j < kSampleHist / 4; j += kSampleThreads) reinterpret_cast<uint4*>(s.hist)[j] = make_uint4(0, 0, 0, 0);
+            if (tid < kSampleBins) s.count[level][tid] = 0;
+            if (lane == 0) s.n_queue[warp] = 0;
             __syncthreads();
             const float bin_lo = (float)bins[0], bin_hi = bin_lo + 1.f;
+            const int copy = lane & (Split::kCopies - 1);
             auto add = [&](int i, uint32_t key) {
                 const float place = sample_place(key);
                 if (level == 1 && !(place >= bin_lo && place < bin_hi)) return;
                 const int bin = level == 1 ? sample_sub(place, bins[0]) : sample_bin(place);
-                const u64 w = weight_of(key, i);
-                if (!w) return;
-                if (by_mass) {
-                    const uint32_t lo = (uint32_t)w & 0x3fffu, mid = (uint32_t)(w >> 14) & 0x3fffu, hi = (uint32_t)(w >> 28);
-                    atomicAdd(&s.mass[level][0][bin], lo);
-                    if (mid) atomicAdd(&s.mass[level][1][bin], mid);
-                    if (hi) atomicAdd(&s.mass[level][2][bin], hi);
+                const float e = exp_of(key, i);
+                if (!(e > 0.f)) return;
+                if (by_mass && kRes) {
+                    uint32_t hi = 0u - kSampleHi, lo = 0u - kSampleLo;
+                    sample_split(e, hi, lo);
+                    atomicAdd(&s.hist[Split::at(0, bin, copy)], lo);
+                    if (hi) atomicAdd(&s.hist[Split::at(1, bin, copy)], hi);
+                    if (level == 1) atomicAdd(&s.count[1][bin], 1u);
+                } else if (by_mass) {
+                    const u64 w = sample_whole(e);
+                    constexpr uint32_t low = (1u << Split::kBits) - 1;
+                    atomicAdd(&s.hist[Split::at(0, bin, copy)], (uint32_t)w & low);
+#pragma unroll
+                    for (int f = 1; f < Split::kFields; ++f) {
+                        const uint32_t v = (uint32_t)(w >> (f * Split::kBits)) & (f < Split::kFields - 1 ? low : ~0u);
+                        if (v) atomicAdd(&s.hist[Split::at(f, bin, copy)], v);
+                    }
+                    if (level == 1) atomicAdd(&s.count[1][bin], 1u);
+                } else {
+                    atomicAdd(&s.hist[Split::at(0, bin, copy)], 1u);
                 }
-                if (!by_mass || level == 1) atomicAdd(&s.count[level][bin], 1u);
             };
             if (level == 0) {
-                if (kRes && !keyed) {
-#pragma unroll 2
-                    for (int i = tid; i < n; i += kSampleThreads) {
-                        xs[i] = __uint_as_float(sample_key(xs[i], mx, t));
-                        add(i, __float_as_uint(xs[i]));
+                if (kRes) {
+                    for (int i = 4 * tid; i < n; i += 4 * kSampleThreads) {
+                        uint4 y = *reinterpret_cast<const uint4*>(xs + i);
+                        if (!keyed) {
+                            y.x = sample_key_plain(__uint_as_float(y.x), mx, t, inv);
+                            y.y = sample_key_plain(__uint_as_float(y.y), mx, t, inv);
+                            y.z = sample_key_plain(__uint_as_float(y.z), mx, t, inv);
+                            y.w = sample_key_plain(__uint_as_float(y.w), mx, t, inv);
+                            *reinterpret_cast<uint4*>(xs + i) = y;
+                        }
+                        add(i, y.x);
+                        add(i + 1, y.y);
+                        add(i + 2, y.z);
+                        add(i + 3, y.w);
                     }
                     keyed = true;
-                    __syncthreads();
                 } else {
 #pragma unroll 2
                     for (int i = tid; i < n; i += kSampleThreads) add(i, key_of(i));
                 }
             } else {
                 // the bin's tokens first, so that they are looked at by full warps
-                uint32_t c = 0;
-#pragma unroll 2
-                for (int at = seg_lo; at < seg_hi; at += 32) {
-                    const float place = at + lane < seg_hi ? sample_place(key_of(at + lane)) : -1.f;
-                    const uint32_t m = __ballot_sync(0xffffffffu, place >= bin_lo && place < bin_hi);
-                    const uint32_t o = c + __popc(m & ((1u << lane) - 1));
-                    if (((m >> lane) & 1u) && o < kSampleQueue) s.queue[warp][o] = (uint32_t)(at + lane);
-                    c += __popc(m);
+                auto put = [&](int i, uint32_t key) {
+                    const float place = sample_place(key);
+                    if (!(place >= bin_lo && place < bin_hi)) return;
+                    const uint32_t o = atomicAdd(&s.n_queue[warp], 1u);
+                    if (o < kSampleQueue) s.queue[warp][o] = (uint32_t)i;
+                };
+                if (kRes) {
+                    const uint32_t lo = __float_as_uint(bin_lo / kSampleBinScale * 0.999999f);  // a little wider than the bin
+                    const uint32_t span = __float_as_uint(bin_hi / kSampleBinScale * 1.000001f) - lo;
+#pragma unroll 4
+                    for (int i = seg_lo + 4 * lane; i < seg_hi; i += 128) {
+                        const uint4 y = *reinterpret_cast<const uint4*>(xs + i);
+                        if (min(min(y.x - lo, y.y - lo), min(y.z - lo, y.w - lo)) > span) continue;
+                        put(i, y.x);
+                        put(i + 1, y.y);
+                        put(i + 2, y.z);
+                        put(i + 3, y.w);
+                    }
+                } else {
+                    for (int i = seg_lo + lane; i < seg_hi; i += 32) put(i, key_of(i));
                 }
                 __syncwarp();
-                queued = c <= kSampleQueue ? (int)c : -1;
+                const int c = (int)s.n_queue[warp];
+                queued = c <= kSampleQueue ? c : -1;
                 if (queued >= 0)
                     for (int j = lane; j < queued; j += 32) add((int)s.queue[warp][j], key_of((int)s.queue[warp][j]));
                 else
                     for (int i = seg_lo + lane; i < seg_hi; i += 32) add(i, key_of(i));
+            }
+            __syncthreads();
+            if (tid < kSampleBins) {
+                u64 sum = 0;
+#pragma unroll
+                for (int f = 0; f < Split::kFields; ++f) {
+                    u64 part = 0;
+#pragma unroll
+                    for (int c = 0; c < Split::kCopies; c += 4) {
+                        const uint4 y = *reinterpret_cast<const uint4*>(&s.hist[Split::at(f, tid, c)]);
+                        part += (u64)y.x + y.y + y.z + y.w;
+                    }
+                    sum += part << (f * Split::kBits);
+                }
+                s.mass[level][tid] = sum;
             }
             team.cl.sync();
             u64 v = 0, cnt = 0;
             if (tid < kSampleBins) {
 #pragma unroll 4
                 for (int r = 0; r < team.C; ++r) {
-                    if (by_mass)
-                        v += (u64)team.at(r, &s.mass[level][0][tid]) + ((u64)team.at(r, &s.mass[level][1][tid]) << 14) +
-                             ((u64)team.at(r, &s.mass[level][2][tid]) << 28);
-                    if (!by_mass || level == 1) cnt += team.at(r, &s.count[level][tid]);
+                    v += team.at(r, &s.mass[level][tid]);
+                    if (by_mass && level == 1) cnt += team.at(r, &s.count[1][tid]);
                 }
-                if (!by_mass) v = cnt;
+                if (!by_mass) cnt = v;
             }
             const u64 inc = warp_scan_u64(v);
             if (lane == 31 && warp < kSampleBins / 32) s.scan[warp] = inc;
@@ -538,7 +677,10 @@ __global__ void __launch_bounds__(kSampleThreads) sample_kernel(SampleParams p, 
                     need = want < 1.0 ? 1 : (u64)want;
                 } else {
                     need = (u64)k;
-                    if (need >= all) return;  // nothing to cut
+                    if (need >= all) {  // nothing to cut
+                        team.cl.sync();  // the masses are read
+                        return;
+                    }
                 }
             }
             if (tid < kSampleBins) {
@@ -590,8 +732,7 @@ __global__ void __launch_bounds__(kSampleThreads) sample_kernel(SampleParams p, 
                 if (by_mass) {
 #pragma unroll
                     for (int level = 0; level < 2; ++level)
-                        if (tid < bins[level])
-                            part += (u64)s.mass[level][0][tid] + ((u64)s.mass[level][1][tid] << 14) + ((u64)s.mass[level][2][tid] << 28);
+                        if (tid < bins[level]) part += s.mass[level][tid];
                     for (int j = lane; j < (int)s.n_list[warp]; j += 32)
                         if (s.list[warp][j] <= cut) part += sample_weight((uint32_t)(s.list[warp][j] >> 32));
                 }
@@ -609,11 +750,15 @@ __global__ void __launch_bounds__(kSampleThreads) sample_kernel(SampleParams p, 
             s.kmax = 0;
         }
         u64 mine, ahead, earlier;
-        scan_runs([&](int i) -> u64 {
-            if (!in_bin(i)) return 0;
-            lo = min(lo, key_of(i));
-            hi = max(hi, key_of(i));
-            return 1;
+        scan_runs([&]() -> u64 {
+            u64 c = 0;
+            for (int i = run_lo; i < run_hi; ++i)
+                if (in_bin(i)) {
+                    lo = min(lo, key_of(i));
+                    hi = max(hi, key_of(i));
+                    ++c;
+                }
+            return c;
         }, mine, ahead);  // its barrier comes after kmin and kmax are set
         lo = __reduce_min_sync(0xffffffffu, lo);
         hi = __reduce_max_sync(0xffffffffu, hi);
@@ -628,9 +773,8 @@ __global__ void __launch_bounds__(kSampleThreads) sample_kernel(SampleParams p, 
             const u64 w = by_mass ? sample_weight(lo) : 1, m = (need - before + w - 1) / w;
             if (tid == 0) s.cut = 0;
             __syncthreads();
-            ahead += earlier;
-            if (ahead < m && m <= ahead + mine)
-                s.cut = comp_of(lo, walk([&](int j) -> u64 { return in_bin(j) ? 1 : 0; }, ahead, m - 1));
+            walk([&](int j) -> u64 { return in_bin(j) ? 1 : 0; }, ahead + earlier, mine, m - 1,
+                 [&](int i) { s.cut = comp_of(lo, i); });
             team.cl.sync();
             const u64 c = lane < team.C ? team.at(lane, &s.cut) : 0;  // one of them is not 0 (or the cut is)
             cut = warp_sum_u64(c);
@@ -659,26 +803,21 @@ __global__ void __launch_bounds__(kSampleThreads) sample_kernel(SampleParams p, 
     if (known) {  // only the CTA that the draw falls into looks at its tokens again
         total = team.sum(local, &earlier);
     } else {
-        scan_runs(kept, mine, ahead);
+        scan_runs(run_mass, mine, ahead);
         total = team.gather(&earlier);
     }
     const u64 here = s.xchg[(team.turn - 1) & 1], r = draw(total);
-    if (r >= earlier && r < earlier + here) {  // the whole CTA
-        if (known) {
-            mine = 0;
-#pragma unroll 4
-            for (int i = run_lo; i < run_hi; ++i) mine += kept(i);
-            u64 all;
-            ahead = team.scan(mine, all) - mine;
-        }
-        ahead += earlier;
-        if (r >= ahead && r < ahead + mine) {
-            const int i = walk(kept, ahead, r);
-            p.out[row] = i0 + i;
-            if (p.prob) p.prob[row] = (float)kept(i) / (float)total;
-        }
+    team.cl.sync();  // shared memory of others is read: the CTAs without the drawn token leave
+    if (r < earlier || r - earlier >= here) return;
+    if (known) {
+        mine = run_mass();
+        u64 all;
+        ahead = team.scan(mine, all) - mine;
     }
-    team.cl.sync();  // nobody leaves while its shared memory is read
+    walk(kept, ahead + earlier, mine, r, [&](int i) {
+        p.out[row] = i0 + i;
+        if (p.prob) p.prob[row] = (float)kept(i) / (float)total;
+    });
 }
 
 }  // namespace amcu
@@ -723,6 +862,7 @@ extern "C" am_status_code amcu_sample(const AmcuSampleArgs* a, void* stream) {
     p.logits = a->logits;
     p.stride = a->row_stride ? a->row_stride : a->vocab;
     p.vocab = a->vocab;
+    p.rows = a->rows;
     p.uniform = a->uniform;
     p.temperature = a->temperature;
     p.top_k = a->top_k;
@@ -735,6 +875,7 @@ extern "C" am_status_code amcu_sample(const AmcuSampleArgs* a, void* stream) {
     int c = 1;
     while (c < 16 && ceil_div(a->vocab, c) > kSampleSlice) c *= 2;
     while (c < 16 && a->rows * c * 2 <= num_sms() && ceil_div(a->vocab, 2 * c) >= 2048) c *= 2;
+    p.ahead = 2 * num_sms() / c;
     const int slice = (int)(ceil_div(a->vocab, 8 * c) * 8);  // the slices of an aligned row are aligned
     const bool res = slice <= kSampleSlice, f32 = a->dtype == AMCU_F32;
     AMCU_REQUIRE(a->rows * c <= INT32_MAX, "amcu_sample: too many rows");
