@@ -10,7 +10,10 @@
 //   O += P V    A = P (tensor memory), B = V^T, O in tensor memory
 // Warps 0-3 and 4-7 are the softmax of the two row tiles, warps 8-11 turn K's
 // codes into fp16 tiles and warps 12-15 V's, warp 16 issues the MMAs and owns the
-// tensor memory. While one row tile's softmax runs, the other's products do. (An
+// tensor memory. While one row tile's softmax runs, the other's products do, and
+// O's first 64 keys are added while the other 64 are weighed (353 against 363 us,
+// d = 64 280 against 288, 3 x 100 rows over 5000 keys of 28 / 4 heads 101 against
+// 106). (An
 // issuing warp for each row tile measured 469 against 432 us, the issuer as the
 // block's first warp 442, polling waits with a sleep 472: 2 x 2048 rows over 8192
 // keys, 32 / 8 heads of 128.)
@@ -53,6 +56,11 @@ struct PfLayout {  // shared memory, bytes
     static constexpr int kParV = kPfKeys / 8 * kVParPitch;
     static constexpr int oQ = 0, oK = oQ + 2 * kQ, oV = oK + 2 * kK, oRawV = oV + 2 * kK, oParV = oRawV + 2 * kRawV,
                          oBar = oParV + 2 * kParV;
+    // Registers from the dequantising warps to the softmax: 8 x kDqRegs + 8 x (192 -
+    // kDqRegs) + 96 = 17 x 96 a lane. As many as neither spills with (2 x 2048 rows
+    // over 8192 keys, 32 / 8 heads: 339 us of d = 128 with 80, 346 with 72; 278 us of
+    // d = 64 with 72, 289 with 80).
+    static constexpr int kDqRegs = D == 128 ? 80 : 72;
     static constexpr int kTotal = oBar + 256 + 1024;  // + alignment slack
 };
 
@@ -161,9 +169,9 @@ __global__ void __launch_bounds__(kPfThreads, 1) kv4_prefill_kernel(Kv4AttnParam
     uint8_t* sm = reinterpret_cast<uint8_t*>((reinterpret_cast<uintptr_t>(pf_raw) + 1023) & ~(uintptr_t)1023);
     uint64_t* bar = reinterpret_cast<uint64_t*>(sm + L::oBar);
     uint64_t *k_full = bar, *k_empty = bar + 2, *v_full = bar + 4, *v_empty = bar + 6, *s_full = bar + 8,
-             *p_full = bar + 10, *o_full = bar + 12, *q_full = bar + 14;
-    uint32_t* tmem_slot = reinterpret_cast<uint32_t*>(bar + 16);
-    int* s_item = reinterpret_cast<int*>(bar + 17);  // b, item of b
+             *p_full = bar + 10, *o_full = bar + 12, *q_full = bar + 14, *p_half = bar + 16, *o_half = bar + 18;
+    uint32_t* tmem_slot = reinterpret_cast<uint32_t*>(bar + 20);
+    int* s_item = reinterpret_cast<int*>(bar + 21);  // b, item of b
 
     const int warp = __shfl_sync(0xffffffffu, threadIdx.x >> 5, 0), lane = threadIdx.x & 31;
     pdl_wait();
@@ -197,6 +205,8 @@ __global__ void __launch_bounds__(kPfThreads, 1) kv4_prefill_kernel(Kv4AttnParam
                 mbar_init(&p_full[i], 4);
                 mbar_init(&o_full[i], 1);
                 mbar_init(&q_full[i], 4);
+                mbar_init(&p_half[i], 4);
+                mbar_init(&o_half[i], 1);
             }
             fence_mbar_init();
         }
@@ -265,18 +275,22 @@ __global__ void __launch_bounds__(kPfThreads, 1) kv4_prefill_kernel(Kv4AttnParam
                 wait(&v_full[j & 1], (j >> 1) & 1);
                 if (more) wait(&k_full[(j + 1) & 1], ((j + 1) >> 1) & 1);
                 for (int i = 0; i < ni_; ++i) {
+                    const uint64_t bb = v_desc + (uint64_t)((j & 1) * (L::kK >> 4));
+                    const uint32_t d = tmem + 256u + (uint32_t)(128 * i), a = tmem + (uint32_t)(128 * i);
+                    constexpr int kHalf = (D * 128) >> 4;  // of V^T: 64 keys
+                    // the first 64 keys' products run beside the weights of the others
+                    wait(&p_half[i], j & 1);
+                    tc_fence_after();
+#pragma unroll
+                    for (int s = 0; s < kPfKeys / 32; ++s)
+                        pf_mma_ts(d, a + (uint32_t)(8 * s), bb + (uint64_t)(s * 2), id_o, s != 0 || j != 0);
+                    pf_commit(&o_half[i]);
                     wait(&p_full[i], j & 1);
                     tc_fence_after();
-                    {
-                        const uint64_t bb = v_desc + (uint64_t)((j & 1) * (L::kK >> 4));
-                        const uint32_t d = tmem + 256u + (uint32_t)(128 * i), a = tmem + (uint32_t)(128 * i);
 #pragma unroll
-                        for (int s = 0; s < kPfKeys / 16; ++s) {
-                            constexpr int kHalf = (D * 128) >> 4;
-                            pf_mma_ts(d, a + (uint32_t)(8 * s), bb + (uint64_t)((s >> 2) * kHalf + (s & 3) * 2), id_o, s != 0 || j != 0);
-                        }
-                        if (more) qk(i, j + 1);
-                    }
+                    for (int s = kPfKeys / 32; s < kPfKeys / 16; ++s)
+                        pf_mma_ts(d, a + (uint32_t)(8 * s), bb + (uint64_t)(kHalf + (s & 3) * 2), id_o, 1);
+                    if (more) qk(i, j + 1);
                     pf_commit(more ? &s_full[i] : &o_full[i]);
                 }
                 pf_commit(&v_empty[j & 1]);
@@ -285,8 +299,7 @@ __global__ void __launch_bounds__(kPfThreads, 1) kv4_prefill_kernel(Kv4AttnParam
         }
         __syncwarp();
     } else if (warp >= 8) {
-        // registers from the dequantising warps to the softmax: 8 x 72 + 8 x 120 + 96 = 17 x 96 a lane
-        asm volatile("setmaxnreg.dec.sync.aligned.u32 72;");
+        asm volatile("setmaxnreg.dec.sync.aligned.u32 %0;" ::"n"(L::kDqRegs));
         const int t = threadIdx.x & 127;
         const int kmax = lim_last + 1;    // keys past it are zeros
         // pages of a tile's eight 16-key blocks, in lanes 0-7; fetched two tiles ahead
@@ -449,7 +462,7 @@ __global__ void __launch_bounds__(kPfThreads, 1) kv4_prefill_kernel(Kv4AttnParam
             asm volatile("cp.async.wait_group 0;" ::: "memory");
         }
     } else {
-        asm volatile("setmaxnreg.inc.sync.aligned.u32 120;");
+        asm volatile("setmaxnreg.inc.sync.aligned.u32 %0;" ::"n"(192 - L::kDqRegs));
         if (warp / 4 < ni) {
         // ---- softmax of row tile i: thread = row
         const int i = warp >> 2;
@@ -467,7 +480,7 @@ __global__ void __launch_bounds__(kPfThreads, 1) kv4_prefill_kernel(Kv4AttnParam
             uint8_t* Q = sm + L::oQ + i * L::kQ;
             const int c = lane % CPR;
             uint32_t eb_mine = 1;
-            constexpr int B = 8;  // loads in flight
+            constexpr int B = D == 128 ? 4 : 8;  // loads in flight
 #pragma unroll 1
             for (int st0 = 0; st0 < 32 / RPW; st0 += B) {
                 uint32_t w[B][4];
@@ -568,15 +581,20 @@ __global__ void __launch_bounds__(kPfThreads, 1) kv4_prefill_kernel(Kv4AttnParam
                     l3 = f2_fma(l3, f2_pack(corr, corr), f2_pack(0.f, 0.f));
                     const __half2 corr2 = __float2half2_rn(corr);
                     asm volatile("tcgen05.wait::st.sync.aligned;" ::: "memory");
-#pragma unroll 1
-                    for (int k = 0; k < q; ++k) {  // P of this tile's earlier columns
+                    if (q & 1) {  // this half's P so far: no product has taken it
                         uint32_t y[16];
-                        tc_ld16(ts + 16 * k, y);
+                        tc_ld16(ts + 16 * (q - 1), y);
 #pragma unroll
                         for (int c = 0; c < 16; ++c) y[c] = pf_h2u(__hmul2(pf_u2h(y[c]), corr2));
-                        tc_st_32x32b_x16(ts + 16 * k, y);
+                        tc_st_32x32b_x16(ts + 16 * (q - 1), y);
                     }
-                    if (j > 0) {  // products of earlier tiles are complete: this tile's scores were committed after them
+                    // products of earlier tiles are complete (this tile's scores were
+                    // committed after them), those of its first half have to be waited for
+                    if (q >= 2) {
+                        wait(&o_half[i], j & 1);
+                        tc_fence_after();
+                    }
+                    if (j > 0 || q >= 2) {
 #pragma unroll 1
                         for (int k = 0; k < D / 16; ++k) {
                             uint32_t y[16];
@@ -603,11 +621,13 @@ __global__ void __launch_bounds__(kPfThreads, 1) kv4_prefill_kernel(Kv4AttnParam
                 }
                 // columns 16 q .. + 15 hold scores that are in registers by now
                 tc_st_32x32b_x16_nowait(ts + 16 * q, pk16);
+                if (q & 1) {
+                    asm volatile("tcgen05.wait::st.sync.aligned;" ::: "memory");
+                    tc_fence_before();
+                    __syncwarp();
+                    if (lane == 0) mbar_arrive(q == 1 ? &p_half[i] : &p_full[i]);
+                }
             }
-            asm volatile("tcgen05.wait::st.sync.aligned;" ::: "memory");
-            tc_fence_before();
-            __syncwarp();
-            if (lane == 0) mbar_arrive(&p_full[i]);
         }
         // ---- out = O / l
         float la, lb;
