@@ -2,6 +2,8 @@
 //
 // out[row, h] = sum_j p_j v_j / sum_j p_j, p_j = exp(scale q . k_j - max), over
 // the positions j <= pos of the row's sequence; k_j = m + s * code.
+#include <algorithm>
+
 #include "kv4.cuh"
 #include "mma_int4.cuh"
 
@@ -41,7 +43,10 @@ constexpr int kDecWarps = 8;
 constexpr int kDecThreads = kDecWarps * 32;
 constexpr int kDecStages = 4;  // 64 ragged rows: 103.7 us, 105.0 with 5, 106.0 with 6
 constexpr int kDecUnit = 16;       // keys per unit
-constexpr int kDecMinUnits = 8;    // units of a CTA at least: one for each warp
+// Units of a CTA at least: one for each warp, or what an item has on average where
+// that is less (an item costs a CTA 2 to 5 us whatever its length: one row over 7
+// keys, 8 kv heads of 64, 21.5 us with all items in one CTA, 5.5 with one in each).
+constexpr int kDecMinUnits = 8;
 constexpr float kLog2e = 1.4426950408889634f;
 constexpr float kDecLift = 3.f;    // p stays below 2^3 before its reference moves
 
@@ -63,6 +68,7 @@ struct DecWork {
     float2* ml;    // [CTA][2][8] (reference, denominator)
     float* o;      // [CTA][2][8][D]
     DecMeta* meta; // [CTA]
+    int64_t items; // (sequence, kv head, column tile) triples of the call, at most
 };
 
 __device__ __forceinline__ void cp16(uint32_t dst, const void* src, uint32_t bytes) {
@@ -143,7 +149,7 @@ __global__ void __launch_bounds__(kDecThreads, 2) kv4_decode_kernel(Kv4AttnParam
         const bool have = kv4_share<kDecThreads>(
                 v.n_seq,
                 [&](int64_t all) {
-                    share = max((all + gridDim.x - 1) / gridDim.x, (int64_t)kDecMinUnits);
+                    share = max((all + gridDim.x - 1) / gridDim.x, min((all + ws.items - 1) / ws.items, (int64_t)kDecMinUnits));
                     return x = blockIdx.x * share;
                 },
                 cost_of, total, b, off);
@@ -661,12 +667,16 @@ using namespace amcu;
 
 namespace {
 
-// CTAs of a call: two to an SM, fewer where the page table cannot hold that many units.
-int64_t dec_ctas(const AmcuKv4AttentionArgs* a) {
+int64_t dec_items(const AmcuKv4AttentionArgs* a) {
     const int64_t cols = a->dtype == AMCU_F32 ? dec_cols<float>() : dec_cols<__nv_bfloat16>();
     const int64_t tiles = ceil_div(a->batch.rows * (a->n_q_heads / a->cache.n_kv_heads), cols) + a->batch.n_seq;
+    return tiles * a->cache.n_kv_heads;
+}
+
+// CTAs of a call: two to an SM, fewer where the page table cannot hold that many units.
+int64_t dec_ctas(const AmcuKv4AttentionArgs* a) {
     const int64_t units = ceil_div(a->batch.max_pages * a->cache.page_size, kDecUnit);
-    const double bound = (double)tiles * (double)a->cache.n_kv_heads * (double)(units > 0 ? units : 1) / kDecMinUnits;
+    const double bound = (double)dec_items(a) * std::max(1.0, (double)units / kDecMinUnits);
     const int64_t most = 2 * num_sms();
     return bound >= (double)most ? most : (int64_t)bound + 1;
 }
@@ -728,6 +738,7 @@ extern "C" am_status_code amcu_attn_kv4(const AmcuKv4AttentionArgs* a, void* str
     DecWork w;
     const unsigned ctas = (unsigned)dec_ctas(a);
     dec_layout(ctas, a->cache.head_dim, static_cast<uint8_t*>(a->workspace), &w);
+    w.items = dec_items(a);
     const bool f32 = a->dtype == AMCU_F32;
     cudaStream_t s = as_stream(stream);
     if (prompts) return kv4_prefill_launch(p, a->cache.head_dim, s);
