@@ -47,6 +47,12 @@ constexpr int kDecUnit = 16;       // keys per unit
 // that is less (an item costs a CTA 2 to 5 us whatever its length: one row over 7
 // keys, 8 kv heads of 64, 21.5 us with all items in one CTA, 5.5 with one in each).
 constexpr int kDecMinUnits = 8;
+// A warp takes whole items by itself, without the CTA's merge, where a CTA would
+// have kDecMany or more of them and none is longer than kDecLong units for each of
+// those (a single long one would keep the others waiting). Sequences of one row,
+// 32 / 8 heads of 128, us so / by CTAs: 64 of 20 keys 11 / 20, 128 of 100 17 / 42, 128
+// of 250 24 / 46, 256 of 100 22 / 61, 256 of 300 39 / 81, 256 of 600 60 / 88.
+constexpr int kDecMany = 2, kDecLong = 8;
 constexpr float kLog2e = 1.4426950408889634f;
 constexpr float kDecLift = 3.f;    // p stays below 2^3 before its reference moves
 
@@ -138,18 +144,24 @@ __global__ void __launch_bounds__(kDecThreads, 2) kv4_decode_kernel(Kv4AttnParam
 
     // ---- this CTA's share [x, x_end) of all units
     const Kv4View& v = p.v;
+    int most = 0;  // units of an item
     auto cost_of = [&](int i) {
         const DecSeq q = dec_seq<T>(v, p.grp, i);
+        if (q.tiles) most = max(most, q.units);
         return (int64_t)q.units * q.tiles * v.nkv;
     };
     int64_t total, share, x;
+    bool alone = false;  // a warp to an item
     {
         int b;
         int64_t off;
         const bool have = kv4_share<kDecThreads>(
                 v.n_seq,
                 [&](int64_t all) {
-                    share = max((all + gridDim.x - 1) / gridDim.x, min((all + ws.items - 1) / ws.items, (int64_t)kDecMinUnits));
+                    const int64_t many = ws.items / gridDim.x;
+                    alone = many >= kDecMany && !__syncthreads_or(most > kDecLong * many);
+                    share = alone ? (all + gridDim.x * kDecWarps - 1) / (gridDim.x * kDecWarps) * kDecWarps
+                                  : max((all + gridDim.x - 1) / gridDim.x, min((all + ws.items - 1) / ws.items, (int64_t)kDecMinUnits));
                     return x = blockIdx.x * share;
                 },
                 cost_of, total, b, off);
@@ -158,12 +170,19 @@ __global__ void __launch_bounds__(kDecThreads, 2) kv4_decode_kernel(Kv4AttnParam
             s_off = off;
         }
     }
-    const int64_t x_end = min(x + share, total);
+    int64_t x_end = min(x + share, total);
     if (threadIdx.x == 0) ws.meta[blockIdx.x].first = -1;
     if (x >= x_end) return;
     __syncthreads();
     int b = s_b;
     int64_t off = s_off;
+    // unit k of this warp's part of a segment is its first + w0 + (k << w_shift)
+    const int w0 = alone ? 0 : warp, w_shift = alone ? 0 : 3;
+    if (alone) {  // the items that begin in this warp's part of the share
+        x += warp * (share / kDecWarps);
+        off += warp * (share / kDecWarps);
+        x_end = min(x + share / kDecWarps, total);
+    }
     const uint32_t ring = smem_u32(smem) + warp * (S * kStage);
     const uint8_t* ring_p = smem + warp * (S * kStage);
     const int page_units_shift = v.page_shift - 4;
@@ -177,8 +196,13 @@ __global__ void __launch_bounds__(kDecThreads, 2) kv4_decode_kernel(Kv4AttnParam
             continue;
         }
         const int item = (int)(off / sq.units), u0 = (int)(off - (int64_t)item * sq.units);
+        if (alone && u0 > 0) {
+            x += sq.units - u0;
+            off += sq.units - u0;
+            continue;
+        }
         const int kvh = item / sq.tiles, ct = item - kvh * sq.tiles;
-        const int u1 = (int)min((int64_t)sq.units, u0 + (x_end - x));
+        const int u1 = alone ? sq.units : (int)min((int64_t)sq.units, u0 + (x_end - x));
         const int cap = (int)min((int64_t)max(sq.ctx, 0), (int64_t)v.max_pages << v.page_shift);  // keys that can exist
         const int cols = min(CT, sq.n * p.grp - ct * CT);
         if (sq.ctx > cap && v.status && threadIdx.x == 0) *v.status = (int32_t)AM_STATUS_OUT_OF_RANGE;
@@ -201,8 +225,8 @@ __global__ void __launch_bounds__(kDecThreads, 2) kv4_decode_kernel(Kv4AttnParam
         const int u_end = min(u1, (lim_last + kDecUnit) / kDecUnit);  // lim_last = -1: none
         const int full = (lim_first + 1) / kDecUnit;  // units before it need no mask
 
-        // ---- ring: unit k of this warp is u0 + warp + 8 k
-        const int nk = u_end > u0 + warp ? (u_end - u0 - warp + kDecWarps - 1) / kDecWarps : 0;
+        // ---- ring
+        const int u_first = u0 + w0, nk = u_end > u_first ? (u_end - u_first - 1 >> w_shift) + 1 : 0;
         int pages = -1;
         bool holes = false;   // a page that is none was met
         const int64_t head_c = ((int64_t)kvh << v.page_shift) * (D / 2), head_p = ((int64_t)kvh << v.page_shift) * (D / 16);
@@ -216,13 +240,13 @@ __global__ void __launch_bounds__(kDecThreads, 2) kv4_decode_kernel(Kv4AttnParam
         auto fetch = [&](int k) {
             if (k < nk) {
                 if ((k & 31) == 0) {  // page ids of the next 32 units, one per lane
-                    const int u = u0 + warp + kDecWarps * (k + lane);
+                    const int u = u_first + ((k + lane) << w_shift);
                     pages = u < u_end ? kv4_page(v, b, u * kDecUnit) : 0;
                     holes |= __any_sync(0xffffffffu, pages < 0);
                 }
                 const int page = __shfl_sync(0xffffffffu, pages, k & 31);
                 const uint32_t st = (uint32_t)(k % S) * kStage, ok = page >= 0 ? 16u : 0u, pg = page >= 0 ? page : 0;
-                const uint32_t slot = (uint32_t)(u0 + warp + kDecWarps * k) & slot_mask;
+                const uint32_t slot = (uint32_t)(u_first + (k << w_shift)) & slot_mask;
                 const uint64_t co = pg * (uint64_t)(uint32_t)v.cps + slot * kCodes;  // pages are below 4 GB
 #pragma unroll
                 for (int i = 0; i < kCodes / 512; ++i) {  // 512 bytes are whole swizzled lines
@@ -299,7 +323,7 @@ __global__ void __launch_bounds__(kDecThreads, 2) kv4_decode_kernel(Kv4AttnParam
             __syncwarp();
             fetch(k + S - 1);
             const uint8_t* st = ring_p + (k % S) * kStage;
-            const int u = u0 + warp + kDecWarps * k;
+            const int u = u_first + (k << w_shift);
             const uint8_t* kpar = st + 2 * kCodes;
             const uint8_t* vpar = kpar + kParams;
 
@@ -534,9 +558,10 @@ __global__ void __launch_bounds__(kDecThreads, 2) kv4_decode_kernel(Kv4AttnParam
         asm volatile("cp.async.wait_group 0;" ::: "memory");
 
         // ---- the warps' sums together: [warp][column][D] and (reference, denominator, minima)
-        __syncthreads();  // the rings are read out
-        float* mo = reinterpret_cast<float*>(smem);
-        float* mx = mo + kDecWarps * 8 * kMS;  // [warp][column][4]
+        if (alone) __syncwarp();
+        else __syncthreads();  // the rings are read out
+        float* mo = reinterpret_cast<float*>(alone ? smem + warp * (S * kStage) : smem);
+        float* mx = mo + (alone ? 1 : kDecWarps) * 8 * kMS;  // [warp][column][4]
         // low nibbles are in units of 2^-24, high ones of 2^-20 (fp32: of 1), both times lift
         const float unlift = nk > 0 ? 1.f / lift : 0.f;
         const float lo_unit = (kWide ? 1.f : 16777216.f) * unlift, hi_unit = (kWide ? 1.f : 1048576.f) * unlift;
@@ -553,14 +578,30 @@ __global__ void __launch_bounds__(kDecThreads, 2) kv4_decode_kernel(Kv4AttnParam
 #pragma unroll
         for (int j = 0; j < (kWide ? 1 : 2); ++j) {
             const int col = kWide ? t : 2 * t + j;
-            float* dst = mo + (warp * 8 + col) * kMS;
+            float* dst = mo + (w0 * 8 + col) * kMS;
 #pragma unroll
             for (int g = 0; g < G; ++g)
 #pragma unroll
                 for (int i = 0; i < 4; ++i)
                     *reinterpret_cast<float2*>(dst + g * kKv4Group + 8 * r + 2 * i) = make_float2(o[g][i][j] * lo_unit, o[g][i][2 + j] * hi_unit);
-            if (r <= G) mx[(warp * 8 + col) * 4 + (r == G ? 1 : 2 + r)] = xa[j];
-            if (r == 0) mx[(warp * 8 + col) * 4] = ref[j];
+            if (r <= G) mx[(w0 * 8 + col) * 4 + (r == G ? 1 : 2 + r)] = xa[j];
+            if (r == 0) mx[(w0 * 8 + col) * 4] = ref[j];
+        }
+        auto put = [&](int col, int d, float val, float l) {
+            const int fcol = ct * CT + col, rw = fcol / p.grp, hd = kvh * p.grp + fcol - rw * p.grp;
+            static_cast<T*>(p.out)[(int64_t)(sq.row0 + rw) * p.os + (int64_t)hd * D + d] = Act<T>::store(l > 0.f ? val / l : 0.f);
+        };
+        if (alone) {
+            __syncwarp();
+            for (int e = lane; e < cols * D; e += 32) {
+                const int col = e / D, d = e % D;
+                const float4 y = *reinterpret_cast<const float4*>(mx + col * 4);
+                put(col, d, mo[col * kMS + d] + (d < kKv4Group ? y.z : y.w), y.y);
+            }
+            __syncwarp();
+            x += sq.units;
+            off += sq.units;
+            continue;
         }
         __syncthreads();
         const bool whole = u0 == 0 && u1 == sq.units;
@@ -581,9 +622,7 @@ __global__ void __launch_bounds__(kDecThreads, 2) kv4_decode_kernel(Kv4AttnParam
                 val = fmaf(fw, mo[(w * 8 + col) * kMS + d] + (d < kKv4Group ? y.z : y.w), val);
             }
             if (whole) {
-                const int fcol = ct * CT + col, rw = fcol / p.grp, hd = kvh * p.grp + fcol - rw * p.grp;
-                static_cast<T*>(p.out)[(int64_t)(sq.row0 + rw) * p.os + (int64_t)hd * D + d] =
-                        Act<T>::store(l > 0.f ? val / l : 0.f);
+                put(col, d, val, l);
             } else {
                 ws.o[((int64_t)slot * 8 + col) * D + d] = val;
                 if (d == 0) ws.ml[slot * 8 + col] = make_float2(m, l);
