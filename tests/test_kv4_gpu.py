@@ -381,6 +381,64 @@ def test_attention_many_sequences(ops):
     check_attention(got, want, torch.bfloat16, 4.0)
 
 
+@pytest.mark.parametrize("dtype", [torch.bfloat16, torch.float32])
+@pytest.mark.parametrize("n,longest,nq,nkv,d,page", [
+    (120, 380, 32, 8, 128, 16),   # each warp takes whole items
+    (120, 384, 32, 8, 128, 64),
+    (120, 2000, 32, 8, 128, 64),  # a long one among them: shares of all units
+    (700, 60, 12, 1, 64, 32),
+    (90, 33, 20, 10, 64, 16),
+])
+def test_attention_many_short_sequences(ops, n, longest, nq, nkv, d, page, dtype):
+    rng = np.random.default_rng(n + longest + d)
+    lens = [(int(c), int(min(c, r))) for c, r in zip(rng.integers(0, min(longest, 380) + 1, n), rng.integers(0, 4, n))]
+    lens[n // 3] = (longest, 1)
+    lens[-1] = (longest, 2)
+    lens[0] = (1, 1)
+    table, start, ctx, total = make_batch(lens, page, rng)
+    cache = random_cache(total, nkv, page, d, rng)
+    poison_unused(cache, table, ctx)
+    q = torch.from_numpy(rng.normal(0, 1.5, (start[-1], nq * d)).astype(np.float32)).to(dtype)
+    want = ref.attention(q.double().numpy(), cache, table, start, ctx, nq, nkv, d)
+    out = torch.full((start[-1], nq * d), float("nan"), dtype=dtype, device="cuda")
+    got = ops.attention_kv4(q.cuda(), dev(cache), di(table), di(start), di(ctx), nq, nkv, d, out=out)
+    check_attention(got, want, dtype, 4.0)
+    assert torch.equal(got, ops.attention_kv4(q.cuda(), dev(cache), di(table), di(start), di(ctx), nq, nkv, d))
+
+
+def test_attention_many_short_sequences_missing_pages(ops):
+    rng = np.random.default_rng(19)
+    lens = [(int(c), 1) for c in rng.integers(1, 129, 150)]
+    lens[7] = (2, 5)  # a context below its rows
+    table, start, ctx, total = make_batch(lens, 16, rng, pages=8)
+    cache = random_cache(total, 8, 16, 64, rng)
+    table[3, 0], table[20, :] = -1, total + 5  # the first page of one, all of another
+    ctx[50] = 8 * 16 + 9  # past the page table
+    table[50] = table[51]
+    q = bf16(rng.normal(0, 1, (start[-1], 32 * 64)))
+    want = ref.attention(q.double().numpy(), cache, table, start, ctx, 32, 8, 64)
+    status = torch.zeros(1, dtype=torch.int32, device="cuda")
+    got = ops.attention_kv4(q.cuda(), dev(cache), di(table), di(start), di(ctx), 32, 8, 64, status=status)
+    check_attention(got, want, torch.bfloat16, 4.0)
+    assert status.item() == 11  # OUT_OF_RANGE
+    assert (got[start[20]] == 0).all() and (got[start[7]: start[7] + 3] == 0).all()
+
+
+@pytest.mark.parametrize("dtype", [torch.bfloat16, torch.float32])
+@pytest.mark.parametrize("ctx,rows", [(1, 1), (7, 2), (20, 1), (120, 3)])
+@pytest.mark.parametrize("nq,nkv,d", [(32, 8, 128), (56, 8, 64), (16, 16, 64)])
+def test_attention_few_keys(ops, ctx, rows, nq, nkv, d, dtype):
+    """Items of fewer units than a CTA has warps."""
+    rng = np.random.default_rng(ctx * 10 + rows + nq)
+    table, start, lens, total = make_batch([(ctx, rows)], 16, rng)
+    cache = random_cache(total, nkv, 16, d, rng)
+    poison_unused(cache, table, lens)
+    q = torch.from_numpy(rng.normal(0, 1.5, (rows, nq * d)).astype(np.float32)).to(dtype)
+    want = ref.attention(q.double().numpy(), cache, table, start, lens, nq, nkv, d)
+    got = ops.attention_kv4(q.cuda(), dev(cache), di(table), di(start), di(lens), nq, nkv, d)
+    check_attention(got, want, dtype, 4.0)
+
+
 # ------------------------------------------------------------------ append and gather
 APPEND = [
     # lens (ctx, rows), nq, nkv, d, page
