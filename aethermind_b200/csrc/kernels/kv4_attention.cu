@@ -205,7 +205,8 @@ __global__ void __launch_bounds__(kDecThreads, 2) kv4_decode_kernel(Kv4AttnParam
         const int u1 = alone ? sq.units : (int)min((int64_t)sq.units, u0 + (x_end - x));
         const int cap = (int)min((int64_t)max(sq.ctx, 0), (int64_t)v.max_pages << v.page_shift);  // keys that can exist
         const int cols = min(CT, sq.n * p.grp - ct * CT);
-        if (sq.ctx > cap && v.status && lane == 0) *v.status = (int32_t)AM_STATUS_OUT_OF_RANGE;  // alone: only this warp sees it
+        // keys past the page table, or rows before position 0 (alone: no other warp meets the item)
+        if ((sq.ctx > cap || sq.ctx < sq.n) && v.status && lane == 0) *v.status = (int32_t)AM_STATUS_OUT_OF_RANGE;
 
         // ---- the tile's columns: this lane's is r (MMA operand), its results are of columns 2t, 2t + 1
         const int c_op = kWide ? r >> 1 : r;

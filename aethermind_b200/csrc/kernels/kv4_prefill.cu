@@ -230,7 +230,7 @@ __global__ void __launch_bounds__(kPfThreads, 1) kv4_prefill_kernel(Kv4AttnParam
     const int lim_last = min(ctx - n + (m_end - 1) / p.grp, cap - 1);     // last key that any row sees
     const int nt = lim_last >= 0 ? lim_last / kPfKeys + 1 : 0;            // key tiles
     const int ni = m_end - m0 > 128 ? 2 : 1;                              // row tiles
-    if (ctx > cap && v.status && threadIdx.x == 0) *v.status = (int32_t)AM_STATUS_OUT_OF_RANGE;
+    if ((ctx > cap || ctx < n) && v.status && threadIdx.x == 0) *v.status = (int32_t)AM_STATUS_OUT_OF_RANGE;
 
     const uint32_t tmem = __shfl_sync(0xffffffffu, *tmem_slot, 0);
     bool ok = true;

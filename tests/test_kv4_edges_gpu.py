@@ -46,3 +46,23 @@ def test_attention_reports_a_context_past_the_page_table(ops, n, keys, nq, nkv, 
         if status.item() != (0 if at is None else OUT_OF_RANGE):
             wrong.append(at)
     assert not wrong
+
+
+@pytest.mark.parametrize("lens,nq,nkv,d", [
+    ([(2, 3)], 8, 2, 64),
+    ([(300, 1), (2, 3)], 8, 2, 64),
+    ([(20, 1)] * 150 + [(2, 3)] + [(20, 1)] * 30, 32, 8, 64),
+    ([(300, 160), (20, 21)], 32, 8, 128),  # the kernel of prompts
+    ([(0, 160)], 32, 8, 64),
+])
+@pytest.mark.parametrize("short", [True, False])
+def test_attention_reports_rows_before_position_0(ops, lens, nq, nkv, d, short):
+    """A context below its rows is reported, as kv4_append does; as many keys as rows are not."""
+    rng = np.random.default_rng(2)
+    lens = lens if short else [(max(c, n), n) for c, n in lens]
+    table, start, ctx, total = make_batch(lens, 16, rng)
+    cache = dev(random_cache(total, nkv, 16, d, rng))
+    q = bf16(rng.normal(0, 1, (start[-1], nq * d))).cuda()
+    status = i32([0])
+    ops.attention_kv4(q, cache, di(table), di(start), di(ctx), nq, nkv, d, status=status)
+    assert status.item() == (OUT_OF_RANGE if short else 0)
