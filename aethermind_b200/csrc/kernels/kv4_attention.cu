@@ -264,22 +264,24 @@ __global__ void __launch_bounds__(kDecThreads, 2) kv4_decode_kernel(Kv4AttnParam
 #pragma unroll
         for (int k = 0; k < S - 1; ++k) fetch(k);
 
-        float amax = 0.f, qsum[G];
+        uint32_t amax = 0;  // bits of the largest |q|: NaN above infinity above the rest
+        float qsum[G];
 #pragma unroll
         for (int g = 0; g < G; ++g) {
             qsum[g] = 0.f;
 #pragma unroll
             for (int i = 0; i < 16; ++i) {
-                amax = fmaxf(amax, fabsf(qv[g][i]));
+                amax = max(amax, __float_as_uint(qv[g][i]) & 0x7fffffffu);
                 qsum[g] += qv[g][i];
             }
             qsum[g] += __shfl_xor_sync(0xffffffffu, qsum[g], 1);
             qsum[g] += __shfl_xor_sync(0xffffffffu, qsum[g], 2);
         }
-        amax = fmaxf(amax, __shfl_xor_sync(0xffffffffu, amax, 1));
-        amax = fmaxf(amax, __shfl_xor_sync(0xffffffffu, amax, 2));
-        const uint32_t eb = min(max(__float_as_uint(amax) >> 23, 1u), 253u);
-        const float inv = __uint_as_float((254u - eb) << 23);
+        amax = max(amax, __shfl_xor_sync(0xffffffffu, amax, 1));
+        amax = max(amax, __shfl_xor_sync(0xffffffffu, amax, 2));
+        const uint32_t eb = min(max(amax >> 23, 1u), 253u);
+        // a row with an element that is no number or infinite has no softmax: all its scores are NaN
+        const float inv = __uint_as_float(amax < 0x7f800000u ? (254u - eb) << 23 : 0x7fc00000u);
         uint32_t qf[2 * G][2][2];  // [word][half of the word][b0, b1]
 #pragma unroll
         for (int j = 0; j < 2 * G; ++j)
@@ -590,7 +592,7 @@ __global__ void __launch_bounds__(kDecThreads, 2) kv4_decode_kernel(Kv4AttnParam
         }
         auto put = [&](int col, int d, float val, float l) {
             const int fcol = ct * CT + col, rw = fcol / p.grp, hd = kvh * p.grp + fcol - rw * p.grp;
-            static_cast<T*>(p.out)[(int64_t)(sq.row0 + rw) * p.os + (int64_t)hd * D + d] = Act<T>::store(l > 0.f ? val / l : 0.f);
+            static_cast<T*>(p.out)[(int64_t)(sq.row0 + rw) * p.os + (int64_t)hd * D + d] = Act<T>::store(l == 0.f ? 0.f : val / l);  // 0: no key; NaN stays
         };
         if (alone) {
             __syncwarp();
@@ -698,7 +700,7 @@ __global__ void __launch_bounds__(kCombineWarps * 32) kv4_combine_kernel(Kv4Attn
         vs = fmaf(fw, so[w][d], vs);
     }
     const int fcol = me.col0 + col, rw = fcol / p.grp, hd = me.head0 + fcol - rw * p.grp;
-    static_cast<T*>(p.out)[(int64_t)(me.row0 + rw) * p.os + (int64_t)hd * D + d] = Act<T>::store(ls > 0.f ? vs / ls : 0.f);
+    static_cast<T*>(p.out)[(int64_t)(me.row0 + rw) * p.os + (int64_t)hd * D + d] = Act<T>::store(ls == 0.f ? 0.f : vs / ls);
 }
 
 }  // namespace amcu

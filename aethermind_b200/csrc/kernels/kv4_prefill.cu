@@ -502,17 +502,19 @@ __global__ void __launch_bounds__(kPfThreads, 1) kv4_prefill_kernel(Kv4AttnParam
                 }
 #pragma unroll
                 for (int u = 0; u < B; ++u) {
-                    float e[8], amax = 0.f;
+                    float e[8];
+                    uint32_t amax = 0;  // bits of the largest |q|: NaN above infinity above the rest
 #pragma unroll
                     for (int k = 0; k < 4; ++k) {
                         e[2 * k] = __uint_as_float(w[u][k] << 16);
                         e[2 * k + 1] = __uint_as_float(w[u][k] & 0xffff0000u);
-                        amax = fmaxf(amax, fmaxf(fabsf(e[2 * k]), fabsf(e[2 * k + 1])));
+                        amax = max(amax, max(__float_as_uint(e[2 * k]) & 0x7fffffffu, __float_as_uint(e[2 * k + 1]) & 0x7fffffffu));
                     }
 #pragma unroll
-                    for (int o = CPR / 2; o > 0; o >>= 1) amax = fmaxf(amax, __shfl_xor_sync(0xffffffffu, amax, o));
-                    const uint32_t eb = min(max(__float_as_uint(amax) >> 23, 1u), 253u);
-                    const float inv = __uint_as_float((254u - eb) << 23);
+                    for (int o = CPR / 2; o > 0; o >>= 1) amax = max(amax, __shfl_xor_sync(0xffffffffu, amax, o));
+                    const uint32_t eb = min(max(amax >> 23, 1u), 253u);
+                    // a row with an element that is no number or infinite has no softmax: all its scores are NaN
+                    const float inv = __uint_as_float(amax < 0x7f800000u ? (254u - eb) << 23 : 0x7fc00000u);
 #pragma unroll
                     for (int k = 0; k < 8; ++k) e[k] *= inv;
                     // in the order 0 4 1 5 2 6 3 7
@@ -632,7 +634,8 @@ __global__ void __launch_bounds__(kPfThreads, 1) kv4_prefill_kernel(Kv4AttnParam
         // ---- out = O / l
         float la, lb;
         f2_unpack(f2_add(l2, l3), la, lb);
-        const float l = la + lb, inv = l > 0.f ? 1.f / l : 0.f;
+        const float l = la + lb, inv = 1.f / l;
+        const bool any = nt > 0 && l != 0.f;  // a key was seen; NaN stays
         if (nt > 0) {
             wait(&o_full[i], 0);
             tc_fence_after();
@@ -648,8 +651,8 @@ __global__ void __launch_bounds__(kPfThreads, 1) kv4_prefill_kernel(Kv4AttnParam
             uint32_t y[16];
 #pragma unroll
             for (int c = 0; c < 16; ++c) {
-                const float a = nt > 0 && l > 0.f ? __uint_as_float(x[2 * c]) * inv : 0.f;
-                const float bb = nt > 0 && l > 0.f ? __uint_as_float(x[2 * c + 1]) * inv : 0.f;
+                const float a = any ? __uint_as_float(x[2 * c]) * inv : 0.f;
+                const float bb = any ? __uint_as_float(x[2 * c + 1]) * inv : 0.f;
                 __nv_bfloat162 h = __floats2bfloat162_rn(a, bb);
                 y[c] = *reinterpret_cast<uint32_t*>(&h);
             }

@@ -6,7 +6,7 @@ import pytest
 torch = pytest.importorskip("torch")
 
 import kv4_reference as ref  # noqa: E402
-from test_kv4_gpu import bf16, dev, di, make_batch, random_cache  # noqa: E402
+from test_kv4_gpu import bf16, check_attention, dev, di, make_batch, poison_unused, random_cache  # noqa: E402
 
 pytestmark = pytest.mark.gpu
 
@@ -66,3 +66,38 @@ def test_attention_reports_rows_before_position_0(ops, lens, nq, nkv, d, short):
     status = i32([0])
     ops.attention_kv4(q, cache, di(table), di(start), di(ctx), nq, nkv, d, status=status)
     assert status.item() == (OUT_OF_RANGE if short else 0)
+
+
+# ------------------------------------------------------------------ numbers that are none
+@pytest.mark.parametrize("dtype", [torch.bfloat16, torch.float32])
+@pytest.mark.parametrize("bad", [float("nan"), float("inf"), -float("inf")])
+@pytest.mark.parametrize("lens,nq,nkv,d", [
+    ([(5, 1), (40, 3)], 8, 2, 128),
+    ([(9000, 2)], 8, 2, 64),               # items cut between CTAs
+    ([(30, 1)] * 160, 32, 8, 128),         # each warp takes whole items
+    ([(20, 21), (300, 160)], 32, 8, 128),  # bf16: the kernel of prompts; the first row sees no key
+    ([(400, 190)], 32, 8, 64),
+])
+def test_attention_of_a_q_that_is_no_number(ops, lens, nq, nkv, d, bad, dtype):
+    """The row's head is NaN where it sees a key, 0 where it sees none; every other head is as it would be."""
+    rng = np.random.default_rng(3)
+    table, start, ctx, total = make_batch(lens, 16, rng)
+    cache = random_cache(total, nkv, 16, d, rng)
+    cache[1][..., 1] = 0.25  # all keys above zero: an infinite element gives scores of one sign
+    poison_unused(cache, table, ctx)
+    rows = start[-1]
+    q = torch.from_numpy(rng.normal(0, 1.5, (rows, nq * d)).astype(np.float32)).to(dtype)
+    want = ref.attention(q.double().numpy(), cache, table, start, ctx, nq, nkv, d)
+    hit = [(0, 1, 3), (rows - 1, nq - 1, d - 1), (rows // 2, 2, d // 2)]
+    for r, h, e in hit:
+        q[r, h * d + e] = bad
+    got = ops.attention_kv4(q.cuda(), dev(cache), di(table), di(start), di(ctx), nq, nkv, d)
+    b = np.repeat(np.arange(len(lens)), np.diff(start))
+    for r, h, _ in hit:
+        part = got[r, h * d:(h + 1) * d]
+        if ctx[b[r]] - start[b[r] + 1] + r >= 0:
+            assert torch.isnan(part).all(), (r, h)
+        else:
+            assert (part == 0).all(), (r, h)
+        part.copy_(torch.from_numpy(want[r, h * d:(h + 1) * d]))
+    check_attention(got, want, dtype, 4.0)
