@@ -146,6 +146,15 @@ __device__ __forceinline__ uint32_t kv4_codes(const float (&x)[4], float s, floa
     return r;
 }
 
+// Minimum and scale of a group. lo is NaN where every element is: such a group
+// stays NaN (m = NaN, s = 0), so that it shows in every row that sees it.
+__device__ __forceinline__ __half kv4_min(float lo) {
+    return __float2half_rn(lo != lo ? lo : fminf(fmaxf(lo, -kHalfMax), kHalfMax));
+}
+__device__ __forceinline__ __half kv4_step(float lo, float hi) {
+    return __float2half_rn(lo != lo ? 0.f : fminf(__fmul_rn(__fsub_rn(hi, lo), 1.f / 15.f), kKv4StepMax));
+}
+
 // A warp takes U times 32 / LPH heads of one row (q heads, then k, then v). A
 // lane holds elements 4l .. 4l + 3 of each half of its head: both members of
 // four rotation pairs, and half a word of codes of each half.
@@ -290,10 +299,7 @@ __global__ void __launch_bounds__(128) kv4_append_kernel(Kv4AppendParams p) {
             lo1 = lo0;
             hi1 = hi0;
         }
-        const __half m0 = __float2half_rn(fminf(fmaxf(lo0, -kHalfMax), kHalfMax));
-        const __half m1 = __float2half_rn(fminf(fmaxf(lo1, -kHalfMax), kHalfMax));
-        const __half s0 = __float2half_rn(fminf(__fmul_rn(__fsub_rn(hi0, lo0), 1.f / 15.f), kKv4StepMax));
-        const __half s1 = __float2half_rn(fminf(__fmul_rn(__fsub_rn(hi1, lo1), 1.f / 15.f), kKv4StepMax));
+        const __half m0 = kv4_min(lo0), m1 = kv4_min(lo1), s0 = kv4_step(lo0, hi0), s1 = kv4_step(lo1, hi1);
         const float f0 = __half2float(s0), f1 = __half2float(s1);
         const float i0 = f0 > 0.f ? __fdividef(1.f, f0) : 0.f, i1 = D == 64 ? i0 : f1 > 0.f ? __fdividef(1.f, f1) : 0.f;
         const uint32_t h0 = kv4_codes(x, f0, __half2float(m0), i0), h1 = kv4_codes(y, f1, __half2float(m1), i1);

@@ -415,6 +415,32 @@ __global__ void __launch_bounds__(kDecThreads, 2) kv4_decode_kernel(Kv4AttnParam
                         vm[hh][g] &= keep;
                     }
                 }
+                // A group of V that is NaN (its minimum is) may be of a key that only some columns
+                // see: 0 times it would reach the others. It goes into the sums of those that do.
+                uint32_t odd = 0;
+#pragma unroll
+                for (int hh = 0; hh < 2; ++hh)
+#pragma unroll
+                    for (int g = 0; g < G; ++g) odd |= __hneu2_mask(u2h(vm[hh][g]), u2h(vm[hh][g]));
+                if (__any_sync(0xffffffffu, odd != 0)) {
+#pragma unroll
+                    for (int hh = 0; hh < 2; ++hh)
+#pragma unroll
+                        for (int g = 0; g < G; ++g) {
+                            const uint32_t nan = __hneu2_mask(u2h(vm[hh][g]), u2h(vm[hh][g]));
+                            vm[hh][g] &= ~nan;
+                            // the first such key of the eight (lanes of equal t hold the same two)
+                            int at = 0x7fffffff;
+                            if (nan) at = u * kDecUnit + 2 * t + 8 * hh + (nan & 0xffffu ? 0 : 1);
+                            at = __reduce_min_sync(0xffffffffu, at);
+#pragma unroll
+                            for (int c = 0; c < 4; ++c)
+                                if (at <= lim[c & 1]) {
+#pragma unroll
+                                    for (int i = 0; i < 4; ++i) o[g][i][c] = __uint_as_float(0x7fc00000u);
+                                }
+                        }
+                }
             }
             // ---- scales of V to where p s keeps its bits: at the warp's first unit, and again for much larger ones
             if (k == 0 || lift != 1.f) {

@@ -172,6 +172,7 @@ __global__ void __launch_bounds__(kPfThreads, 1) kv4_prefill_kernel(Kv4AttnParam
              *p_full = bar + 10, *o_full = bar + 12, *q_full = bar + 14, *p_half = bar + 16, *o_half = bar + 18;
     uint32_t* tmem_slot = reinterpret_cast<uint32_t*>(bar + 20);
     int* s_item = reinterpret_cast<int*>(bar + 21);  // b, item of b
+    int* s_nan = reinterpret_cast<int*>(bar + 22);   // first key whose group of V is NaN
 
     const int warp = __shfl_sync(0xffffffffu, threadIdx.x >> 5, 0), lane = threadIdx.x & 31;
     pdl_wait();
@@ -209,6 +210,7 @@ __global__ void __launch_bounds__(kPfThreads, 1) kv4_prefill_kernel(Kv4AttnParam
                 mbar_init(&o_half[i], 1);
             }
             fence_mbar_init();
+            s_nan[0] = s_nan[1] = 0x7fffffff;
         }
         __syncwarp();
         asm volatile("tcgen05.alloc.cta_group::1.sync.aligned.shared::cta.b32 [%0], %1;" ::"r"(smem_u32(tmem_slot)),
@@ -430,7 +432,14 @@ __global__ void __launch_bounds__(kPfThreads, 1) kv4_prefill_kernel(Kv4AttnParam
                         sc[y] = pf_u2h(__byte_perm(p0, p1, 0x5410));
                         mn[y] = pf_u2h(__byte_perm(p0, p1, 0x7632));
                         const float2 top = __half22float2(mn[y]), step = __half22float2(sc[y]);
-                        big |= top.x + 15.f * step.x >= 65504.f || top.y + 15.f * step.y >= 65504.f;
+                        big |= !(top.x + 15.f * step.x < 65504.f && top.y + 15.f * step.y < 65504.f);  // also NaN
+                    }
+                    // a NaN becomes 65504 below, as 0 times it would reach rows that do not see the
+                    // key; those that do take their NaN at the end
+                    if (big) {
+#pragma unroll 1
+                        for (int i = 0; i < 8; ++i)
+                            if ((lds_u32(ps + i * (4 * G) + 4 * g) & 0x7fff0000u) > 0x7c000000u) atomicMin(&s_nan[g], j * kPfKeys + 8 * tg + i);
                     }
                     uint32_t cw[8];
 #pragma unroll
@@ -637,6 +646,7 @@ __global__ void __launch_bounds__(kPfThreads, 1) kv4_prefill_kernel(Kv4AttnParam
         const float l = la + lb, inv = 1.f / l;
         const bool any = nt > 0 && l != 0.f;  // a key was seen; NaN stays
         if (nt > 0) {
+            wait(&v_full[(nt - 1) & 1], ((nt - 1) >> 1) & 1);  // s_nan is complete
             wait(&o_full[i], 0);
             tc_fence_after();
         }
@@ -649,10 +659,11 @@ __global__ void __launch_bounds__(kPfThreads, 1) kv4_prefill_kernel(Kv4AttnParam
                 tc_ld32_wait(x);
             }
             uint32_t y[16];
+            const float mul = s_nan[q / 2] <= lim ? __uint_as_float(0x7fc00000u) : inv;
 #pragma unroll
             for (int c = 0; c < 16; ++c) {
-                const float a = any ? __uint_as_float(x[2 * c]) * inv : 0.f;
-                const float bb = any ? __uint_as_float(x[2 * c + 1]) * inv : 0.f;
+                const float a = any ? __uint_as_float(x[2 * c]) * mul : 0.f;
+                const float bb = any ? __uint_as_float(x[2 * c + 1]) * mul : 0.f;
                 __nv_bfloat162 h = __floats2bfloat162_rn(a, bb);
                 y[c] = *reinterpret_cast<uint32_t*>(&h);
             }

@@ -437,8 +437,9 @@ am_status_code amcu_sample(const AmcuSampleArgs* args, void* stream);
 /* 8 * (j / (head_dim / 64)) + i in nibble i (bits 4i..4i+3).                 */
 /* Quantising x (fp32, per group): m = fp16(min x), s = fp16(min((max x -     */
 /* min x) * fp32(1/15), 4366)), code = clamp(rint((x - m) / s), 0, 15); s = 0 */
-/* gives code 0. m saturates at +-65504; NaN elements are left out of min and max and    */
-/* stored as code 0.                                                          */
+/* gives code 0. m saturates at +-65504; NaN elements are left out of min and */
+/* max and stored as code 0; a group of NaN alone has m = NaN, s = 0 and reads */
+/* as NaN.                                                                    */
 /* ------------------------------------------------------------------------ */
 typedef struct AmcuKv4Cache {
     void* k_codes;
@@ -504,7 +505,9 @@ am_status_code amcu_kv4_gather(const AmcuKv4GatherArgs* args, void* stream);
 /* Causal GQA attention of the call's rows over the cache, which already holds
  * them: out = sum_j softmax_j(scale * q . k_j) v_j over positions j up to the
  * row's own. Rows that see no key are zero; a row of q (one head) with a NaN or
- * infinite element that sees one is NaN. Any mixture of single tokens and
+ * infinite element that sees one is NaN, and so is a row that sees a NaN key, and
+ * the 64 elements of a NaN group of a value that it sees (no other row, also in the
+ * same call). Any mixture of single tokens and
  * prompts; n_q_heads a multiple of n_kv_heads. Sums and softmax statistics are
  * fp32; bf16 calls take p and the cache's values to 11 bits on the way (fp16; an
  * element beyond 65504 may be taken as 65504). A bounded wait that runs out

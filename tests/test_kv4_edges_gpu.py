@@ -101,3 +101,75 @@ def test_attention_of_a_q_that_is_no_number(ops, lens, nq, nkv, d, bad, dtype):
             assert (part == 0).all(), (r, h)
         part.copy_(torch.from_numpy(want[r, h * d:(h + 1) * d]))
     check_attention(got, want, dtype, 4.0)
+
+
+@pytest.mark.parametrize("dtype", [torch.bfloat16, torch.float32])
+@pytest.mark.parametrize("d", [64, 128])
+@pytest.mark.parametrize("steps", [1, 4])
+def test_append_of_groups_that_are_no_numbers(ops, d, steps, dtype):
+    """A group of NaN alone reads as NaN, whether a norm made it or not; its neighbours are as they would be."""
+    rng = np.random.default_rng(7)
+    nq, nkv, page = 8, 2, 32
+    rows = 24 if steps == 1 else 7000  # few and many steps to a warp
+    x = torch.from_numpy(rng.normal(0, 1, (rows, (nq + 2 * nkv) * d)).astype(np.float32)).to(dtype).cuda()
+    k0, v0 = nq * d, (nq + nkv) * d
+    bad = x.clone()
+    bad[3, v0: v0 + 64] = float("nan")            # the first group of a value
+    bad[5, v0 + 2 * d - 64: v0 + 2 * d] = float("nan")   # the last one of the row
+    bad[9, k0 + d + 7] = float("nan")             # one element of a key: the norm spreads it over the head
+    cs = torch.from_numpy(ref.rope_table(10000.0, d, rows)).cuda()
+    pages = -(-rows // page)
+    args = (i32([list(range(pages))]), i32([0, rows]), i32([rows]))
+    w = torch.ones(d, dtype=dtype, device="cuda")
+    got = []
+    for t in (x, bad):
+        cache = ops.kv4_cache(pages, page, nkv, d)
+        q = ops.kv4_append(t[:, :k0], t[:, k0:v0], t[:, v0:], cache, *args, cs, nq, nkv, d, q_norm=w, k_norm=w)
+        got.append((q, *ops.kv4_gather(cache, *args, rows, nkv, d, dtype=torch.float32)))
+    (q, k, v), (bq, bk, bv) = got
+    assert torch.equal(q, bq)
+    assert torch.isnan(bk[9, d:]).all()
+    bk[9, d:] = k[9, d:]
+    assert torch.isnan(bv[3, :64]).all() and torch.isnan(bv[5, -64:]).all()
+    bv[3, :64], bv[5, -64:] = v[3, :64], v[5, -64:]
+    assert torch.equal(k, bk) and torch.equal(v, bv)
+
+
+@pytest.mark.parametrize("dtype", [torch.bfloat16, torch.float32])
+@pytest.mark.parametrize("lens,at,nq,nkv,d", [
+    ([(40, 5), (40, 5)], 37, 8, 2, 128),   # rows 0 and 1 of five do not see it
+    ([(40, 5), (40, 5)], 3, 8, 2, 64),
+    ([(9000, 3)], 8998, 8, 2, 64),         # items cut between CTAs
+    ([(9000, 3)], 4001, 8, 2, 128),
+    ([(30, 2)] * 160, 29, 32, 8, 128),     # each warp takes whole items
+    ([(300, 160)], 220, 32, 8, 128),       # bf16: the kernel of prompts
+    ([(400, 190), (300, 20)], 399, 32, 8, 64),
+    ([(300, 160)], 5, 32, 8, 128),
+])
+def test_attention_over_keys_and_values_that_are_no_numbers(ops, lens, at, nq, nkv, d, dtype):
+    """A NaN key is in every element of the rows that see it, a NaN group of a value in its 64 elements of them, and
+    neither is in another row, head or sequence."""
+    rng = np.random.default_rng(11)
+    table, start, ctx, total = make_batch(lens, 16, rng)
+    cache = random_cache(total, nkv, 16, d, rng)
+    poison_unused(cache, table, ctx)
+    rows = start[-1]
+    q = torch.from_numpy(rng.normal(0, 1.5, (rows, nq * d)).astype(np.float32)).to(dtype)
+    want = ref.attention(q.double().numpy(), cache, table, start, ctx, nq, nkv, d)
+    heads, grp = want.reshape(rows, nq, d).copy(), nq // nkv
+    kc, kp, vc, vp = cache
+    for b, (kh, vh, g) in ((0, (0, 1, 0)), (len(lens) - 1, (1, 0, d // 64 - 1))):
+        if at >= ctx[b]:
+            continue
+        page, slot = table[b, at // 16], at % 16
+        for par, h, i in ((kp, kh, 0), (vp, vh, g)):
+            par[page, h, slot, i] = (0, np.nan)
+        for r in range(start[b], start[b + 1]):
+            if ctx[b] - start[b + 1] + r >= at:
+                heads[r, kh * grp:(kh + 1) * grp] = np.nan
+                heads[r, vh * grp:(vh + 1) * grp, 64 * g:64 * g + 64] = np.nan
+    got = ops.attention_kv4(q.cuda(), dev(cache), di(table), di(start), di(ctx), nq, nkv, d)
+    nan = torch.from_numpy(np.isnan(heads).reshape(rows, -1)).cuda()
+    assert nan.any() and torch.equal(torch.isnan(got), nan)
+    got[nan] = torch.from_numpy(want).to(dtype).cuda()[nan]
+    check_attention(got, want, dtype, 4.0)
