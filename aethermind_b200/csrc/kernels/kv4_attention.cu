@@ -313,7 +313,7 @@ __global__ void __launch_bounds__(kDecThreads, 2) kv4_decode_kernel(Kv4AttnParam
             for (int g = 0; g < G; ++g) qg[g][j] = __shfl_sync(0xffffffffu, qsum[g] * sl, src);
         }
         float ref[2] = {-1e30f, -1e30f};
-        float lift = kWide ? 0.f : 1.f;  // V's scales are multiplied by it (0: not chosen yet)
+        float lift = 0.f;  // V's scales are multiplied by it (0: not chosen yet, every scale so far is 0)
         float o[G][4][4], xa[4] = {};
 #pragma unroll
         for (int g = 0; g < G; ++g)
@@ -442,8 +442,8 @@ __global__ void __launch_bounds__(kDecThreads, 2) kv4_decode_kernel(Kv4AttnParam
                         }
                 }
             }
-            // ---- scales of V to where p s keeps its bits: at the warp's first unit, and again for much larger ones
-            if (k == 0 || lift != 1.f) {
+            // ---- scales of V to where p s keeps its bits: at the warp's first unit with any, and again for much larger ones
+            if (lift != 1.f) {
                 float top = 0.f;  // over the unit's 16 keys: the largest scale, fp32: the largest element
 #pragma unroll
                 for (int hh = 0; hh < 2; ++hh)
@@ -458,8 +458,8 @@ __global__ void __launch_bounds__(kDecThreads, 2) kv4_decode_kernel(Kv4AttnParam
                 top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, 2));
                 // to [64, 128), fp32: [1024, 2048)
                 const float fits = __uint_as_float(((kWide ? 264u : 260u) - (__float_as_uint(fmaxf(top, 6e-8f)) >> 23)) << 23);
-                if (k == 0) {
-                    if (kWide || (top > 0.f && top < 0.03125f)) lift = fits;
+                if (lift == 0.f) {
+                    if (kWide || top > 0.f) lift = kWide || top < 0.03125f ? fits : 1.f;
                 } else if (top * lift >= (kWide ? 32768.f : 4096.f)) {
                     const float corr = fits / lift;
                     lift = fits;
@@ -592,7 +592,7 @@ __global__ void __launch_bounds__(kDecThreads, 2) kv4_decode_kernel(Kv4AttnParam
         float* mo = reinterpret_cast<float*>(alone ? smem + warp * (S * kStage) : smem);
         float* mx = mo + (alone ? 1 : kDecWarps) * 8 * kMS;  // [warp][column][4]
         // low nibbles are in units of 2^-24, high ones of 2^-20 (fp32: of 1), both times lift
-        const float unlift = nk > 0 ? 1.f / lift : 0.f;
+        const float unlift = lift > 0.f ? 1.f / lift : 0.f;
         const float lo_unit = (kWide ? 1.f : 16777216.f) * unlift, hi_unit = (kWide ? 1.f : 1048576.f) * unlift;
         if (kWide) {  // high and low columns of one head
 #pragma unroll

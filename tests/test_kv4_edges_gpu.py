@@ -173,3 +173,25 @@ def test_attention_over_keys_and_values_that_are_no_numbers(ops, lens, at, nq, n
     assert nan.any() and torch.equal(torch.isnan(got), nan)
     got[nan] = torch.from_numpy(want).to(dtype).cuda()[nan]
     check_attention(got, want, dtype, 4.0)
+
+
+# ------------------------------------------------------------------ numbers far apart
+@pytest.mark.parametrize("s", [6e-8, 1e-6, 1e-4])
+@pytest.mark.parametrize("hole", [False, True])
+@pytest.mark.parametrize("n", [1, 150])
+def test_attention_small_values_after_zeros(ops, s, hole, n):
+    """Values of one number only (scale 0), or a page that is none, before values with the smallest scales. bf16:
+    p and p s are rounded to 11 bits, the result to 8: 2^-8 of its norm."""
+    rng = np.random.default_rng(4)
+    nq, nkv, d = 8, 2, 128
+    table, start, ctx, total = make_batch([(400, 1)] * n, 16, rng)
+    cache = random_cache(total, nkv, 16, d, rng)
+    cache[3][..., 0] = np.float16(s)
+    cache[3][..., 1] = 0
+    cache[3][table[:, :9], ..., 0] = 0
+    if hole:
+        table[:, 0] = -1
+    q = bf16(rng.normal(0, 1, (n, nq * d)))
+    want = ref.attention(q.double().numpy(), cache, table, start, ctx, nq, nkv, d)
+    got = ops.attention_kv4(q.cuda(), dev(cache), di(table), di(start), di(ctx), nq, nkv, d).double().cpu().numpy()
+    assert np.linalg.norm(got - want) <= 2.0 ** -8 * np.linalg.norm(want)
