@@ -425,22 +425,20 @@ __global__ void __launch_bounds__(kPfThreads, 1) kv4_prefill_kernel(Kv4AttnParam
 #pragma unroll
                 for (int g = 0; g < G; ++g) {
                     __half2 sc[4], mn[4];
-                    bool big = false;
+                    __half2 top;  // largest element of the tokens' groups
 #pragma unroll
                     for (int y = 0; y < 4; ++y) {
                         const uint32_t p0 = lds_u32(ps + (2 * y) * (4 * G) + 4 * g), p1 = lds_u32(ps + (2 * y + 1) * (4 * G) + 4 * g);
                         sc[y] = pf_u2h(__byte_perm(p0, p1, 0x5410));
                         mn[y] = pf_u2h(__byte_perm(p0, p1, 0x7632));
-                        const float2 top = __half22float2(mn[y]), step = __half22float2(sc[y]);
-                        big |= !(top.x + 15.f * step.x < 65504.f && top.y + 15.f * step.y < 65504.f);  // also NaN
+                        const __half2 most = __hfma2(__float2half2_rn(15.f), sc[y], mn[y]);
+                        top = y == 0 ? most : __hmax2_nan(top, most);
                     }
+                    const bool big = !__hblt2(top, pf_u2h(0x7c007c00u));  // beyond fp16, or NaN
                     // a NaN becomes 65504 below, as 0 times it would reach rows that do not see the
-                    // key; those that do take their NaN at the end
-                    if (big) {
-#pragma unroll 1
-                        for (int i = 0; i < 8; ++i)
-                            if ((lds_u32(ps + i * (4 * G) + 4 * g) & 0x7fff0000u) > 0x7c000000u) atomicMin(&s_nan[g], j * kPfKeys + 8 * tg + i);
-                    }
+                    // key; those that do take their NaN at the end (each thread looks at one token)
+                    if (big && (lds_u32(ps + q8 * (4 * G) + 4 * g) & 0x7fff0000u) > 0x7c000000u)
+                        atomicMin(&s_nan[g], j * kPfKeys + 8 * tg + q8);
                     uint32_t cw[8];
 #pragma unroll
                     for (int i = 0; i < 8; ++i) cw[i] = lds_u32(src + i * (D / 2) + 4 * g);
