@@ -29,16 +29,19 @@ namespace amcu {
 // which makes the integer dot product exact up to fp32 sums; scale and minimum
 // of a key's group are applied to the 64-element sums (m through sum(q)). In the
 // second product the rows that come from low nibbles are 2^-4 of the others until
-// the end, the scales of V go into p (p s, rounded to 11 bits), and the minima and the softmax denominator are three more rows of
-// the product. p s is fp16: where a warp's scales are below 2^-5 they are lifted by a power of two, so precision is relative to the largest scales
-// that the warp meets, not to 6e-8. The MMA aligns its products by their operands'
-// exponents, subnormals' by that of 2^-14: sums with such codes are good to 2^-17 of
-// their largest term, which bf16 does not see.
+// the end, the scales of V go into p (p s, rounded to 11 bits), and the minima and
+// the softmax denominator are three more rows of the product. p and p s are fp16: a
+// tail of many keys under one that has most of the mass keeps its bits because p is
+// counted in 2^-10 of the largest (p of 2^-20 lost 2 to 80% of such a tail where it was
+// counted in the largest itself), and scales below 2^-4 or above 4 are lifted by a power
+// of two, so that precision is relative to the largest that the warp meets. The MMA
+// aligns its products by their operands' exponents, subnormals' by that of 2^-14: sums
+// with such codes are good to 2^-17 of their largest term, which bf16 does not see.
 //
 // fp32 calls work with normal halves around zero, c - 8 = (1024 + c) - 1032, and 8 s
 // more in the minimum. An average over many keys is small beside its terms, so
 // there V's elements are formed whole, m + s c in fp32, and go into the product as
-// a high and a low half; p, times 2^12 to keep its low half normal, does too.
+// a high and a low half; p, counted in 2^-12 of the largest, does too.
 constexpr int kDecWarps = 8;
 constexpr int kDecThreads = kDecWarps * 32;
 constexpr int kDecStages = 4;  // 64 ragged rows: 103.7 us, 105.0 with 5, 106.0 with 6
@@ -54,7 +57,10 @@ constexpr int kDecMinUnits = 8;
 // of 250 24 / 46, 256 of 100 22 / 61, 256 of 300 39 / 81, 256 of 600 60 / 88.
 constexpr int kDecMany = 2, kDecLong = 8;
 constexpr float kLog2e = 1.4426950408889634f;
-constexpr float kDecLift = 3.f;    // p stays below 2^3 before its reference moves
+constexpr float kDecLift = 3.f;    // scores pass their largest so far by that much (log2) before the reference moves
+// The reference lies that far below the largest score: p is up to 2^13 (fp32: 2^15) and
+// an fp16 normal, rounded to 11 bits, down to 2^-24 (2^-26) of the largest one.
+template <typename T> constexpr float dec_head() { return sizeof(T) == 2 ? 10.f : 12.f; }
 
 template <typename T> constexpr int dec_cols() { return sizeof(T) == 2 ? 8 : 4; }  // (row, head) pairs per tile
 template <int D> constexpr int dec_stage_bytes() { return 2 * kDecUnit * (D / 2 + D / 16) + 16; }
@@ -313,7 +319,11 @@ __global__ void __launch_bounds__(kDecThreads, 2) kv4_decode_kernel(Kv4AttnParam
             for (int g = 0; g < G; ++g) qg[g][j] = __shfl_sync(0xffffffffu, qsum[g] * sl, src);
         }
         float ref[2] = {-1e30f, -1e30f};
-        float lift = 0.f;  // V's scales are multiplied by it (0: not chosen yet, every scale so far is 0)
+        float lift = 0.f;     // fp32: V's elements are multiplied by it (0: not chosen yet)
+        uint32_t s_most = 0;  // bf16: 4 / lift in both halves, a power of two; a scale above it asks for another lift
+        auto lift_of = [](uint32_t most) {  // 0: not chosen yet, every scale so far is 0
+            return __uint_as_float((256u << 23) - __float_as_uint(__low2float(u2h(most))));
+        };
         float o[G][4][4], xa[4] = {};
 #pragma unroll
         for (int g = 0; g < G; ++g)
@@ -442,25 +452,24 @@ __global__ void __launch_bounds__(kDecThreads, 2) kv4_decode_kernel(Kv4AttnParam
                         }
                 }
             }
-            // ---- scales of V to where p s keeps its bits: at the warp's first unit with any, and again for much larger ones
-            if (lift != 1.f) {
-                float top = 0.f;  // over the unit's 16 keys: the largest scale, fp32: the largest element
+            // fp32: elements of V to where their two halves keep their bits, at the warp's first unit and
+            // again for much larger ones
+            if (kWide) {
+                float top = 0.f;  // the largest element of the unit's 16 keys
 #pragma unroll
                 for (int hh = 0; hh < 2; ++hh)
 #pragma unroll
                     for (int g = 0; g < G; ++g) {
                         const float2 sv = __half22float2(u2h(vs[hh][g])), mv = __half22float2(u2h(vm[hh][g]));
-                        top = fmaxf(top, kWide ? fmaxf(fmaxf(fabsf(mv.x), fabsf(fmaf(15.f, sv.x, mv.x))),
-                                                       fmaxf(fabsf(mv.y), fabsf(fmaf(15.f, sv.y, mv.y))))
-                                               : fmaxf(sv.x, sv.y));
+                        top = fmaxf(top, fmaxf(fmaxf(fabsf(mv.x), fabsf(fmaf(15.f, sv.x, mv.x))),
+                                               fmaxf(fabsf(mv.y), fabsf(fmaf(15.f, sv.y, mv.y)))));
                     }
                 top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, 1));
                 top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, 2));
-                // to [64, 128), fp32: [1024, 2048)
-                const float fits = __uint_as_float(((kWide ? 264u : 260u) - (__float_as_uint(fmaxf(top, 6e-8f)) >> 23)) << 23);
+                const float fits = __uint_as_float((264u - (__float_as_uint(fmaxf(top, 6e-8f)) >> 23)) << 23);  // to [1024, 2048)
                 if (lift == 0.f) {
-                    if (kWide || top > 0.f) lift = kWide || top < 0.03125f ? fits : 1.f;
-                } else if (top * lift >= (kWide ? 32768.f : 4096.f)) {
+                    lift = fits;
+                } else if (top * lift >= 32768.f) {
                     const float corr = fits / lift;
                     lift = fits;
 #pragma unroll
@@ -471,19 +480,37 @@ __global__ void __launch_bounds__(kDecThreads, 2) kv4_decode_kernel(Kv4AttnParam
                             for (int c = 0; c < 4; ++c) o[g][i][c] *= corr;
                 }
             }
-            // ---- softmax: the reference moves only when a score passes it by kDecLift
+            // ---- softmax: the reference moves only when a score passes the largest so far by kDecLift;
+            // bf16: and V's lift when a scale passes s_most
+            constexpr float kHead = dec_head<T>();
             float pr[4];
 #pragma unroll
             for (int c = 0; c < 4; ++c) pr[c] = sc[c] - ref[c & 1];
-            if (__any_sync(0xffffffffu, fmaxf(fmaxf(pr[0], pr[1]), fmaxf(pr[2], pr[3])) > kDecLift)) {
+            __half2 s_top = u2h(vs[0][0]);
+#pragma unroll
+            for (int e = 1; e < 2 * G; ++e) s_top = __hmax2(s_top, u2h(vs[e & 1][e >> 1]));
+            const bool odd_scale = !kWide && __hgt2_mask(s_top, u2h(s_most)) != 0;
+            if (__any_sync(0xffffffffu, odd_scale || fmaxf(fmaxf(pr[0], pr[1]), fmaxf(pr[2], pr[3])) > kHead + kDecLift)) {
+                float s_corr = 1.f;
+                if (!kWide && __any_sync(0xffffffffu, odd_scale)) {
+                    float top = fmaxf(__low2float(s_top), __high2float(s_top));  // over the unit's 16 keys
+                    top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, 1));
+                    top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, 2));
+                    // usual scales stay as they are, others go to [1/4, 1/2): p s is up to 2^15, and normal
+                    // down to p of 2^-20 of the largest
+                    const float fits = __uint_as_float((252u - min(__float_as_uint(top) >> 23, 138u)) << 23);
+                    const float next = s_most == 0 && top >= 0.0625f && top <= 4.f ? 1.f : fits;
+                    if (s_most != 0) s_corr = next * __uint_as_float((254u << 23) - __float_as_uint(lift_of(s_most)));
+                    s_most = h2u(__float2half2_rn(__uint_as_float((256u << 23) - __float_as_uint(next))));
+                }
 #pragma unroll
                 for (int j = 0; j < 2; ++j) {
                     float m = fmaxf(sc[j], sc[2 + j]);
                     m = fmaxf(m, __shfl_xor_sync(0xffffffffu, m, 4));
                     m = fmaxf(m, __shfl_xor_sync(0xffffffffu, m, 8));
                     m = fmaxf(m, __shfl_xor_sync(0xffffffffu, m, 16));
-                    m = fmaxf(m, ref[j]);
-                    const float corr = ex2(ref[j] - m);
+                    m = fmaxf(m - kHead, ref[j]);
+                    const float corr = ex2(ref[j] - m), o_corr = corr * s_corr;
                     ref[j] = m;
                     pr[j] = sc[j] - m;
                     pr[2 + j] = sc[2 + j] - m;
@@ -493,13 +520,13 @@ __global__ void __launch_bounds__(kDecThreads, 2) kv4_decode_kernel(Kv4AttnParam
                     for (int g = 0; g < G; ++g)
 #pragma unroll
                         for (int i = 0; i < 4; ++i) {
-                            o[g][i][j] *= corr;
-                            o[g][i][2 + j] *= corr;
+                            o[g][i][j] *= o_corr;
+                            o[g][i][2 + j] *= o_corr;
                         }
                 }
             }
 #pragma unroll
-            for (int c = 0; c < 4; ++c) pr[c] = kWide ? ex2(pr[c]) * 4096.f : ex2(pr[c]);
+            for (int c = 0; c < 4; ++c) pr[c] = ex2(pr[c]);
             uint32_t pb[2], ps[2][G];  // p, and p times the groups' scales (bf16)
 #pragma unroll
             for (int hh = 0; hh < 2; ++hh) {
@@ -511,7 +538,8 @@ __global__ void __launch_bounds__(kDecThreads, 2) kv4_decode_kernel(Kv4AttnParam
                     pb[hh] = two(pr[2 * hh]);
                 } else {
                     pb[hh] = movm_trans(h2u(__floats2half2_rn(pr[2 * hh], pr[2 * hh + 1])));
-                    if (lift != 1.f) {
+                    if (s_most != 0x44004400u) {
+                        const float lift = lift_of(s_most);
 #pragma unroll
                         for (int g = 0; g < G; ++g) {
                             const float2 y = __half22float2(u2h(vs[hh][g]));
@@ -592,7 +620,7 @@ __global__ void __launch_bounds__(kDecThreads, 2) kv4_decode_kernel(Kv4AttnParam
         float* mo = reinterpret_cast<float*>(alone ? smem + warp * (S * kStage) : smem);
         float* mx = mo + (alone ? 1 : kDecWarps) * 8 * kMS;  // [warp][column][4]
         // low nibbles are in units of 2^-24, high ones of 2^-20 (fp32: of 1), both times lift
-        const float unlift = lift > 0.f ? 1.f / lift : 0.f;
+        const float unlift = kWide ? (lift > 0.f ? 1.f / lift : 0.f) : 0.25f * __low2float(u2h(s_most));
         const float lo_unit = (kWide ? 1.f : 16777216.f) * unlift, hi_unit = (kWide ? 1.f : 1048576.f) * unlift;
         if (kWide) {  // high and low columns of one head
 #pragma unroll

@@ -195,3 +195,49 @@ def test_attention_small_values_after_zeros(ops, s, hole, n):
     want = ref.attention(q.double().numpy(), cache, table, start, ctx, nq, nkv, d)
     got = ops.attention_kv4(q.cuda(), dev(cache), di(table), di(start), di(ctx), nq, nkv, d).double().cpu().numpy()
     assert np.linalg.norm(got - want) <= 2.0 ** -8 * np.linalg.norm(want)
+
+
+def one_token_with_most_of_the_mass(lens, nq, nkv, d, dtype, s, s_first):
+    """Inputs whose first key is e^3 to e^14 times as likely as every other one (by row and head), and the result.
+    s: V's scale (its minimum is 0), s_first: the first key's. All other keys are alike, so that a rounding of p or of
+    p s is every key's and does not average out."""
+    rng = np.random.default_rng(5)
+    page = 64
+    table, start, ctx, total = make_batch(lens, page, rng)
+    kc, kp, vc, vp = random_cache(total, nkv, page, d, rng)
+    kp[..., 0], kp[..., 1] = 0, 0.25
+    vp[..., 0], vp[..., 1] = np.float16(s), 0
+    kp[table[:, 0], :, 0, :, 1] = 1.25
+    vp[table[:, 0], :, 0, :, 0] = np.float16(s_first)
+    rows = start[-1]
+    gap = np.linspace(3, 14, rows * nq).reshape(rows, nq)
+    q = torch.from_numpy(np.repeat(gap / d, d, 1).astype(np.float32)).to(dtype)
+    rest = np.exp(-q.double().numpy().reshape(rows, nq, d).sum(-1))  # the others' p
+    want = np.zeros((rows, nq, d))
+    for b, (c, n) in enumerate(lens):
+        v = ref.values(vc[table[b]], vp[table[b]]).transpose(1, 0, 2, 3).reshape(nkv, -1, d)
+        total_v = np.cumsum(v[:, 1:], 1)
+        for r in range(start[b], start[b + 1]):
+            others = c - n + r - start[b]
+            for h in range(nq):
+                e, g = rest[r, h], h // (nq // nkv)
+                want[r, h] = (v[g, 0] + e * total_v[g, others - 1]) / (1 + e * others)
+    return (q.cuda(), dev((kc, kp, vc, vp)), di(table), di(start), di(ctx), nq, nkv, d), want
+
+
+def worst_head(got, want):
+    got = got.double().cpu().numpy().reshape(want.shape)
+    return (np.linalg.norm(got - want, axis=-1) / np.linalg.norm(want, axis=-1)).max()
+
+
+@pytest.mark.parametrize("s,s_first", [(0.3, 0), (0.07, 0), (0.04, 0), (3.0, 0), (9.0, 0), (100.0, 0), (0.3, 0.3),
+                                       (0.3, 30.0), (100.0, 0.3), (1e-5, 4000.0)])
+@pytest.mark.parametrize("lens,nq,nkv,d", [
+    ([(600, 1)] * 160, 32, 8, 64),   # each warp takes whole items
+    ([(20000, 1)], 12, 2, 128),      # items cut between CTAs
+    ([(300, 2), (90, 1)], 8, 2, 128),
+])
+def test_attention_of_one_token_with_most_of_the_mass(ops, lens, nq, nkv, d, s, s_first):
+    """bf16: p and p s are rounded to 11 bits (2^-12 each), the result to 8 (2^-9): no head is off by 2^-8."""
+    args, want = one_token_with_most_of_the_mass(lens, nq, nkv, d, torch.bfloat16, s, s_first)
+    assert worst_head(ops.attention_kv4(*args, scale=1.0), want) <= 2.0 ** -8
