@@ -25,11 +25,12 @@
 // m + s c in fp16: (1024 + c) - 1024 exactly, then one fused multiply-add
 // rounded once to 11 bits (an element beyond fp16 becomes 65504).
 //
-// The softmax reference of a row moves only when a score passes it by 2^8 (p
-// stays inside fp16, whose relative precision does not depend on the
-// reference), and to a whole power of two: the sum, O and what the tile has of P
-// already are then rescaled exactly. So the scores are read once, without
-// knowing their tile's maximum first.
+// The softmax reference of a row lies 2^7 to 2^8 below the largest score when it is
+// set and moves only when a score passes that by 2^8 more (p, in fp16, is then 2^15),
+// and to a whole power of two: the sum, O and what the tile has of P already are then
+// rescaled without a rounding (P where it stays normal). So the scores are read once, without knowing their tile's
+// maximum first. (With the reference at the largest score itself p of 2^-20 kept 4
+// bits: 3% of a row of many such keys under one that has most of the mass.)
 //
 // Waits are bounded: one that runs out records an error code, and the CTA goes
 // through its control flow without waiting again.
@@ -44,7 +45,10 @@ constexpr int kPfMmaWarp = 16;
 constexpr int kPfDqThreads = 128;
 constexpr int32_t kErrKv4Wait = 0x501;
 constexpr float kPfLog2e = 1.4426950408889634f;
-constexpr float kPfLift = 8.f;
+// A score may pass the largest so far by kPfLift before the reference moves, to
+// kPfHead below the new largest: p is up to 2^15, and an fp16 normal, rounded to 11 bits,
+// down to 2^-20 of the largest one (2^-32 is still counted).
+constexpr float kPfLift = 8.f, kPfHead = 7.f;
 
 template <int D>
 struct PfLayout {  // shared memory, bytes
@@ -572,7 +576,7 @@ __global__ void __launch_bounds__(kPfThreads, 1) kv4_prefill_kernel(Kv4AttnParam
             for (int q = 0; q < 4; ++q) {
                 uint32_t(&z)[32] = x[q & 1];
                 tc_ld32_wait(z);
-                // the reference moves only for a score that passes it by kPfLift
+                // the reference moves only for a score that passes the largest so far by kPfLift
                 float m4[4];
 #pragma unroll
                 for (int c = 0; c < 4; ++c) m4[c] = fmaxf(__uint_as_float(z[c]), __uint_as_float(z[c + 4]));
@@ -582,9 +586,9 @@ __global__ void __launch_bounds__(kPfThreads, 1) kv4_prefill_kernel(Kv4AttnParam
                     for (int k = 0; k < 4; ++k)
                         m4[k] = fmaxf(fmaxf(m4[k], __uint_as_float(z[c + k])), __uint_as_float(z[c + k + 4]));
                 const float mx = fmaxf(fmaxf(m4[0], m4[1]), fmaxf(m4[2], m4[3])) * f;
-                if (__any_sync(0xffffffffu, mx > ref + kPfLift)) {
+                if (__any_sync(0xffffffffu, mx > ref + (kPfHead + kPfLift))) {
                     // to a whole number, so that every rescaling is by a power of two
-                    const float nref = mx > ref ? ceilf(fminf(mx, 1e30f)) : ref, corr = pf_ex2(ref - nref);
+                    const float nref = mx > ref + kPfHead ? ceilf(fminf(mx, 1e30f)) - kPfHead : ref, corr = pf_ex2(ref - nref);
                     ref = nref;
                     l2 = f2_fma(l2, f2_pack(corr, corr), f2_pack(0.f, 0.f));
                     l3 = f2_fma(l3, f2_pack(corr, corr), f2_pack(0.f, 0.f));

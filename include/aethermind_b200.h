@@ -504,12 +504,12 @@ typedef struct AmcuKv4GatherArgs {
 am_status_code amcu_kv4_gather(const AmcuKv4GatherArgs* args, void* stream);
 /* Causal GQA attention of the call's rows over the cache, which already holds
  * them: out = sum_j softmax_j(scale * q . k_j) v_j over positions j up to the
- * row's own. Rows that see no key are zero; a row of q (one head) with a NaN or
- * infinite element that sees one is NaN, and so is a row that sees a NaN key, and
- * the 64 elements of a NaN group of a value that it sees (no other row, also in the
- * same call). Any mixture of single tokens and
- * prompts; n_q_heads a multiple of n_kv_heads. Sums and softmax statistics are
- * fp32; bf16 calls take p and the cache's values to 11 bits on the way (fp16; an
+ * row's own. Any mixture of single tokens and prompts; n_q_heads a multiple of
+ * n_kv_heads. Rows that see no key are zero. A row of q (one head) with a NaN or
+ * infinite element that sees a key is NaN; so is a row that sees a NaN key, and the
+ * 64 elements of a NaN group of a value that it sees (no other row, also in the same
+ * call). Sums and softmax statistics are fp32; bf16 calls take p (of 2^-20 of the
+ * row's largest and more) and the cache's values to 11 bits on the way (fp16; an
  * element beyond 65504 may be taken as 65504). A bounded wait that runs out
  * records 0x501 in the device error word. */
 typedef struct AmcuKv4AttentionArgs {

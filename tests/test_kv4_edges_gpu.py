@@ -241,3 +241,20 @@ def test_attention_of_one_token_with_most_of_the_mass(ops, lens, nq, nkv, d, s, 
     """bf16: p and p s are rounded to 11 bits (2^-12 each), the result to 8 (2^-9): no head is off by 2^-8."""
     args, want = one_token_with_most_of_the_mass(lens, nq, nkv, d, torch.bfloat16, s, s_first)
     assert worst_head(ops.attention_kv4(*args, scale=1.0), want) <= 2.0 ** -8
+
+
+def in_the_kernel_of_prompts(lens, nq, nkv, sms=148):
+    """The rule by which bf16 calls go to the kernel of prompts."""
+    cols = sum(n for _, n in lens) * (nq // nkv)
+    tiles = (cols // 256 + len(lens)) * nkv
+    return -(-cols // 8) * nkv * 2 > 5 * sms * -(-tiles // sms)
+
+
+@pytest.mark.parametrize("s_first", [0, 0.3, 30.0])
+@pytest.mark.parametrize("lens,nq,nkv,d", [([(8192, 200)], 16, 1, 64), ([(8192, 200)], 16, 1, 128),
+                                           ([(4000, 160), (700, 100)], 32, 8, 64)])
+def test_attention_prompts_of_one_token_with_most_of_the_mass(ops, lens, nq, nkv, d, s_first):
+    """As above; p is rounded once (2^-12), the result to 8 bits (2^-9)."""
+    assert in_the_kernel_of_prompts(lens, nq, nkv)
+    args, want = one_token_with_most_of_the_mass(lens, nq, nkv, d, torch.bfloat16, 0.3, s_first)
+    assert worst_head(ops.attention_kv4(*args, scale=1.0), want) <= 2.0 ** -8
