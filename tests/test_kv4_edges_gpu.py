@@ -258,3 +258,13 @@ def test_attention_prompts_of_one_token_with_most_of_the_mass(ops, lens, nq, nkv
     assert in_the_kernel_of_prompts(lens, nq, nkv)
     args, want = one_token_with_most_of_the_mass(lens, nq, nkv, d, torch.bfloat16, 0.3, s_first)
     assert worst_head(ops.attention_kv4(*args, scale=1.0), want) <= 2.0 ** -8
+
+
+@pytest.mark.parametrize("s,s_first", [(0.3, 0), (0.04, 0), (100.0, 0), (0.3, 30.0), (100.0, 0.3)])
+@pytest.mark.parametrize("lens,nq,nkv,d", [([(600, 1)] * 160, 32, 8, 64), ([(20000, 1)], 12, 2, 128),
+                                           ([(300, 2), (90, 1)], 8, 2, 128)])
+def test_attention_fp32_of_one_token_with_most_of_the_mass(ops, lens, nq, nkv, d, s, s_first):
+    """fp32: a score of up to 14 carries an error of 2^-20 from its fp32 sums, p and the elements of V 2^-22 each: below
+    4e-6 in all."""
+    args, want = one_token_with_most_of_the_mass(lens, nq, nkv, d, torch.float32, s, s_first)
+    assert worst_head(ops.attention_kv4(*args, scale=1.0), want) <= 4e-6
