@@ -480,7 +480,7 @@ typedef struct AmcuKv4AppendArgs {
     const void* q;               /* [rows, n_q_heads * head_dim] */
     const void* k;               /* [rows, n_kv_heads * head_dim] */
     const void* v;
-    void* q_out;                 /* [rows, n_q_heads * head_dim]; may be q */
+    void* q_out;                 /* [rows, n_q_heads * head_dim]; may be q. Rows out of range are zero. */
     int64_t q_stride, k_stride, v_stride, q_out_stride;   /* elements, even */
     const void* q_norm;          /* [head_dim] or NULL */
     const void* k_norm;          /* [head_dim] or NULL */

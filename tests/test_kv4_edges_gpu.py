@@ -268,3 +268,47 @@ def test_attention_fp32_of_one_token_with_most_of_the_mass(ops, lens, nq, nkv, d
     4e-6 in all."""
     args, want = one_token_with_most_of_the_mass(lens, nq, nkv, d, torch.float32, s, s_first)
     assert worst_head(ops.attention_kv4(*args, scale=1.0), want) <= 4e-6
+
+
+# ------------------------------------------------------------------ rows that are nowhere
+@pytest.mark.parametrize("d,many", [(64, False), (64, True), (128, True)])
+@pytest.mark.parametrize("dtype", [torch.bfloat16, torch.float32])
+def test_append_rows_out_of_range_give_zeros(ops, d, many, dtype):
+    """q_out of rows before position 0 or past the rotation table is zero, in both layouts of the kernel."""
+    rng = np.random.default_rng(4)
+    nq, nkv, page = 6, 1, 16
+    n = 12000 if many else 0  # further rows, so that a warp takes several steps
+    table = np.arange(3 * 800, dtype=np.int32).reshape(3, 800)
+    start, ctx = np.array([0, 4, 8, 8 + n], np.int32), np.array([18, 2, n], np.int32)
+    rows = 8 + n
+    x = torch.from_numpy(rng.normal(0, 1, (rows, (nq + 2) * d)).astype(np.float32)).to(dtype).cuda()
+    cs = torch.from_numpy(ref.rope_table(10000.0, d, max(n, 17))).cuda()  # position 17 of sequence 0 where n is 0
+    cache = ops.kv4_cache(3 * 800, page, nkv, d)
+    status = i32([0])
+    args = (x[:, nq * d: (nq + 1) * d], x[:, (nq + 1) * d:], cache, di(table), di(start), di(ctx), cs, nq, nkv, d)
+    out = torch.full((rows, nq * d), float("nan"), dtype=dtype, device="cuda")
+    ops.kv4_append(x[:, : nq * d], *args, q_out=out, status=status)
+    zero = (out == 0).all(1).cpu().numpy()
+    want = np.zeros(rows, bool)
+    want[4:6] = True          # positions -2, -1
+    want[3] = not many        # position 17, past the table
+    np.testing.assert_array_equal(zero, want)
+    assert not torch.isnan(out).any() and status.item() == OUT_OF_RANGE
+
+
+@pytest.mark.parametrize("starts", [[0, 2, 4], [1, 2, 6], [2, 3, 4], [0, 0, 0], [6, 6, 6]])
+def test_append_and_gather_rows_of_no_sequence(ops, starts):
+    d, nq, nkv = 64, 4, 2
+    x = torch.ones(6, 8 * d, dtype=torch.bfloat16, device="cuda")
+    cs = torch.from_numpy(ref.rope_table(10000.0, d, 64)).cuda()
+    args = (i32([[0], [1]]), i32(starts), i32([9, 9]))
+    none = torch.tensor([not starts[0] <= r < starts[-1] for r in range(6)])
+    cache, status = ops.kv4_cache(2, 16, nkv, d), i32([0])
+    out = torch.full((6, nq * d), float("nan"), dtype=torch.bfloat16, device="cuda")
+    ops.kv4_append(x[:, : nq * d], x[:, : nkv * d], x[:, : nkv * d], cache, *args, cs, nq, nkv, d, q_out=out,
+                   status=status)
+    assert torch.equal((out == 0).all(1).cpu(), none) and status.item() == OUT_OF_RANGE
+    status.zero_()
+    k, v = ops.kv4_gather(cache, *args, 6, nkv, d, status=status)
+    assert torch.equal((k == 0).all(1).cpu(), none) and torch.equal((v == 0).all(1).cpu(), none)
+    assert status.item() == OUT_OF_RANGE
