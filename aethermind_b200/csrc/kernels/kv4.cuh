@@ -117,6 +117,21 @@ __device__ __forceinline__ bool kv4_share(int n_seq, P pick, F cost, int64_t& to
     }
 }
 
+// Rows of the call that no sequence has (row_start does not begin at 0 or does not
+// end at `rows`) are zero in the attention's output. first, end: row_start's ends.
+template <typename T, int THREADS>
+__device__ __forceinline__ void kv4_zero_uncovered(const Kv4View& v, int first, int end, void* out, int64_t stride, int width) {
+    first = min(max(first, 0), v.rows);
+    end = min(max(end, first), v.rows);
+    const int n = first + v.rows - end;
+    if (n == 0) return;
+    if (v.status && threadIdx.x == 0) *v.status = (int32_t)AM_STATUS_OUT_OF_RANGE;
+    for (int i = blockIdx.x; i < n; i += gridDim.x) {
+        T* o = static_cast<T*>(out) + (int64_t)(i < first ? i : end + (i - first)) * stride;
+        for (int e = threadIdx.x; e < width; e += THREADS) o[e] = Act<T>::store(0.f);
+    }
+}
+
 struct Kv4AttnParams {
     Kv4View v;
     const void* q;

@@ -155,6 +155,7 @@ __global__ void __launch_bounds__(kDecThreads, 2) kv4_decode_kernel(Kv4AttnParam
 
     // ---- this CTA's share [x, x_end) of all units
     const Kv4View& v = p.v;
+    const int row_first = v.row_start[0], row_end = v.row_start[v.n_seq];
     int most = 0;  // units of an item
     auto cost_of = [&](int i) {
         const DecSeq q = dec_seq<T>(v, p.grp, i);
@@ -181,6 +182,7 @@ __global__ void __launch_bounds__(kDecThreads, 2) kv4_decode_kernel(Kv4AttnParam
             s_off = off;
         }
     }
+    kv4_zero_uncovered<T, kDecThreads>(v, row_first, row_end, p.out, p.os, p.nq * D);
     int64_t x_end = min(x + share, total);
     if (threadIdx.x == 0) ws.meta[blockIdx.x].first = -1;
     if (x >= x_end) return;

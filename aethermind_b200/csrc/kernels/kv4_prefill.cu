@@ -185,6 +185,7 @@ __global__ void __launch_bounds__(kPfThreads, 1) kv4_prefill_kernel(Kv4AttnParam
     // ---- this CTA's item: sequence, kv head and row tile
     const Kv4View& v = p.v;
     {
+        const int row_first = v.row_start[0], row_end = v.row_start[v.n_seq];
         auto cost = [&](int b) {
             int r0, n;
             kv4_rows(v, b, r0, n);
@@ -193,6 +194,7 @@ __global__ void __launch_bounds__(kPfThreads, 1) kv4_prefill_kernel(Kv4AttnParam
         int64_t total, off;
         int b;
         const bool have = kv4_share<kPfThreads>(v.n_seq, [&](int64_t) { return (int64_t)blockIdx.x; }, cost, total, b, off);
+        kv4_zero_uncovered<__nv_bfloat16, kPfThreads>(v, row_first, row_end, p.out, p.os, p.nq * D);
         if ((int64_t)blockIdx.x >= total) return;
         if (have) {
             s_item[0] = b;

@@ -457,9 +457,11 @@ typedef struct AmcuKv4Cache {
  * row_start[b + 1] - 1 of the call (any number, also none); ctx_len[b] counts
  * its tokens WITH them, so row r of n is at position ctx_len[b] - n + r.
  * page_table[b][p / page_size] names position p's page. row_start is
- * non-decreasing from 0 to `rows`. A position below 0 or past the page table,
- * or a page outside [0, num_pages), is never read or written; where a row or
- * key needed it, *status (device, optional) becomes AM_STATUS_OUT_OF_RANGE. */
+ * non-decreasing from 0 to `rows`; rows that it leaves to no sequence are zero in
+ * the outputs and out of range (a call with n_seq 0 touches nothing). A position
+ * below 0 or past the page table, or a page outside [0, num_pages), is never read
+ * or written; where a row or key needed it, *status (device, optional) becomes
+ * AM_STATUS_OUT_OF_RANGE. */
 typedef struct AmcuKv4Batch {
     const int32_t* page_table;   /* device [n_seq][max_pages] */
     int64_t table_stride;        /* elements; 0 = max_pages */

@@ -312,3 +312,32 @@ def test_append_and_gather_rows_of_no_sequence(ops, starts):
     k, v = ops.kv4_gather(cache, *args, 6, nkv, d, status=status)
     assert torch.equal((k == 0).all(1).cpu(), none) and torch.equal((v == 0).all(1).cpu(), none)
     assert status.item() == OUT_OF_RANGE
+
+
+@pytest.mark.parametrize("dtype", [torch.bfloat16, torch.float32])
+@pytest.mark.parametrize("rows,starts,lens", [
+    (6, [0, 2, 4], [9, 9]), (6, [1, 2, 6], [9, 9]), (6, [2, 3, 4], [9, 9]), (6, [0, 0, 0], [9, 9]),
+    (400, list(range(5, 396)), [20] * 390),     # each warp takes whole items
+    (300, [3, 180, 290], [300, 200]),                 # bf16: the kernel of prompts
+    (700, [0, 0, 0], [300, 200]),
+])
+def test_attention_rows_of_no_sequence(ops, rows, starts, lens, dtype):
+    """They are zero and reported; the others are as in a call without them."""
+    rng = np.random.default_rng(6)
+    nq, nkv, d = 32, 8, 64
+    pages = -(-max(lens) // 16)
+    cache = dev(random_cache(pages * len(lens), nkv, 16, d, rng))
+    table = i32(np.arange(pages * len(lens)).reshape(len(lens), pages).tolist())
+    q = torch.from_numpy(rng.normal(0, 1, (rows, nq * d)).astype(np.float32)).to(dtype).cuda()
+    status = i32([0])
+    out = torch.full((rows, nq * d), float("nan"), dtype=dtype, device="cuda")
+    ops.attention_kv4(q, cache, table, i32(starts), i32(lens), nq, nkv, d, out=out, status=status)
+    first, end = starts[0], starts[-1]
+    assert (out[:first] == 0).all() and (out[end:] == 0).all() and status.item() == OUT_OF_RANGE
+    if end > first:
+        status.zero_()
+        alone = ops.attention_kv4(q[first:end].clone(), cache, table, i32([x - first for x in starts]), i32(lens), nq,
+                                  nkv, d, status=status)
+        assert status.item() == 0
+        err = (out[first:end].double() - alone.double()).norm() / alone.double().norm()
+        assert err <= (2.0 ** -8 if dtype == torch.bfloat16 else 1e-5)
