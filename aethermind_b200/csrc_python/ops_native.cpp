@@ -17,6 +17,7 @@
 #include <torch/csrc/Exceptions.h>
 #include <torch/csrc/autograd/python_variable.h>
 
+#include <initializer_list>
 #include <stdexcept>
 #include <string>
 
@@ -118,6 +119,13 @@ void kv4(PyObject* cache, PyObject* table, PyObject* start, PyObject* ctx, PyObj
     *b = AmcuKv4Batch{static_cast<const int32_t*>(pt.data_ptr()), n_seq > 1 ? pt.stride(0) : 0, pt.size(1),
                       static_cast<const int32_t*>(rs.data_ptr()), static_cast<const int32_t*>(cl.data_ptr()), n_seq, rows,
                       static_cast<int32_t*>(ptr(st))};
+}
+
+// A call with rows but no sequence: the C ABI touches nothing, the rows are zero and out of range.
+void nowhere(const AmcuKv4Batch& b, PyObject* status, std::initializer_list<at::Tensor> outputs) {
+    if (b.n_seq > 0 || b.rows == 0) return;
+    for (const at::Tensor& t : outputs) t.zero_();
+    if (status != Py_None) THPVariable_Unpack(status).as_strided({1}, {1}).fill_((int64_t)AM_STATUS_OUT_OF_RANGE);
 }
 
 // Runs `f`, turning refusals into ValueError and torch's errors into theirs.
@@ -222,6 +230,7 @@ PyObject* py_append(PyObject*, PyObject* const* a, Py_ssize_t n) {
         s.max_pos = cs.size(0);
         s.n_q_heads = n_q;
         const am_status_code code = f_append(&s, stream_of(here));
+        if (code == AM_STATUS_OK) nowhere(s.batch, a[15], {out});
         return code != AM_STATUS_OK ? PyLong_FromLong(code) : THPVariable_Wrap(std::move(out));
     });
 }
@@ -241,6 +250,7 @@ PyObject* py_gather(PyObject*, PyObject* const* a, Py_ssize_t n) {
         s.v_out = v.data_ptr();
         s.k_out_stride = s.v_out_stride = n_kv * d;
         const am_status_code code = f_gather(&s, stream_of(here));
+        if (code == AM_STATUS_OK) nowhere(s.batch, a[8], {k, v});
         return code != AM_STATUS_OK ? PyLong_FromLong(code) : pair(std::move(k), std::move(v));
     });
 }
@@ -272,6 +282,7 @@ PyObject* py_attention(PyObject*, PyObject* const* a, Py_ssize_t n) {
             s.workspace_size = bytes;
         }
         const am_status_code code = f_attn(&s, stream_of(here));
+        if (code == AM_STATUS_OK) nowhere(s.batch, a[10], {out});
         return code != AM_STATUS_OK ? PyLong_FromLong(code) : THPVariable_Wrap(std::move(out));
     });
 }

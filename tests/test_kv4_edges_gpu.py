@@ -341,3 +341,22 @@ def test_attention_rows_of_no_sequence(ops, rows, starts, lens, dtype):
         assert status.item() == 0
         err = (out[first:end].double() - alone.double()).norm() / alone.double().norm()
         assert err <= (2.0 ** -8 if dtype == torch.bfloat16 else 1e-5)
+
+
+def test_rows_but_no_sequence(ops):
+    d, nq, nkv, rows = 64, 4, 2, 5
+    cache, status = ops.kv4_cache(2, 16, nkv, d), i32([0])
+    x = torch.ones(rows, nq * d, dtype=torch.bfloat16, device="cuda")
+    cs = torch.from_numpy(ref.rope_table(10000.0, d, 64)).cuda()
+    args = (cache, torch.zeros(0, 1, dtype=torch.int32, device="cuda"), i32([0]), i32([]))
+
+    def out():
+        return torch.full((rows, nq * d), float("nan"), dtype=torch.bfloat16, device="cuda")
+
+    for call in (lambda: [ops.attention_kv4(x, *args, nq, nkv, d, out=out(), status=status)],
+                 lambda: ops.kv4_gather(*args, rows, nkv, d, status=status),
+                 lambda: [ops.kv4_append(x, x[:, : nkv * d], x[:, : nkv * d], *args, cs, nq, nkv, d, q_out=out(),
+                                         status=status)]):
+        status.zero_()
+        torch.empty(rows, nq * d, dtype=torch.bfloat16, device="cuda").fill_(float("nan"))  # what fresh memory may hold
+        assert all((t == 0).all() for t in call()) and status.item() == OUT_OF_RANGE
