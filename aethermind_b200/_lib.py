@@ -257,7 +257,7 @@ def native():
         path = Path(__file__).resolve().parent / "lib" / "_ops_native.so"
         if not path.exists():
             raise RuntimeError(f"aethermind_b200 native binding not built ({path}); "
-                               "run `python -m aethermind_b200.build`")
+                               "run `python -m aethermind_b200.build` with a CUDA torch installed")
         loader = importlib.machinery.ExtensionFileLoader("_ops_native", str(path))
         m = importlib.util.module_from_spec(importlib.util.spec_from_loader("_ops_native", loader))
         loader.exec_module(m)

@@ -81,7 +81,13 @@ def _compile(src: Path, hdr: str, verbose: bool) -> Path:
 
 
 def build(verbose: bool = False) -> Path:
+    """The C library, which needs nvcc alone, and the torch extension where there is a torch to build it against."""
+    lib = build_library(verbose)
     build_native()
+    return lib
+
+
+def build_library(verbose: bool = False) -> Path:
     OBJ_DIR.mkdir(exist_ok=True)
     LIB_DIR.mkdir(exist_ok=True)
     hdr = _headers_digest()
@@ -106,12 +112,17 @@ def build(verbose: bool = False) -> Path:
     return LIB
 
 
-def build_native() -> Path:
+def build_native() -> Path | None:
     """The CPython extension lib/_ops_native.so (csrc_python/ops_native.cpp), against
-    the headers of the torch that is installed."""
+    the headers of the torch that is installed; None where there is none with CUDA."""
     import sysconfig
 
-    import torch
+    try:
+        import torch
+    except ImportError:
+        return None
+    if torch.version.cuda is None:
+        return None
     src = PKG / "csrc_python" / "ops_native.cpp"
     base = Path(torch.__file__).resolve().parent
     cmd = [_host_cxx(), "-std=c++20", "-O2", "-fPIC", "-shared", "-fvisibility=hidden",
