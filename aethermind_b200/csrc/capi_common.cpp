@@ -1,4 +1,5 @@
 // Error objects, per-thread last-error message and device queries of the C ABI.
+#include <atomic>
 #include <cuda_runtime.h>
 
 #include <cstdarg>
@@ -36,15 +37,15 @@ am_status_code set_error(am_status_code code, const char* fmt, ...) {
 void clear_error() { g_last_error.clear(); }
 
 int num_sms() {
-    static int per_dev[64] = {};
+    static std::atomic<int> per_dev[64] = {};
     int dev = 0;
     if (cudaGetDevice(&dev) != cudaSuccess || dev < 0 || dev >= 64) return 148;
-    if (per_dev[dev] == 0) {  // benign race: every writer stores the same value
-        int n = 0;
+    int n = per_dev[dev].load(std::memory_order_relaxed);
+    if (n == 0) {  // every writer stores the same value
         if (cudaDeviceGetAttribute(&n, cudaDevAttrMultiProcessorCount, dev) != cudaSuccess || n <= 0) return 148;
-        per_dev[dev] = n;
+        per_dev[dev].store(n, std::memory_order_relaxed);
     }
-    return per_dev[dev];
+    return n;
 }
 
 bool pdl_enabled() {
@@ -65,15 +66,16 @@ void set_func_attr_once(const void* func, cudaFuncAttribute attr, int value) {
 }
 
 int smem_per_sm() {
-    static int per_dev[64] = {};
+    static std::atomic<int> per_dev[64] = {};
     int dev = 0;
     if (cudaGetDevice(&dev) != cudaSuccess || dev < 0 || dev >= 64) return 228 * 1024;
-    if (per_dev[dev] == 0) {  // benign race: every writer stores the same value
-        int v = 0;
-        cudaDeviceGetAttribute(&v, cudaDevAttrMaxSharedMemoryPerMultiprocessor, dev);
-        per_dev[dev] = v > 0 ? v : 228 * 1024;
+    int n = per_dev[dev].load(std::memory_order_relaxed);
+    if (n == 0) {  // every writer stores the same value
+        cudaDeviceGetAttribute(&n, cudaDevAttrMaxSharedMemoryPerMultiprocessor, dev);
+        if (n <= 0) n = 228 * 1024;
+        per_dev[dev].store(n, std::memory_order_relaxed);
     }
-    return per_dev[dev];
+    return n;
 }
 
 int32_t* device_error_word() {
