@@ -6,6 +6,7 @@ import pytest
 torch = pytest.importorskip("torch")
 
 import kv4_reference as ref  # noqa: E402
+import test_kv4_gpu as base  # noqa: E402
 from test_kv4_gpu import bf16, check_attention, dev, di, make_batch, poison_unused, random_cache  # noqa: E402
 
 pytestmark = pytest.mark.gpu
@@ -360,3 +361,72 @@ def test_rows_but_no_sequence(ops):
         status.zero_()
         torch.empty(rows, nq * d, dtype=torch.bfloat16, device="cuda").fill_(float("nan"))  # what fresh memory may hold
         assert all((t == 0).all() for t in call()) and status.item() == OUT_OF_RANGE
+
+
+# ------------------------------------------------------------------ calls that are large enough for other layouts
+@pytest.mark.parametrize("norms", [False, True])
+@pytest.mark.parametrize("dtype", [torch.bfloat16, torch.float32])
+@pytest.mark.parametrize("lens,nq,nkv,d,page", [
+    ([(2100, 2100), (1000, 700), (3, 1), (0, 0), (4000, 3900)], 32, 8, 64, 64),
+    ([(2500, 2500), (900, 77)], 13, 3, 128, 16),             # heads that do not fill a warp's steps
+    ([(9000, 8900), (700, 699), (1, 1)], 5, 1, 64, 256),
+    ([(5000, 4900)], 7, 1, 128, 32),
+])
+def test_append_of_prompts(ops, lens, nq, nkv, d, page, dtype, norms):
+    """The kernel that takes four steps to a warp (rows times steps above 128 an SM), bit for bit without norms."""
+    assert sum(n for _, n in lens) * -(-(nq + 2 * nkv) // (256 // d)) > 128 * 148
+    (base.test_append_with_norms if norms else base.test_append_bit_exact_without_norm)(ops, lens, nq, nkv, d, page, dtype)
+
+
+def rising(lens, nq, nkv, d, exact):
+    """A cache whose scores grow by hundreds along the keys. exact: every key is a whole number of 2^-4 below 2^7, so
+    that 11 bits hold it."""
+    rng = np.random.default_rng(31)
+    page = 64
+    table, start, ctx, total = make_batch(lens, page, rng)
+    kc, kp, vc, vp = random_cache(total, nkv, page, d, rng)
+    if exact:
+        kp[..., 0], kp[..., 1] = 2.0 ** -4, -0.5
+    for b, (c, _) in enumerate(lens):
+        for i in range(c):
+            step = np.round(0.16 * i) / 16 if exact else 0.01 * i
+            kp[table[b, i // page], :, i % page, :, 1] += np.float16(step)
+    q = bf16(np.abs(rng.normal(0, 1, (start[-1], nq * d))))
+    want = ref.attention(q.double().numpy(), (kc, kp, vc, vp), table, start, ctx, nq, nkv, d)
+    return (q.cuda(), dev((kc, kp, vc, vp)), di(table), di(start), di(ctx), nq, nkv, d), want
+
+
+@pytest.mark.parametrize("lens,nq,nkv,d", [([(700, 150)], 32, 8, 128), ([(700, 200), (300, 60)], 32, 8, 64),
+                                           ([(520, 130)], 40, 8, 128)])
+def test_attention_prompts_of_rising_scores(ops, lens, nq, nkv, d):
+    """The softmax reference moves many times in the kernel of prompts. Scores of hundreds in fp32 sums: 2^-13 in the
+    exponent; p to 11 bits and the result to 8: 2^-8."""
+    assert in_the_kernel_of_prompts(lens, nq, nkv)
+    args, want = rising(lens, nq, nkv, d, exact=True)
+    got = ops.attention_kv4(*args).double().cpu().numpy()
+    assert np.linalg.norm(got - want) <= 2.0 ** -8 * np.linalg.norm(want)
+
+
+@pytest.mark.parametrize("exact", [True, False])
+@pytest.mark.parametrize("lens,nq,nkv,d", [([(700, 64)], 32, 8, 128), ([(700, 3), (90, 1)], 32, 8, 64)])
+def test_attention_of_rising_scores(ops, lens, nq, nkv, d, exact):
+    """The same in the kernel of single tokens, whose codes are exact whatever the scale: sums of hundreds to 2^-17 of
+    their largest term are 2^-8 in the exponent, the result 2^-9."""
+    assert not in_the_kernel_of_prompts(lens, nq, nkv)
+    args, want = rising(lens, nq, nkv, d, exact)
+    got = ops.attention_kv4(*args).double().cpu().numpy()
+    assert np.linalg.norm(got - want) <= 2.0 ** -7 * np.linalg.norm(want)
+
+
+@pytest.mark.parametrize("lens,nq,nkv,d,page", [
+    ([(200, 130)], 32, 8, 128, 64),
+    ([(129, 95), (300, 64), (3, 1), (0, 0), (257, 63)], 32, 8, 128, 32),
+    ([(200, 100), (383, 33)], 64, 8, 128, 16),
+    ([(485, 229), (90, 2)], 32, 8, 64, 256),
+    ([(513, 300)], 16, 16, 64, 128),
+    ([(3000, 3000)], 1, 1, 64, 32),     # one q head to a kv head
+    ([(400, 400)], 24, 3, 128, 16),
+])
+def test_attention_in_the_kernel_of_prompts(ops, lens, nq, nkv, d, page):
+    assert in_the_kernel_of_prompts(lens, nq, nkv)
+    base.test_attention_prompts(ops, lens, nq, nkv, d, page)
