@@ -39,13 +39,16 @@ __device__ __forceinline__ float warp_max(float v) {
     return v;
 }
 
-// Streaming 128-bit global load that bypasses L1 allocation (weights are read
-// exactly once per step).
+// Streaming 128-bit global load that bypasses L1 allocation, for data read once. Not
+// the non-coherent form: that wants data which nothing writes while the kernel is
+// resident, and under programmatic dependent launch the kernel that writes it may still
+// be running when this one's CTAs start (they wait in pdl_wait).
 __device__ __forceinline__ uint4 ld_stream_u4(const void* p) {
     uint4 r;
-    asm volatile("ld.global.nc.L1::no_allocate.v4.u32 {%0,%1,%2,%3}, [%4];"
+    asm volatile("ld.global.L1::no_allocate.v4.u32 {%0,%1,%2,%3}, [%4];"
                  : "=r"(r.x), "=r"(r.y), "=r"(r.z), "=r"(r.w)
-                 : "l"(p));
+                 : "l"(p)
+                 : "memory");
     return r;
 }
 __device__ __forceinline__ uint4 ld_u4(const void* p) {

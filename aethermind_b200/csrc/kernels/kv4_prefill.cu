@@ -337,12 +337,12 @@ __global__ void __launch_bounds__(kPfThreads, 1) kv4_prefill_kernel(Kv4AttnParam
                     const uint4* src = reinterpret_cast<const uint4*>(v.kc + kv4_code_off<D>(v, page, kvh, slot));
 #pragma unroll
                     for (int c = 0; c < WPR / 4; ++c) {
-                        const uint4 y = __ldg(src + c);
+                        const uint4 y = src[c];
                         raw[4 * c] = y.x; raw[4 * c + 1] = y.y; raw[4 * c + 2] = y.z; raw[4 * c + 3] = y.w;
                     }
                     const uint32_t* ps = reinterpret_cast<const uint32_t*>(v.kp + kv4_param_off<D>(v, page, kvh, slot));
 #pragma unroll
-                    for (int g = 0; g < G; ++g) par[g] = __ldg(ps + g);
+                    for (int g = 0; g < G; ++g) par[g] = ps[g];
                 }
             };
             int pages = pages_of(0), ahead = pages_of(1);
