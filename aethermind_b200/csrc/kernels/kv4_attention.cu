@@ -45,20 +45,22 @@ namespace amcu {
 // times 2^11 so that it keeps its bits where p is small. The MMA truncates what it adds
 // to an accumulator, so a unit's sums start at 0 and are added to the others' by
 // rounding additions (600 keys, one with nearly all the mass, in one warp: relative
-// error 2.1e-5 without either, 3e-6 with both).
+// error 2.1e-5 without either, 3.7e-6 with both; 64 sequences of 65536 keys: 9.7e-6 and
+// 1.1e-7. Thousands of equal keys under one that has half the mass still lose up to
+// 1e-4, as in any running sum of 32 bits).
 constexpr int kDecWarps = 8;
 constexpr int kDecThreads = kDecWarps * 32;
-constexpr int kDecStages = 4;  // 64 ragged rows: 103.7 us, 105.0 with 5, 106.0 with 6
+constexpr int kDecStages = 4;  // 64 ragged rows: 103.4 us, 103.8 with 3, 104.8 with 5
 constexpr int kDecUnit = 16;       // keys per unit
 // Units of a CTA at least: one for each warp, or what an item has on average where
 // that is less (an item costs a CTA 2 to 5 us whatever its length: one row over 7
-// keys, 8 kv heads of 64, 21.5 us with all items in one CTA, 5.5 with one in each).
+// keys, 8 kv heads of 64, 21.5 us with all items in one CTA, 6.0 with one in each).
 constexpr int kDecMinUnits = 8;
 // A warp takes whole items by itself, without the CTA's merge, where a CTA would
 // have kDecMany or more of them and none is longer than kDecLong units for each of
 // those (a single long one would keep the others waiting). Sequences of one row,
-// 32 / 8 heads of 128, us so / by CTAs: 64 of 20 keys 11 / 20, 128 of 100 17 / 42, 128
-// of 250 24 / 46, 256 of 100 22 / 61, 256 of 300 39 / 81, 256 of 600 60 / 88.
+// 32 / 8 heads of 128, us so / by CTAs: 64 of 20 keys 12 / 17, 128 of 100 20 / 34, 128
+// of 250 23 / 34, 256 of 100 21 / 47, 256 of 300 34 / 65, 256 of 600 55 / 84.
 constexpr int kDecMany = 2, kDecLong = 8;
 constexpr float kLog2e = 1.4426950408889634f;
 constexpr float kDecLift = 3.f;    // scores pass their largest so far by that much (log2) before the reference moves

@@ -62,8 +62,8 @@ struct PfLayout {  // shared memory, bytes
                          oBar = oParV + 2 * kParV;
     // Registers from the dequantising warps to the softmax: 8 x kDqRegs + 8 x (192 -
     // kDqRegs) + 96 = 17 x 96 a lane. As many as neither spills with (2 x 2048 rows
-    // over 8192 keys, 32 / 8 heads: 339 us of d = 128 with 80, 346 with 72; 278 us of
-    // d = 64 with 72, 289 with 80).
+    // over 8192 keys, 32 / 8 heads: 329 us of d = 128 with 80, 345 with 72; 271 us of
+    // d = 64 with 72, 273 with 80).
     static constexpr int kDqRegs = D == 128 ? 80 : 72;
     static constexpr int kTotal = oBar + 256 + 1024;  // + alignment slack
 };
@@ -702,9 +702,15 @@ static void launch_prefill(const Kv4AttnParams& p, unsigned ctas, cudaStream_t s
 bool kv4_prefill_wanted(const Kv4View& v, int64_t grp) {
     // A wave of row tiles (one to an SM) takes about as long as 2.5 eight-column
     // tiles of the other kernel on every SM: this kernel once there are more columns.
-    // Measured (us, this / the other; 32 / 8 heads of 128, one sequence): 4096 keys, 96
-    // rows 90 / 80, 128 rows 91 / 97, 256 rows 89 / 170; 1000 keys, 64 rows 38 / 39, 128
-    // rows 37 / 52. Four sequences of 16 rows over 4096 keys: 81 / 62, of 32: 81 / 97.
+    // Measured (us, this / the other), 32 / 8 heads of 128, one sequence: 4096 keys, 64
+    // rows 76 / 52, 96 rows 77 / 73, 128 rows 77 / 89, 256 rows 77 / 159; 1000 keys, 64
+    // rows 28 / 30, 128 rows 28 / 44; four sequences of 16 rows over 4096 keys 69 / 53, of
+    // 32 70 / 89. Groups of 1, 7 and 8 heads have the same border in columns: 192 rows of
+    // 16 / 16 heads 76 / 73, 128 of 28 / 4 77 / 81, 64 of 64 / 8 78 / 89 (4096 keys).
+    // The rule knows no context, though this kernel takes as long for one row tile as
+    // for a wave of them: 96 rows of 32 / 8 heads over 32768 keys 532 / 378. With heads of
+    // 64 the other kernel is the faster one for up to half as many columns again: 96 rows
+    // over 4096 keys 64 / 49, over 32768 458 / 245, 192 rows 65 / 81 and 459 / 473.
     const int64_t cols = v.rows * grp, tiles = (cols / kPfRows + v.n_seq) * v.nkv, sms = num_sms();
     return ceil_div(cols, 8) * v.nkv * 2 > 5 * sms * ceil_div(tiles, sms);
 }

@@ -277,8 +277,8 @@ struct SampleTeam {
 // Bound by latency (exchanges of the cluster, barriers) and, without top-k, by
 // the instructions per token (22 for the mass, 30 and two shared atomics for the
 // histogram). The next row of these SMs is fetched into L2 meanwhile. 192 fp32
-// rows of 128256: 45 us if all are greedy, 88 with top-k 40, 92 with the
-// temperature alone, 178 with top-p 0.95, 165 with top-k 1000. Before the
+// rows of 128256: 38 us if all are greedy, 80 with top-k 40, 85 with the
+// temperature alone, 173 with top-p 0.95, 162 with top-k 1000. Before the
 // division without a branch, split sums, copies of the histogram and the
 // drawn run walked by a warp: 50, 91, 139, 265, 227.
 template <typename T, bool kRes>
