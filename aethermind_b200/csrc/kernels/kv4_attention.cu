@@ -438,20 +438,21 @@ __global__ void __launch_bounds__(kDecThreads, 2) kv4_decode_kernel(Kv4AttnParam
                         vm[hh][g] &= keep;
                     }
                 }
-                // A group of V that is NaN (its minimum is) may be of a key that only some columns
-                // see: 0 times it would reach the others. It goes into the sums of those that do.
+                // A group of V that is NaN (its minimum or scale is) may be of a key that only some
+                // columns see: 0 times it would reach the others. It goes into the sums of those that do.
                 uint32_t odd = 0;
 #pragma unroll
                 for (int hh = 0; hh < 2; ++hh)
 #pragma unroll
-                    for (int g = 0; g < G; ++g) odd |= __hneu2_mask(u2h(vm[hh][g]), u2h(vm[hh][g]));
+                    for (int g = 0; g < G; ++g) odd |= __hneu2_mask(u2h(vm[hh][g]), u2h(vm[hh][g])) | __hneu2_mask(u2h(vs[hh][g]), u2h(vs[hh][g]));
                 if (__any_sync(0xffffffffu, odd != 0)) {
 #pragma unroll
                     for (int hh = 0; hh < 2; ++hh)
 #pragma unroll
                         for (int g = 0; g < G; ++g) {
-                            const uint32_t nan = __hneu2_mask(u2h(vm[hh][g]), u2h(vm[hh][g]));
+                            const uint32_t nan = __hneu2_mask(u2h(vm[hh][g]), u2h(vm[hh][g])) | __hneu2_mask(u2h(vs[hh][g]), u2h(vs[hh][g]));
                             vm[hh][g] &= ~nan;
+                            vs[hh][g] &= ~nan;
                             // the first such key of the eight (lanes of equal t hold the same two)
                             int at = 0x7fffffff;
                             if (nan) at = u * kDecUnit + 2 * t + 8 * hh + (nan & 0xffffu ? 0 : 1);

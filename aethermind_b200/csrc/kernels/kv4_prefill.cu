@@ -25,12 +25,13 @@
 // m + s c in fp16: (1024 + c) - 1024 exactly, then one fused multiply-add
 // rounded once to 11 bits (an element beyond fp16 becomes 65504).
 //
-// The softmax reference of a row lies 2^7 to 2^8 below the largest score when it is
-// set and moves only when a score passes that by 2^8 more (p, in fp16, is then 2^15),
-// and to a whole power of two: the sum, O and what the tile has of P already are then
-// rescaled without a rounding (P where it stays normal). So the scores are read once, without knowing their tile's
-// maximum first. (With the reference at the largest score itself p of 2^-20 kept 4
-// bits: 3% of a row of many such keys under one that has most of the mass.)
+// The softmax reference of a row lies 2^6 to 2^7 below the largest score when it is
+// set, and moves only when a score passes it by 2^15 (p is in fp16), and to a whole
+// power of two: the sum, O and what the tile has of P already are then rescaled
+// without a rounding (P where it stays normal). So the scores are read once, without
+// knowing their tile's maximum first. (With the reference at the largest score itself
+// p of 2^-20 kept 4 bits: 3% of a row of many such keys under one that has most of the
+// mass.)
 //
 // Waits are bounded: one that runs out records an error code, and the CTA goes
 // through its control flow without waiting again.
@@ -47,7 +48,7 @@ constexpr int32_t kErrKv4Wait = 0x501;
 constexpr float kPfLog2e = 1.4426950408889634f;
 // A score may pass the largest so far by kPfLift before the reference moves, to
 // kPfHead below the new largest: p is up to 2^15, and an fp16 normal, rounded to 11 bits,
-// down to 2^-20 of the largest one (2^-32 is still counted).
+// down to 2^-20 of the largest one (2^-31 is still counted).
 constexpr float kPfLift = 8.f, kPfHead = 7.f;
 
 template <int D>
@@ -443,8 +444,10 @@ __global__ void __launch_bounds__(kPfThreads, 1) kv4_prefill_kernel(Kv4AttnParam
                     const bool big = !__hblt2(top, pf_u2h(0x7c007c00u));  // beyond fp16, or NaN
                     // a NaN becomes 65504 below, as 0 times it would reach rows that do not see the
                     // key; those that do take their NaN at the end (each thread looks at one token)
-                    if (big && (lds_u32(ps + q8 * (4 * G) + 4 * g) & 0x7fff0000u) > 0x7c000000u)
-                        atomicMin(&s_nan[g], j * kPfKeys + 8 * tg + q8);
+                    if (big) {
+                        const __half2 par = pf_u2h(lds_u32(ps + q8 * (4 * G) + 4 * g));
+                        if (__hneu2_mask(par, par)) atomicMin(&s_nan[g], j * kPfKeys + 8 * tg + q8);
+                    }
                     uint32_t cw[8];
 #pragma unroll
                     for (int i = 0; i < 8; ++i) cw[i] = lds_u32(src + i * (D / 2) + 4 * g);

@@ -137,6 +137,7 @@ def test_append_of_groups_that_are_no_numbers(ops, d, steps, dtype):
 
 
 @pytest.mark.parametrize("dtype", [torch.bfloat16, torch.float32])
+@pytest.mark.parametrize("pair", [(0, np.nan), (np.nan, 0.5)])  # scale and minimum of a group that is no number
 @pytest.mark.parametrize("lens,at,nq,nkv,d", [
     ([(40, 5), (40, 5)], 37, 8, 2, 128),   # rows 0 and 1 of five do not see it
     ([(40, 5), (40, 5)], 3, 8, 2, 64),
@@ -147,7 +148,7 @@ def test_append_of_groups_that_are_no_numbers(ops, d, steps, dtype):
     ([(400, 190), (300, 20)], 399, 32, 8, 64),
     ([(300, 160)], 5, 32, 8, 128),
 ])
-def test_attention_over_keys_and_values_that_are_no_numbers(ops, lens, at, nq, nkv, d, dtype):
+def test_attention_over_keys_and_values_that_are_no_numbers(ops, lens, at, nq, nkv, d, pair, dtype):
     """A NaN key is in every element of the rows that see it, a NaN group of a value in its 64 elements of them, and
     neither is in another row, head or sequence."""
     rng = np.random.default_rng(11)
@@ -164,7 +165,7 @@ def test_attention_over_keys_and_values_that_are_no_numbers(ops, lens, at, nq, n
             continue
         page, slot = table[b, at // 16], at % 16
         for par, h, i in ((kp, kh, 0), (vp, vh, g)):
-            par[page, h, slot, i] = (0, np.nan)
+            par[page, h, slot, i] = pair
         for r in range(start[b], start[b + 1]):
             if ctx[b] - start[b + 1] + r >= at:
                 heads[r, kh * grp:(kh + 1) * grp] = np.nan
